@@ -341,6 +341,64 @@ LB2_API int32_t lb2_attention_bwd(void* dq, void* dk, void* dv, void* dbias, con
                                   const void* k, const void* v, int32_t causal, double scale, const lb2_attention_dims* dims,
                                   int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- windowed attention, relative position bias ---------------------------------------------------- */
+/* Buckets of relative positions for a learned bias (no counterpart in the reference; it feeds the bias of
+ * scaled_dot_product_attention, lib/LuxLib/src/impl/attention.jl:76-118). Bucket j holds the distances from first[j] (first[0] = 0, not
+ * falling) up to the next bucket's start; the last one all that follow. bidirectional = 0: the distance of key s from query l is
+ * max(l - s, 0); 1: |l - s|, and keys after the query have `count` buckets of their own behind the others. A table has one column of
+ * `heads` values per bucket: (heads, count or 2 count), the weight of Lux's Embedding(buckets => heads). */
+#define LB2_MAX_REL_BUCKETS 64
+typedef struct lb2_rel_buckets {
+  int32_t count;
+  int32_t bidirectional;
+  int32_t first[LB2_MAX_REL_BUCKETS];
+} lb2_rel_buckets;
+
+/* bias[s, l, h] = table[h, bucket(s - l - offset)] as a (keys, queries, heads) array, offset = the first query's position; backward:
+ * dtable[h, j] = sum over the pairs of bucket j and over the B samples of dbias (keys, queries, heads, B), fixed order. No counterpart in
+ * the reference. */
+LB2_API int32_t lb2_relpos_bias_fwd(void* bias, const void* table, const lb2_rel_buckets* buckets, int64_t keys, int64_t queries,
+                                    int64_t heads, int64_t offset, int32_t dtype, void* stream);
+LB2_API size_t lb2_relpos_bias_bwd_workspace_bytes(const lb2_rel_buckets* buckets, int64_t keys, int64_t queries, int64_t heads, int64_t B);
+LB2_API int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_buckets* buckets, int64_t keys, int64_t queries,
+                                    int64_t heads, int64_t B, int64_t offset, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* Attention over a sliding window and a few first tokens: scaled_dot_product_attention (lib/LuxLib/src/impl/attention.jl:5-131; the
+ * window has no counterpart in the reference) with query l seeing key s where |l - s| < window or s < sinks, s <= l if causal, and
+ * neither is at or past lengths[b] (device array; NULL: all tokens count), without the weights in memory. Layouts as in
+ * lb2_attention_fwd: q (head_dim, heads, queries, batch), k, v -> x (value_dim, heads, queries, batch); logits = scale * k'q, plus
+ * table[h, bucket(s - l)] unless table and buckets are NULL. A query that sees nothing gives a zero row; keys that it does not see
+ * do not reach it, infinities and NaN among them. head_dim and value_dim up to 256.
+ * stats (2, queries, heads, batch), fp32, for the backward call: each softmax's maximum and the log of its sum relative to that (0 and
+ * +inf for a query that sees nothing); NULL: not kept.
+ * Backward: dq, dk, dv, and dtable (NULL without a table), zero for tokens past lengths[b]; every sum has a fixed order. */
+typedef struct lb2_window_dims {
+  int64_t head_dim, value_dim, heads, kv_heads, queries, keys, batch, window, sinks, causal;
+} lb2_window_dims;
+LB2_API int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const void* k, const void* v, const void* table,
+                                         const lb2_rel_buckets* buckets, const int32_t* lengths, double scale,
+                                         const lb2_window_dims* dims, int32_t dtype, void* stream);
+LB2_API size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* dims, const lb2_rel_buckets* buckets, int32_t dtype);
+LB2_API int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const float* stats,
+                                         const void* q, const void* k, const void* v, const void* table, const lb2_rel_buckets* buckets,
+                                         const int32_t* lengths, double scale, const lb2_window_dims* dims, int32_t dtype,
+                                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* One new token per sequence over a ring cache (no counterpart in the reference; the attention is that of
+ * lib/LuxLib/src/impl/attention.jl:76-118, causal). dims->keys is the cache's capacity: kcache (head_dim, kv_heads, capacity, batch),
+ * vcache (value_dim, kv_heads, capacity, batch); position p lies in slot p while p < sinks, then in sinks + (p - sinks) mod
+ * (capacity - sinks). capacity >= sinks + window. lengths[b] tokens are in the cache; the new one, at position lengths[b], is put there
+ * and attends: q (head_dim, heads, batch), k, v of kv_heads -> x (value_dim, heads, batch). lengths[b] < 0: no sequence in that place,
+ * x = 0 and the cache stays. lengths itself is not changed. dims->queries and dims->causal are not read. */
+LB2_API int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, const void* q, const void* k, const void* v,
+                                          const void* table, const lb2_rel_buckets* buckets, const int32_t* lengths, double scale,
+                                          const lb2_window_dims* dims, int32_t dtype, void* stream);
+/* Puts the tokens of k (head_dim, kv_heads, keys, batch) and v that a cache of `capacity` slots holds after lengths[b] of them (NULL: all
+ * keys) into their slots; the other slots stay. No counterpart in the reference. */
+LB2_API int32_t lb2_window_cache_fill(void* kcache, void* vcache, const void* k, const void* v, const int32_t* lengths, int64_t capacity,
+                                      const lb2_window_dims* dims, int32_t dtype, void* stream);
+
 /* ---- Scale layer ------------------------------------------------------------------------------- */
 /* y = act.(x .* weight .+ bias) (src/layers/basic.jl:452-461; the {False} method has no bias: bias = NULL) with
  * weight / bias of the layer's dims and x of shape (dims..., batch...): a (D, B) column-major view, D = prod(dims).

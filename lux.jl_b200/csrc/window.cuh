@@ -1,0 +1,172 @@
+// Windowed attention: what its kernels share. Which keys a query sees, the bias of a relative position, and the rows that are
+// computed again one key at a time where an infinity or NaN was met.
+//
+// Query l and key s (positions of one sequence of n tokens, n = lengths[b] or all) see each other when
+//   l < n, s < n,  s <= l if causal,  |l - s| < window or s < sinks.
+// z[s, l] = scale * k_s . q_l + table[h, bucket(s - l)],  p = softmax of z over the visible s (nothing visible: all zero).
+#pragma once
+#include "common.cuh"
+
+namespace lb2 {
+
+int32_t check_rel_buckets(const lb2_rel_buckets* t);   // relpos.cu
+
+constexpr int kWinMaxBuckets = LB2_MAX_REL_BUCKETS;   // per side
+
+struct WinParams {
+  const void *q, *k, *v, *table;
+  const int32_t* lengths;
+  int D, E, H, Hkv, rep, L, S, B;
+  int window, sinks, causal;
+  float scale;
+  lb2_rel_buckets buckets;    // count = 0: no bias
+};
+
+__device__ __forceinline__ int win_tokens(const WinParams& p, int b, int n) {
+  return p.lengths == nullptr ? n : max(0, min(n, p.lengths[b]));
+}
+// The keys that some query of [l0, l1) sees: [0, sinks) and [lo, hi), lo >= sinks.
+__device__ __forceinline__ void win_key_range(const WinParams& p, int l0, int l1, int keys, int* sinks, int* lo, int* hi) {
+  *hi = p.causal ? min(keys, l1) : keys;
+  *sinks = min(p.sinks, *hi);
+  if (!p.causal) *hi = min(keys, l1 - 1 + p.window);
+  *lo = max(*sinks, l0 - p.window + 1);
+}
+// The queries that see some key of [s0, s1).
+__device__ __forceinline__ void win_query_range(const WinParams& p, int s0, int s1, int queries, int* lo, int* hi) {
+  *lo = p.causal ? s0 : (s0 < p.sinks ? 0 : max(0, s0 - p.window + 1));
+  *hi = s0 < p.sinks ? queries : min(queries, s1 - 1 + p.window);
+}
+__device__ __forceinline__ bool win_sees(const WinParams& p, int l, int s) {
+  if (p.causal && s > l) return false;
+  return abs(l - s) < p.window || s < p.sinks;
+}
+// the keys of [0, keys) that query l sees are not none
+__device__ __forceinline__ bool win_any(const WinParams& p, int l, int keys) {
+  int sinks, lo, hi;
+  win_key_range(p, l, l + 1, keys, &sinks, &lo, &hi);
+  return sinks > 0 || lo < hi;
+}
+
+// bucket of the relative position rel = s - l: the last one that starts at or below the distance
+__device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, int rel) {
+  const int dist = t.bidirectional ? abs(rel) : max(-rel, 0);
+  int lo = 0, n = t.count;                  // invariant: first[lo] <= dist, the answer lies in [lo, lo + n)
+  while (n > 1) {
+    const int half = n >> 1;
+    if (t.first[lo + half] <= dist) { lo += half; n -= half; } else { n = half; }
+  }
+  return lo + (t.bidirectional && rel > 0 ? t.count : 0);
+}
+template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, int h, int rel) {
+  return to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, rel)]);
+}
+
+// ---- rows once more ---------------------------------------------------------------------------
+// A tile's products multiply the weights that the mask made zero with whatever the array holds there: an infinity or NaN in a
+// place that the row does not see would reach it. Rows whose results are not finite are therefore computed again by one warp over
+// the visible keys (or queries) alone. Lane i holds features i, i + 32, ...
+constexpr int kWinMaxDim = 256;
+constexpr int kWinLaneDims = kWinMaxDim / 32;
+template <typename T> __device__ __forceinline__ void win_load_lane(const T* row, int n, int lane, float (&v)[kWinLaneDims]) {
+#pragma unroll
+  for (int i = 0; i < kWinLaneDims; ++i) v[i] = lane + 32 * i < n ? to_f32(row[lane + 32 * i]) : 0.f;
+}
+template <typename T> __device__ __forceinline__ void win_store_lane(T* row, int n, int lane, const float (&v)[kWinLaneDims]) {
+#pragma unroll
+  for (int i = 0; i < kWinLaneDims; ++i)
+    if (lane + 32 * i < n) row[lane + 32 * i] = from_f32<T>(v[i]);
+}
+// dot of n features; lanes past them hold zeros on both sides
+__device__ __forceinline__ float win_dot_lane(const float (&a)[kWinLaneDims], const float (&b)[kWinLaneDims], int n) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWinLaneDims; ++i)
+    if (32 * i < n) s = fmaf(a[i], b[i], s);
+  return warp_sum(s);
+}
+template <typename T> __device__ __forceinline__ const T* win_q_row(const WinParams& p, const void* base, int n, int l, int h, int b) {
+  return static_cast<const T*>(base) + (((int64_t)b * p.L + l) * p.H + h) * n;
+}
+template <typename T> __device__ __forceinline__ const T* win_kv_row(const WinParams& p, const void* base, int n, int s, int g, int b) {
+  return static_cast<const T*>(base) + (((int64_t)b * p.S + s) * p.Hkv + g) * n;
+}
+
+// stats of a row: the maximum m of its logits and log(sum of exp(z - m)), apart: m + log(sum) would lose the sum beside an m as large
+// as the type's lowest value. p = exp((z - m) - log(sum)); a row that sees nothing has (0, inf).
+template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, float2* stats, int l, int h, int b, int keys) {
+  const int lane = threadIdx.x & 31, g = h / p.rep;
+  float q[kWinLaneDims], t[kWinLaneDims], o[kWinLaneDims] = {};
+  win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, q);
+  float m = -INFINITY, sum = 0.f;
+  int sinks, lo, hi;
+  win_key_range(p, l, l + 1, keys, &sinks, &lo, &hi);
+  for (int i0 = 0, n = sinks + max(0, hi - lo); i0 < n; ++i0) {
+    const int s = i0 < sinks ? i0 : lo + (i0 - sinks);
+    win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
+    float z = win_dot_lane(q, t, p.D) * p.scale;
+    if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
+    const float mn = fmaxf(m, z), ref = mn == -INFINITY ? 0.f : mn;
+    const float keep = expf(m - ref), w = expf(z - ref);
+    win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, t);
+#pragma unroll
+    for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(w, t[i], o[i] * keep);
+    sum = sum * keep + w;
+    m = mn;
+  }
+#pragma unroll
+  for (int i = 0; i < kWinLaneDims; ++i) o[i] /= sum;
+  win_store_lane(x + (((int64_t)b * p.L + l) * p.H + h) * p.E, p.E, lane, o);
+  if (stats != nullptr && lane == 0) *stats = make_float2(m, logf(sum));
+}
+
+// stats, delta: of query l, head h
+template <typename T>
+__device__ __noinline__ void win_row_dq(const WinParams& p, T* dq, const void* dx, float2 stats, float delta, int l, int h, int b, int keys) {
+  const int lane = threadIdx.x & 31, g = h / p.rep;
+  float q[kWinLaneDims], go[kWinLaneDims], t[kWinLaneDims], u[kWinLaneDims], o[kWinLaneDims] = {};
+  win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, q);
+  win_load_lane(win_q_row<T>(p, dx, p.E, l, h, b), p.E, lane, go);
+  int sinks, lo, hi;
+  win_key_range(p, l, l + 1, keys, &sinks, &lo, &hi);
+  for (int i0 = 0, n = sinks + max(0, hi - lo); i0 < n; ++i0) {
+    const int s = i0 < sinks ? i0 : lo + (i0 - sinks);
+    win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
+    win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, u);
+    float z = win_dot_lane(q, t, p.D) * p.scale;
+    if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
+    const float ds = expf((z - stats.x) - stats.y) * (win_dot_lane(go, u, p.E) - delta) * p.scale;
+#pragma unroll
+    for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(ds, t[i], o[i]);
+  }
+  win_store_lane(dq + (((int64_t)b * p.L + l) * p.H + h) * p.D, p.D, lane, o);
+}
+
+// stats, delta: [batch][head][query]
+template <typename T>
+__device__ __noinline__ void win_row_dkv(const WinParams& p, T* dk, T* dv, const void* dx, const float2* stats, const float* delta, int s, int g,
+                                         int b, int queries) {
+  const int lane = threadIdx.x & 31;
+  float k[kWinLaneDims], v[kWinLaneDims], t[kWinLaneDims], u[kWinLaneDims], ok[kWinLaneDims] = {}, ov[kWinLaneDims] = {};
+  win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, k);
+  win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, v);
+  int lo, hi;
+  win_query_range(p, s, s + 1, queries, &lo, &hi);
+  for (int j = 0; j < p.rep; ++j) {
+    const int h = g * p.rep + j;
+    for (int l = lo; l < hi; ++l) {
+      win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, t);
+      win_load_lane(win_q_row<T>(p, dx, p.E, l, h, b), p.E, lane, u);
+      float z = win_dot_lane(t, k, p.D) * p.scale;
+      if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
+      const int64_t at = ((int64_t)b * p.H + h) * p.L + l;
+      const float w = expf((z - stats[at].x) - stats[at].y), ds = w * (win_dot_lane(u, v, p.E) - delta[at]) * p.scale;
+#pragma unroll
+      for (int i = 0; i < kWinLaneDims; ++i) { ov[i] = fmaf(w, u[i], ov[i]); ok[i] = fmaf(ds, t[i], ok[i]); }
+    }
+  }
+  win_store_lane(dk + (((int64_t)b * p.S + s) * p.Hkv + g) * p.D, p.D, lane, ok);
+  win_store_lane(dv + (((int64_t)b * p.S + s) * p.Hkv + g) * p.E, p.E, lane, ov);
+}
+
+}  // namespace lb2

@@ -9,7 +9,9 @@ from .ops import (ConvDims, PoolDims, add_activation, batchnorm, bias_activation
                   needs_preactivation, rrule_add_activation, rrule_batchnorm, rrule_bias_activation, rrule_fused_conv,
                   rrule_fused_dense, rrule_groupnorm, rrule_instancenorm, rrule_layernorm, rrule_maxpool, rrule_meanpool, mse_loss,
                   rrule_mse_loss, conv_transpose_bias_activation, rrule_conv_transpose, conv_transpose_output_size, scale, rrule_scale, cross_entropy_loss, rrule_cross_entropy_loss, batched_matmul, rrule_batched_matmul,
-                  scaled_dot_product_attention, rrule_scaled_dot_product_attention, rrule_conv_batchnorm)
+                  scaled_dot_product_attention, rrule_scaled_dot_product_attention, rrule_conv_batchnorm,
+                  RelativeBuckets, relative_position_bias, rrule_relative_position_bias, windowed_attention, rrule_windowed_attention,
+                  windowed_attention_step, windowed_cache_fill)
 
 __all__ = [
     "ArgumentError", "DimensionMismatch", "LuxLibB200Error", "ConvDims", "PoolDims",
@@ -19,4 +21,6 @@ __all__ = [
     "rrule_fused_dense", "rrule_fused_conv", "rrule_batchnorm", "rrule_groupnorm", "rrule_instancenorm", "rrule_layernorm", "maxpool", "meanpool", "rrule_maxpool", "rrule_meanpool",
     "rrule_bias_activation", "mse_loss", "rrule_mse_loss", "conv_transpose_bias_activation", "rrule_conv_transpose", "conv_transpose_output_size", "scale", "rrule_scale", "cross_entropy_loss", "rrule_cross_entropy_loss", "batched_matmul", "rrule_batched_matmul",
     "scaled_dot_product_attention", "rrule_scaled_dot_product_attention", "rrule_conv_batchnorm",
+    "RelativeBuckets", "relative_position_bias", "rrule_relative_position_bias", "windowed_attention", "rrule_windowed_attention",
+    "windowed_attention_step", "windowed_cache_fill",
 ]

@@ -46,6 +46,18 @@ class AttentionDims(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("head_dim", "value_dim", "heads", "kv_heads", "queries", "keys", "batch")]
 
 
+class WindowDims(C.Structure):
+    """lb2_window_dims"""
+    _fields_ = [(n, C.c_int64) for n in ("head_dim", "value_dim", "heads", "kv_heads", "queries", "keys", "batch", "window", "sinks", "causal")]
+
+
+MAX_REL_BUCKETS = 64
+
+
+class RelBuckets(C.Structure):
+    """lb2_rel_buckets"""
+    _fields_ = [("count", C.c_int32), ("bidirectional", C.c_int32), ("first", C.c_int32 * MAX_REL_BUCKETS)]
+
 
 class OptLeaf(C.Structure):
     """lb2_opt_leaf"""
@@ -107,6 +119,15 @@ PROTOTYPES = {
     "lb2_attention_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i32, _dbl, C.POINTER(AttentionDims), _i32, _p, _sz, _p]),
     "lb2_attention_bwd_workspace_bytes": (_sz, [C.POINTER(AttentionDims), _i32]),
     "lb2_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _dbl, C.POINTER(AttentionDims), _i32, _p, _sz, _p]),
+    "lb2_relpos_bias_fwd": (_i32, [_p, _p, C.POINTER(RelBuckets), _i64, _i64, _i64, _i64, _i32, _p]),
+    "lb2_relpos_bias_bwd_workspace_bytes": (_sz, [C.POINTER(RelBuckets), _i64, _i64, _i64, _i64]),
+    "lb2_relpos_bias_bwd": (_i32, [_p, _p, C.POINTER(RelBuckets), _i64, _i64, _i64, _i64, _i64, _i32, _p, _sz, _p]),
+    "lb2_window_attention_fwd": (_i32, [_p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32, _p]),
+    "lb2_window_attention_bwd_workspace_bytes": (_sz, [C.POINTER(WindowDims), C.POINTER(RelBuckets), _i32]),
+    "lb2_window_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32,
+                                        _p, _sz, _p]),
+    "lb2_window_attention_step": (_i32, [_p, _p, _p, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32, _p]),
+    "lb2_window_cache_fill": (_i32, [_p, _p, _p, _p, _p, _i64, C.POINTER(WindowDims), _i32, _p]),
     "lb2_conv_fwd_sums_is_fused": (_i32, [_p, _i32]),
     "lb2_conv_fwd_sums_workspace_bytes": (_sz, [_p, _i32]),
     "lb2_conv_fwd_sums": (_i32, [_p, _fp, _p, _p, _p, _i32, C.c_uint32, _p, _sz, _p]),

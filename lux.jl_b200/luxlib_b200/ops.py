@@ -10,6 +10,7 @@ Arrays are column-major device arrays (see arrays.py); activations are named by 
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 import functools
 import math
@@ -21,7 +22,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ArgumentError, DimensionMismatch
-from .arrays import as_colmajor, current_stream, dtype_code, jl_empty, jl_reshape, ptr, workspace
+from .arrays import as_colmajor, current_stream, dtype_code, is_colmajor, jl_empty, jl_reshape, ptr, workspace
 
 # --------------------------------------------------------------------------------------------
 # activations
@@ -759,14 +760,18 @@ def rrule_scaled_dot_product_attention(q, k, v, *, scale=None, mask=None, is_cau
     causal = 1 if is_causal else 0
     bias_c = mask_c = None
     bias_bs = mask_bs = 0
+    shared = None                # a bias per head that all samples share (relative_position_bias): its shape
     if bias is not None:
-        bias_c = as_colmajor(bias.to(Q.dtype))
+        bias_c = bias.to(Q.dtype)
+        if Bn > 1 and tuple(bias_c.shape) == (S, Lq, H) + (1,) * len(batch_shape):
+            shared, bias_c = tuple(bias_c.shape), bias_c.expand((S, Lq, H) + batch_shape)
+        bias_c = as_colmajor(bias_c)
         if tuple(bias_c.shape) == (S, Lq):
             bias_bs = 0
         elif tuple(bias_c.shape) == (S, Lq, H) + batch_shape:
             bias_bs = S * Lq
         else:
-            raise DimensionMismatch("bias must have the shape (S, L) or (S, L, H, B...)")
+            raise DimensionMismatch("bias must have the shape (S, L), (S, L, H, 1...) or (S, L, H, B...)")
     if mask is not None:
         mask_c = as_colmajor(mask.to(torch.uint8))
         if tuple(mask_c.shape) == (S, Lq):
@@ -801,6 +806,11 @@ def rrule_scaled_dot_product_attention(q, k, v, *, scale=None, mask=None, is_cau
             _, wsp, wsn = _ws(_query("lb2_bias_act_bwd_workspace_bytes", device.index, 1, S * Lq, H * Bn), device)
             _cabi.check(lib.lb2_bias_act_bwd(None, ptr(db), ptr(full), None, None, 1, S * Lq, H * Bn, dt, act_code("identity"), wsp, wsn,
                                              current_stream(device)))
+        if shared is not None:   # ... or by the samples alone
+            full, db = db, jl_empty(shared, Q.dtype, device)
+            _, wsp, wsn = _ws(_query("lb2_bias_act_bwd_workspace_bytes", device.index, 1, S * Lq * H, Bn), device)
+            _cabi.check(lib.lb2_bias_act_bwd(None, ptr(db), ptr(full), None, None, 1, S * Lq * H, Bn, dt, act_code("identity"), wsp, wsn,
+                                             current_stream(device)))
         return dq, dk, dv, db
 
     return (out, w), pullback
@@ -809,6 +819,263 @@ def rrule_scaled_dot_product_attention(q, k, v, *, scale=None, mask=None, is_cau
 def scaled_dot_product_attention(q, k, v, **kw):
     """(x, attention weights) of LuxLib.scaled_dot_product_attention for head_dim = 1, token_dim = 3."""
     return rrule_scaled_dot_product_attention(q, k, v, **kw)[0]
+
+
+# --------------------------------------------------------------------------------------------
+# windowed attention, relative position bias
+# --------------------------------------------------------------------------------------------
+@dataclass(frozen=True)
+class RelativeBuckets:
+    """Buckets of relative positions (key - query) for a learned bias. Bucket j of a side holds the distances from first[j] up to
+    the next bucket's start, the last one all that follow. bidirectional: keys after the query have buckets of their own, behind the
+    others; else their distance counts as 0. A bias table is the weight of Embedding(len(buckets) => heads): (heads, len(buckets))."""
+    first: Tuple[int, ...]
+    bidirectional: bool = True
+
+    def __post_init__(self):
+        f = tuple(int(d) for d in self.first)
+        object.__setattr__(self, "first", f)
+        if not 1 <= len(f) <= _cabi.MAX_REL_BUCKETS:
+            raise ArgumentError(f"1 to {_cabi.MAX_REL_BUCKETS} buckets per side, not {len(f)}")
+        if f[0] != 0 or any(b < a for a, b in zip(f, f[1:])) or f[-1] >= 2 ** 31:
+            raise ArgumentError("the buckets' first distances start at 0, do not fall and stay below 2^31")
+
+    @staticmethod
+    def make(num_buckets: int, max_distance: int, bidirectional: bool = True) -> "RelativeBuckets":
+        """`num_buckets` in all (bidirectional: half of them per side): one distance each for the first half e of a side's n, then
+        logarithmic: bucket e + j starts at the smallest d with log(d / e) / log(max_distance / e) * (n - e) >= j, decided in
+        whole numbers."""
+        n = int(num_buckets)
+        if bidirectional:
+            if n % 2:
+                raise ArgumentError("bidirectional buckets come in pairs")
+            n //= 2
+        if not 1 <= n <= _cabi.MAX_REL_BUCKETS:
+            raise ArgumentError(f"1 to {_cabi.MAX_REL_BUCKETS} buckets per side, not {n}")
+        e, top = n // 2, int(max_distance)
+        if n > 1 and not e < top < 2 ** 31:
+            raise ArgumentError(f"max_distance must exceed the {e} exact distances")
+        return RelativeBuckets(_bucket_starts(n, e, top), bool(bidirectional))
+
+    def __len__(self):
+        return len(self.first) * (2 if self.bidirectional else 1)
+
+    def bucket(self, rel: int) -> int:
+        """The bucket of the relative position `rel` = key - query."""
+        dist = abs(rel) if self.bidirectional else max(-rel, 0)
+        return bisect.bisect_right(self.first, dist) - 1 + (len(self.first) if self.bidirectional and rel > 0 else 0)
+
+
+@functools.lru_cache(maxsize=256)
+def _bucket_starts(n: int, e: int, top: int):
+    starts = list(range(max(e, 1)))
+    for j in range(len(starts) - e, n - e):
+        lo, hi = e, top                               # the smallest d of [e, top] with (d / e)^(n-e) >= (top / e)^j
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** (n - e) * e ** j >= top ** j * e ** (n - e):
+                hi = mid
+            else:
+                lo = mid + 1
+        starts.append(lo)
+    return tuple(starts)
+
+
+@functools.lru_cache(maxsize=256)
+def _buckets_struct(buckets: RelativeBuckets):
+    t = _cabi.RelBuckets(len(buckets.first), int(buckets.bidirectional))
+    t.first[:len(buckets.first)] = buckets.first
+    return t
+
+
+def _on_one_device(**tensors):
+    """All on one CUDA device, which is returned: a host pointer would be read by the kernels as a device address."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device.type != "cuda" or (device is not None and t.device != device):
+            raise ArgumentError(f"{name} must be on the CUDA device of the other arrays, not on {t.device}")
+        device = t.device
+    return device
+
+
+def _launch(device, name, *args):
+    """The entry point `name` on the arrays' device, whichever is current, on its current stream."""
+    lib = _cabi.load()
+    if device.index == torch.cuda.current_device():
+        _cabi.check(getattr(lib, name)(*args, current_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            _cabi.check(getattr(lib, name)(*args, current_stream(device)))
+
+
+def _table_of(table, buckets, heads: int):
+    """The bias table as the library takes it, and its buckets' descriptor."""
+    if (table is None) != (buckets is None):
+        raise ArgumentError("table and buckets must both be given or both be nothing")
+    if table is None:
+        return None, None
+    if tuple(table.shape) != (heads, len(buckets)):
+        raise DimensionMismatch(f"the bias table must have the shape (heads, buckets) = ({heads}, {len(buckets)}), not {tuple(table.shape)}")
+    return as_colmajor(table), C.byref(_buckets_struct(buckets))
+
+
+def relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: int, *, offset: int = 0):
+    """bias[s, l, h, 1] = table[h, bucket(s - l - offset)] for key s and query l: the bias of scaled_dot_product_attention, the same
+    for all samples. `offset` is the first query's position."""
+    if table.dim() != 2:
+        raise DimensionMismatch("the bias table must be a matrix (heads, buckets)")
+    S, Lq, H = int(keys), int(queries), table.shape[0]
+    device = _on_one_device(table=table)
+    T, plan = _table_of(table, buckets, H)
+    bias = jl_empty((S, Lq, H, 1), T.dtype, device)
+    _launch(device, "lb2_relpos_bias_fwd", ptr(bias), ptr(T), plan, S, Lq, H, int(offset), dtype_code(T.dtype))
+    return bias
+
+
+def rrule_relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: int, *, offset: int = 0):
+    """Forward + pullback Δ -> ∂table; Δ (S, L, H, ...) is summed over its further dimensions."""
+    bias = relative_position_bias(table, buckets, keys, queries, offset=offset)
+    S, Lq, H = bias.shape[:3]
+
+    def pullback(delta):
+        if tuple(delta.shape[:3]) != (S, Lq, H):
+            raise DimensionMismatch(f"the cotangent must have the shape ({S}, {Lq}, {H}, ...)")
+        d = _cotangent(delta, bias.dtype)
+        device = _on_one_device(table=bias, cotangent=d)
+        plan, Bn = C.byref(_buckets_struct(buckets)), math.prod(d.shape[3:])
+        dtable = jl_empty((H, len(buckets)), bias.dtype, device)
+        _, wsp, wsn = _ws(_cabi.load().lb2_relpos_bias_bwd_workspace_bytes(plan, S, Lq, H, Bn), device)
+        _launch(device, "lb2_relpos_bias_bwd", ptr(dtable), ptr(d), plan, S, Lq, H, Bn, int(offset), dtype_code(bias.dtype), wsp, wsn)
+        return dtable
+
+    return bias, pullback
+
+
+def _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths, want_stats):
+    if q.dim() < 4 or k.dim() != q.dim() or v.dim() != q.dim():
+        raise AssertionError("N must be at least 4")
+    device = _on_one_device(q=q, k=k, v=v, table=table, lengths=lengths)
+    q, k, v, table = _promote(q, k, v, table)
+    Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
+    D, H, Lq = Q.shape[:3]
+    Hkv, S = Kx.shape[1], Kx.shape[2]
+    E, batch_shape = V.shape[0], tuple(Q.shape[3:])
+    if Kx.shape[0] != D:
+        raise AssertionError("`q` and `k` must have the same head dimension")
+    if batch_shape != tuple(Kx.shape[3:]) or batch_shape != tuple(V.shape[3:]):
+        raise DimensionMismatch("All dimensions (except first 3) of q, k, v must be the same")
+    if V.shape[2] != S or V.shape[1] != Hkv:
+        raise AssertionError("`v` and `k` must have the same number of tokens and heads")
+    if Hkv == 0 or H % Hkv != 0:
+        raise AssertionError("num_heads must be divisible by num_kv_groups")
+    Bn = math.prod(batch_shape)
+    if lengths is not None:
+        if lengths.numel() != Bn:
+            raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {lengths.numel()}")
+        lengths = as_colmajor(lengths.to(torch.int32))
+    Tb, plan = _table_of(table, buckets, H)
+    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
+    dt = dtype_code(Q.dtype)
+    dims = _cabi.WindowDims(D, E, H, Hkv, Lq, S, Bn, int(window), int(sinks), int(bool(is_causal)))
+    out = jl_empty((E, H, Lq) + batch_shape, Q.dtype, device)
+    stats = torch.empty(2 * Lq * H * Bn, dtype=torch.float32, device=device) if want_stats else None
+    _launch(device, "lb2_window_attention_fwd", ptr(out), ptr(stats), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lengths), sc, C.byref(dims), dt)
+    return out, (stats, Q, Kx, V, Tb, plan, lengths, sc, dims, dt, device)
+
+
+def windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal: bool = True, scale=None, table=None, buckets=None, lengths=None):
+    """scaled_dot_product_attention over a sliding window: query l sees key s where |l - s| < window or s < sinks, and s <= l with
+    `is_causal`; weights are not formed. q (D, H, L, B...), k (D, Hkv, S, B...), v (E, Hkv, S, B...) -> x (E, H, L, B...); logits =
+    k'q / scale (default sqrt(D)), plus table[h, bucket(s - l)] when a bias `table` (H, len(buckets)) and its RelativeBuckets are given.
+    `lengths` (B...): how many tokens of each sample count; queries past them, and queries that see nothing, give zeros."""
+    return _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths, False)[0]
+
+
+def rrule_windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal: bool = True, scale=None, table=None, buckets=None, lengths=None):
+    """Forward + pullback Δ -> (∂q, ∂k, ∂v, ∂table); ∂table is None without a table."""
+    x, (stats, Q, Kx, V, Tb, plan, lens, sc, dims, dt, device) = _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets,
+                                                                                   lengths, True)
+
+    def pullback(dx):
+        if tuple(dx.shape) != tuple(x.shape):
+            raise DimensionMismatch("the cotangent must have the shape of the output")
+        G = _cotangent(dx, Q.dtype)
+        _on_one_device(q=Q, cotangent=G)
+        dq, dk, dv = (jl_empty(tuple(t.shape), Q.dtype, device) for t in (Q, Kx, V))
+        dtable = jl_empty(tuple(Tb.shape), Q.dtype, device) if Tb is not None else None
+        _, wsp, wsn = _ws(_cabi.load().lb2_window_attention_bwd_workspace_bytes(C.byref(dims), plan, dt), device)
+        _launch(device, "lb2_window_attention_bwd", ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(G), ptr(x), ptr(stats), ptr(Q), ptr(Kx), ptr(V),
+                ptr(Tb), plan, ptr(lens), sc, C.byref(dims), dt, wsp, wsn)
+        return dq, dk, dv, dtable
+
+    return x, pullback
+
+
+def _check_caches(kcache, vcache, k, v):
+    """The caches are written in place: they are taken as they are or not at all."""
+    for name, c, t in (("kcache", kcache, k), ("vcache", vcache, v)):
+        if c.dtype != t.dtype:
+            raise ArgumentError(f"{name} holds {c.dtype}, the new tokens are {t.dtype}")
+        if not is_colmajor(c):
+            raise ArgumentError(f"{name} must be a dense column-major array")
+        if c.dim() < 3 or c.shape[0] != t.shape[0] or c.shape[1] != t.shape[1]:
+            raise DimensionMismatch(f"{name} must have the shape (features, kv heads, capacity, batch...) of the tokens it takes")
+    if tuple(kcache.shape[2:]) != tuple(vcache.shape[2:]):
+        raise DimensionMismatch("kcache and vcache must have the same capacity and batch")
+
+
+def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, sinks: int = 0, scale=None, table=None, buckets=None):
+    """The causal windowed_attention of one new token per sample, q (D, H, B...), k (D, Hkv, B...), v (E, Hkv, B...) -> x (E, H, B...),
+    over the caches kcache (D, Hkv, capacity, B...), vcache (E, Hkv, capacity, B...), which take the token in place: position p goes to
+    slot p while p < sinks, then to sinks + (p - sinks) mod (capacity - sinks); capacity >= sinks + window. `lengths` (B..., Int32 on
+    the device, not changed) counts the tokens before this one; where it is negative there is no sequence: x is zero, the caches stay."""
+    device = _on_one_device(q=q, k=k, v=v, kcache=kcache, vcache=vcache, lengths=lengths, table=table)
+    if q.dim() < 3 or k.dim() != q.dim() or v.dim() != q.dim():
+        raise AssertionError("N must be at least 3")
+    if not (q.dtype == k.dtype == v.dtype) or (table is not None and table.dtype != q.dtype):
+        raise ArgumentError("q, k, v and the table must have one element type")
+    _check_caches(kcache, vcache, k, v)
+    Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
+    (D, H), (E, Hkv), batch_shape = Q.shape[:2], V.shape[:2], tuple(Q.shape[2:])
+    if Kx.shape[0] != D or Kx.shape[1] != Hkv:
+        raise AssertionError("`q` and `k` must have the same head dimension, `k` and `v` the same heads")
+    if any(tuple(t.shape[-len(batch_shape):]) != batch_shape for t in (Kx, V)) or tuple(kcache.shape[3:]) != batch_shape:
+        raise DimensionMismatch("q, k, v and the caches must have the same batch")
+    if Hkv == 0 or H % Hkv != 0:
+        raise AssertionError("num_heads must be divisible by num_kv_groups")
+    Bn = math.prod(batch_shape)
+    if lengths.dtype != torch.int32 or lengths.numel() != Bn:
+        raise ArgumentError(f"lengths must hold one Int32 per sample ({Bn})")
+    lens = as_colmajor(lengths)
+    Tb, plan = _table_of(table, buckets, H)
+    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
+    dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache.shape[2], Bn, int(window), int(sinks), 1)
+    x = jl_empty((E, H) + batch_shape, Q.dtype, device)
+    _launch(device, "lb2_window_attention_step", ptr(x), ptr(kcache), ptr(vcache), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lens), sc,
+            C.byref(dims), dtype_code(Q.dtype))
+    return x
+
+
+def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
+    """Puts a prompt k (D, Hkv, S, B...), v (E, Hkv, S, B...) into the caches of windowed_attention_step, as if its tokens had come one by
+    one; `lengths` (B...) as in windowed_attention. The slots that hold none of them stay as they are."""
+    device = _on_one_device(kcache=kcache, vcache=vcache, k=k, v=v, lengths=lengths)
+    if k.dim() < 4 or v.dim() != k.dim():
+        raise AssertionError("N must be at least 4")
+    _check_caches(kcache, vcache, k, v)
+    Kx, V = as_colmajor(k), as_colmajor(v)
+    if tuple(Kx.shape[1:]) != tuple(V.shape[1:]) or tuple(Kx.shape[3:]) != tuple(kcache.shape[3:]):
+        raise DimensionMismatch("k, v and the caches must have the same heads, tokens and batch")
+    Bn = math.prod(Kx.shape[3:])
+    if lengths is not None:
+        if lengths.numel() != Bn:
+            raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {lengths.numel()}")
+        lengths = as_colmajor(lengths.to(torch.int32))
+    dims = _cabi.WindowDims(Kx.shape[0], V.shape[0], 0, Kx.shape[1], 0, Kx.shape[2], Bn, 1, int(sinks), 1)
+    _launch(device, "lb2_window_cache_fill", ptr(kcache), ptr(vcache), ptr(Kx), ptr(V), ptr(lengths), kcache.shape[2], C.byref(dims),
+            dtype_code(Kx.dtype))
 
 
 # --------------------------------------------------------------------------------------------
