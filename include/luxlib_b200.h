@@ -370,8 +370,8 @@ LB2_API int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_r
  * lb2_attention_fwd: q (head_dim, heads, queries, batch), k, v -> x (value_dim, heads, queries, batch); logits = scale * k'q, plus
  * table[h, bucket(s - l)] unless table and buckets are NULL. A query that sees nothing gives a zero row; keys that it does not see
  * do not reach it, infinities and NaN among them. head_dim and value_dim up to 256.
- * stats (2, queries, heads, batch), fp32, for the backward call: each softmax's maximum and the log of its sum relative to that (0 and
- * +inf for a query that sees nothing); NULL: not kept.
+ * stats (2, queries, heads, batch), fp32, 8-byte aligned, for the backward call: a reference value of each softmax and the log2 of its
+ * sum relative to that (0 and +inf for a query that sees nothing); NULL: not kept.
  * Backward: dq, dk, dv, and dtable (NULL without a table), zero for tokens past lengths[b]; every sum has a fixed order. */
 typedef struct lb2_window_dims {
   int64_t head_dim, value_dim, heads, kv_heads, queries, keys, batch, window, sinks, causal;

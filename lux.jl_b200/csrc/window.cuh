@@ -18,9 +18,14 @@ struct WinParams {
   const int32_t* lengths;
   int D, E, H, Hkv, rep, L, S, B;
   int window, sinks, causal;
-  float scale;
+  float scale, scale2;        // of the logits; scale2 = scale * log2(e)
   lb2_rel_buckets buckets;    // count = 0: no bias
 };
+
+// Logits are kept times log2(e): p = 2^((z2 - m2) - log2(sum)). A finite bias stays finite: the type's lowest value is a mask
+// whose rows still have a softmax.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float win_bias2(float b) { return isinf(b) ? b : fminf(fmaxf(b * kLog2e, -3.402823466e38f), 3.402823466e38f); }
 
 __device__ __forceinline__ int win_tokens(const WinParams& p, int b, int n) {
   return p.lengths == nullptr ? n : max(0, min(n, p.lengths[b]));
@@ -59,7 +64,7 @@ __device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, int rel) {
   return lo + (t.bidirectional && rel > 0 ? t.count : 0);
 }
 template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, int h, int rel) {
-  return to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, rel)]);
+  return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, rel)]));
 }
 
 // ---- rows once more ---------------------------------------------------------------------------
@@ -92,8 +97,8 @@ template <typename T> __device__ __forceinline__ const T* win_kv_row(const WinPa
   return static_cast<const T*>(base) + (((int64_t)b * p.S + s) * p.Hkv + g) * n;
 }
 
-// stats of a row: the maximum m of its logits and log(sum of exp(z - m)), apart: m + log(sum) would lose the sum beside an m as large
-// as the type's lowest value. p = exp((z - m) - log(sum)); a row that sees nothing has (0, inf).
+// stats of a row: the reference m2 that its logits were compared with (their maximum, or a little less) and log2(sum of 2^(z2 - m2)),
+// apart: their sum would lose the second beside an m2 as large as the type's lowest value. A row that sees nothing has (0, inf).
 template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, float2* stats, int l, int h, int b, int keys) {
   const int lane = threadIdx.x & 31, g = h / p.rep;
   float q[kWinLaneDims], t[kWinLaneDims], o[kWinLaneDims] = {};
@@ -104,10 +109,10 @@ template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& 
   for (int i0 = 0, n = sinks + max(0, hi - lo); i0 < n; ++i0) {
     const int s = i0 < sinks ? i0 : lo + (i0 - sinks);
     win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
-    float z = win_dot_lane(q, t, p.D) * p.scale;
+    float z = win_dot_lane(q, t, p.D) * p.scale2;
     if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
     const float mn = fmaxf(m, z), ref = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - ref), w = expf(z - ref);
+    const float keep = exp2f(m - ref), w = exp2f(z - ref);
     win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, t);
 #pragma unroll
     for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(w, t[i], o[i] * keep);
@@ -117,7 +122,7 @@ template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& 
 #pragma unroll
   for (int i = 0; i < kWinLaneDims; ++i) o[i] /= sum;
   win_store_lane(x + (((int64_t)b * p.L + l) * p.H + h) * p.E, p.E, lane, o);
-  if (stats != nullptr && lane == 0) *stats = make_float2(m, logf(sum));
+  if (stats != nullptr && lane == 0) *stats = make_float2(m, log2f(sum));
 }
 
 // stats, delta: of query l, head h
@@ -133,9 +138,9 @@ __device__ __noinline__ void win_row_dq(const WinParams& p, T* dq, const void* d
     const int s = i0 < sinks ? i0 : lo + (i0 - sinks);
     win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
     win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, u);
-    float z = win_dot_lane(q, t, p.D) * p.scale;
+    float z = win_dot_lane(q, t, p.D) * p.scale2;
     if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
-    const float ds = expf((z - stats.x) - stats.y) * (win_dot_lane(go, u, p.E) - delta) * p.scale;
+    const float ds = exp2f((z - stats.x) - stats.y) * (win_dot_lane(go, u, p.E) - delta) * p.scale;
 #pragma unroll
     for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(ds, t[i], o[i]);
   }
@@ -157,10 +162,10 @@ __device__ __noinline__ void win_row_dkv(const WinParams& p, T* dk, T* dv, const
     for (int l = lo; l < hi; ++l) {
       win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, t);
       win_load_lane(win_q_row<T>(p, dx, p.E, l, h, b), p.E, lane, u);
-      float z = win_dot_lane(t, k, p.D) * p.scale;
+      float z = win_dot_lane(t, k, p.D) * p.scale2;
       if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
       const int64_t at = ((int64_t)b * p.H + h) * p.L + l;
-      const float w = expf((z - stats[at].x) - stats[at].y), ds = w * (win_dot_lane(u, v, p.E) - delta[at]) * p.scale;
+      const float w = exp2f((z - stats[at].x) - stats[at].y), ds = w * (win_dot_lane(u, v, p.E) - delta[at]) * p.scale;
 #pragma unroll
       for (int i = 0; i < kWinLaneDims; ++i) { ov[i] = fmaf(w, u[i], ov[i]); ok[i] = fmaf(ds, t[i], ok[i]); }
     }

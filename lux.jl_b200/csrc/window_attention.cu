@@ -10,7 +10,7 @@
 //
 // This file: the CUDA-core kernels, which serve Float32 and every feature count up to 256, and the entry points.
 #include "common.cuh"
-#include "window.cuh"
+#include "window_tc.cuh"
 
 namespace lb2 {
 
@@ -141,7 +141,7 @@ template <int DP> struct WinTile {
 template <typename T, int BM> __device__ __forceinline__ void win_fill_diag(float* diag, int* bucket, const WinParams& p, int h, int l0, int s0) {
   for (int i = threadIdx.x; i < 2 * BM - 1; i += kWinThreads) {
     const int rel = -(l0 - s0 + i - (BM - 1)), b = win_bucket(p.buckets, rel);
-    diag[i] = to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * b]);
+    diag[i] = win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * b]));
     if (bucket != nullptr) bucket[i] = b;
   }
 }
@@ -190,17 +190,17 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int c = tx + 16 * j, s = s0 + c;
-        float u = z[i][j] * p.scale;
+        float u = z[i][j] * p.scale2;
         if (p.buckets.count > 0) u += sD[r - c + BM - 1];
         z[i][j] = s < keys && win_sees(p, l, s) ? u : -INFINITY;
         mx = fmaxf(mx, z[i][j]);
       }
       mx = half_max(mx);
-      const float ref = mx == -INFINITY ? 0.f : mx, keep = expf(m[i] - ref);
+      const float ref = mx == -INFINITY ? 0.f : mx, keep = exp2f(m[i] - ref);
       float part = 0.f;
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const float w = expf(z[i][j] - ref);
+        const float w = exp2f(z[i][j] - ref);
         part += w;
         sP[r * LDP + tx + 16 * j] = w;
       }
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
       ok = ok && finite4(o[i][c]);
       win_put4(xb + (int64_t)l * p.H * p.E, 4 * tx + 64 * c, p.E, any ? o[i][c] : make_float4(0.f, 0.f, 0.f, 0.f), inv);
     }
-    if (lb != nullptr && tx == 0) lb[l] = any ? make_float2(m[i], logf(sum[i])) : make_float2(0.f, INFINITY);
+    if (lb != nullptr && tx == 0) lb[l] = any ? make_float2(m[i], log2f(sum[i])) : make_float2(0.f, INFINITY);
     if (any && !ok) bad[ty + 16 * i] = 1;
   }
   __syncthreads();
@@ -305,9 +305,9 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq,
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         const int r = ty + 16 * i, c = tx + 16 * j, l = l0 + r, s = s0 + c;
-        float u = z[i][j] * p.scale;
+        float u = z[i][j] * p.scale2;
         if (p.buckets.count > 0) u += sD[r - c + BM - 1];
-        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? expf((u - ls[i].x) - ls[i].y) * (dp[i][j] - de[i]) : 0.f;
+        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? exp2f((u - ls[i].x) - ls[i].y) * (dp[i][j] - de[i]) : 0.f;
       }
     if (p.buckets.count > 0) {          // sums along the diagonals, then those of a bucket, each in order
       __syncthreads();
@@ -406,10 +406,10 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
 #pragma unroll
         for (int jj = 0; jj < TM; ++jj) {
           const int c = tx + 16 * jj, s = s0 + c;
-          float u = z[i][jj] * p.scale;
+          float u = z[i][jj] * p.scale2;
           if (p.buckets.count > 0) u += sD[r - c + BM - 1];
           const bool in = l < queries && s < keys && win_sees(p, l, s);
-          const float w = in ? expf((u - ls.x) - ls.y) : 0.f;
+          const float w = in ? exp2f((u - ls.x) - ls.y) : 0.f;
           sP[r * LDP + c] = w;
           sS[r * LDP + c] = in ? w * (dp[i][jj] - de) : 0.f;
         }
@@ -473,7 +473,7 @@ WinParams win_params(const lb2_window_dims* d, const void* q, const void* k, con
   p.window = (int)(d->window < most ? d->window : most);
   p.sinks = (int)(d->sinks < d->keys ? d->sinks : d->keys);
   p.causal = d->causal != 0;
-  p.scale = (float)scale;
+  p.scale = (float)scale; p.scale2 = (float)(scale * 1.4426950408889634);
   if (t != nullptr) p.buckets = *t;
   return p;
 }
@@ -518,6 +518,8 @@ int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const voi
               LB2_BAD_ALIGN, "pointer not aligned to the element size");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const WinParams p = win_params(d, q, k, v, table, buckets, lengths, scale);
+  if (win_tc_serves(d, dtype) && aligned_to(x, 16) && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16))
+    return win_tc_fwd(p, x, reinterpret_cast<float2*>(stats), st);
   const int tile = win_simt_tile(d);
   const int64_t tiles = win_tiles(d->queries, tile), blocks = tiles * d->heads * d->batch;
   LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");

@@ -18,7 +18,7 @@ struct StepParams {
   const void *q, *k, *v, *table;
   const int32_t* lengths;
   int D, E, H, Hkv, rep, C, window, sinks;
-  float scale;
+  float scale2;
   lb2_rel_buckets buckets;
 };
 
@@ -46,10 +46,10 @@ template <typename T> __global__ void __launch_bounds__(256) win_step_kernel(con
     const int s = i < early ? i : lo + (i - early);
     const int64_t slot = ring_slot(s, p.sinks, ring);
     win_load_lane(s == n ? kn : kc + slot * p.Hkv * p.D, p.D, lane, t);
-    float z = win_dot_lane(q, t, p.D) * p.scale;
-    if (p.buckets.count > 0) z += to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, s - n)]);
+    float z = win_dot_lane(q, t, p.D) * p.scale2;
+    if (p.buckets.count > 0) z += win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, s - n)]));
     const float mn = fmaxf(m, z), ref = mn == -INFINITY ? 0.f : mn;
-    const float keep = expf(m - ref), w = expf(z - ref);
+    const float keep = exp2f(m - ref), w = exp2f(z - ref);
     win_load_lane(s == n ? vn : vc + slot * p.Hkv * p.E, p.E, lane, t);
 #pragma unroll
     for (int j = 0; j < kWinLaneDims; ++j) o[j] = fmaf(w, t[j], o[j] * keep);
@@ -63,11 +63,11 @@ template <typename T> __global__ void __launch_bounds__(256) win_step_kernel(con
   float top = -INFINITY, total = 0.f;
   for (int w = 0; w < 8; ++w) top = fmaxf(top, sm[w]);
   const float ref = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < 8; ++w) total += ss[w] * expf(sm[w] - ref);
+  for (int w = 0; w < 8; ++w) total += ss[w] * exp2f(sm[w] - ref);
   for (int e = threadIdx.x; e < p.E; e += 256) {
     float a = 0.f;
     for (int w = 0; w < 8; ++w)
-      if (w < count) a = fmaf(so[w][e], expf(sm[w] - ref), a);           // a warp without a key adds nothing
+      if (w < count) a = fmaf(so[w][e], exp2f(sm[w] - ref), a);           // a warp without a key adds nothing
     xr[e] = from_f32<T>(a / total);
   }
   if (h % p.rep == 0) {
@@ -139,7 +139,7 @@ int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, const voi
   p.x = x; p.kcache = kcache; p.vcache = vcache; p.q = q; p.k = k; p.v = v; p.table = table; p.lengths = lengths;
   p.D = (int)d->head_dim; p.E = (int)d->value_dim; p.H = (int)d->heads; p.Hkv = (int)d->kv_heads; p.rep = (int)(d->heads / d->kv_heads);
   p.C = (int)d->keys; p.window = (int)d->window; p.sinks = (int)d->sinks;
-  p.scale = (float)scale;
+  p.scale2 = (float)(scale * 1.4426950408889634);
   if (buckets != nullptr) p.buckets = *buckets;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LB2_DISPATCH_DTYPE(dtype, { win_step_kernel<T><<<(unsigned)(d->heads * d->batch), 256, 0, st>>>(p); });

@@ -1,0 +1,139 @@
+// Windowed attention on the tensor cores (BFloat16, up to 128 features): declarations shared by its forward and backward kernels.
+#pragma once
+#include "tc_ptx.cuh"
+#include "window.cuh"
+
+namespace lb2 {
+
+constexpr int kWtTile = 128;                 // queries and keys of a tile
+constexpr int kWtBox = kWtTile * 128;        // bytes of a TMA box: 128 tokens x 64 features
+// what the tensor-core kernels serve: rows of whole 16-byte vectors for TMA, at most two boxes of features
+bool win_tc_serves(const lb2_window_dims* d, int32_t dtype);
+int32_t win_tc_fwd(const WinParams& p, void* x, float2* stats, cudaStream_t st);
+
+// token arrays (features, heads, tokens, batch) in boxes of 64 features x 128 tokens of one head
+inline bool wt_encode(CUtensorMap* map, const void* ptr, int64_t features, int64_t heads, int64_t tokens, int64_t batch) {
+  TensorMapEncodeFn enc = tensor_map_encoder();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)features, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)batch};
+  cuuint64_t strides[3] = {(cuuint64_t)(features * 2), (cuuint64_t)(features * heads * 2), (cuuint64_t)(features * heads * tokens * 2)};
+  cuuint32_t box[4] = {64, 1, kWtTile, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Shared-memory descriptors of a tile of 128 tokens in boxes: features as the contraction (K-major: 32 bytes per step of 16, the
+// next box after four) or tokens as the contraction (MN-major: 16 rows of 128 bytes per step, boxes side by side along N).
+constexpr uint32_t kWtDescHi = ((1024u >> 4) & 0x3FFFu) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint64_t wt_desc_k(uint32_t addr) { return ((uint64_t)kWtDescHi << 32) | ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint64_t wt_desc_mn(uint32_t addr) {
+  return ((uint64_t)kWtDescHi << 32) | ((addr >> 4) & 0x3FFFu) | ((uint32_t)(kWtBox >> 4) << 16);
+}
+__host__ __device__ constexpr uint32_t wt_idesc(int n, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kWtTile >> 4) << 24);
+}
+// D[128][128] = A . B' over NB boxes of features, both K-major in shared memory
+template <int NB> __device__ __forceinline__ void wt_mma_features(uint32_t d, uint32_t a, uint32_t b) {
+  const uint64_t ad = wt_desc_k(a), bd = wt_desc_k(b);
+#pragma unroll
+  for (int ks = 0; ks < 4 * NB; ++ks) {
+    const uint32_t at = (ks >> 2) * (kWtBox >> 4) + (ks & 3) * 2;
+    umma<false>(d, ad + at, bd + at, wt_idesc(kWtTile, false), ks != 0 ? 1u : 0u);
+  }
+}
+// A operand in TMEM: 128 lanes x 128 values, two bf16 per column
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[128][64 NB] (+)= P . V: P from TMEM, V a tile of 128 tokens
+template <int NB> __device__ __forceinline__ void wt_mma_tokens(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
+  const uint64_t vd = wt_desc_mn(v);
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t u;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  return u;
+}
+__device__ __forceinline__ void bar_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// The tiles of 128 keys that a tile of queries visits: [0, nsink) and [first, last).
+struct WtTiles {
+  int nsink, first, last;
+  __device__ __forceinline__ int count() const { return nsink + max(0, last - first); }
+  __device__ __forceinline__ int at(int i) const { return i < nsink ? i : first + (i - nsink); }
+  __device__ __forceinline__ bool has(int t) const { return t < nsink || (t >= first && t < last); }
+};
+__device__ __forceinline__ WtTiles wt_key_tiles(const WinParams& p, int l0, int queries, int keys) {
+  WtTiles r{0, 0, 0};
+  if (l0 >= queries) return r;
+  int sinks, lo, hi;
+  win_key_range(p, l0, min(l0 + kWtTile, queries), keys, &sinks, &lo, &hi);
+  r.nsink = (sinks + kWtTile - 1) / kWtTile;
+  if (lo < hi) { r.first = max(r.nsink, lo / kWtTile); r.last = (hi + kWtTile - 1) / kWtTile; }
+  return r;
+}
+// the tiles of both
+__device__ __forceinline__ WtTiles wt_union(const WtTiles& a, const WtTiles& b) {
+  if (a.count() == 0) return b;
+  if (b.count() == 0) return a;
+  WtTiles r;
+  r.nsink = max(a.nsink, b.nsink);
+  const bool ea = a.first >= a.last, eb = b.first >= b.last;
+  r.first = ea ? b.first : (eb ? a.first : min(a.first, b.first));
+  r.last = ea ? b.last : (eb ? a.last : max(a.last, b.last));
+  r.first = max(r.first, r.nsink);
+  return r;
+}
+// Which columns of a tile a row sees: s = s0 + j with j <= hi and (j >= lo or j < sink).
+struct WtSeen { int lo, hi, sink; };
+__device__ __forceinline__ WtSeen wt_seen(const WinParams& p, int l, int queries, int s0, int keys) {
+  WtSeen w;
+  w.lo = l - p.window + 1 - s0;
+  w.sink = p.sinks - s0;
+  w.hi = (p.causal ? min(l, keys - 1) : keys - 1) - s0;
+  if (!p.causal && w.sink <= 0) w.hi = min(w.hi, l + p.window - 1 - s0);
+  if (l >= queries) w.hi = -1;
+  return w;
+}
+// non-causal tiles with sinks: the sink columns are seen beyond the window's end, the others are not
+__device__ __forceinline__ bool wt_sees(const WinParams& p, const WtSeen& w, int l, int s0, int j) {
+  return j <= w.hi && (j < w.sink || (j >= w.lo && (p.causal || s0 + j < l + p.window)));
+}
+// every row of the tile sees every key of it
+__device__ __forceinline__ bool wt_all_seen(const WinParams& p, int l0, int queries, int s0, int keys) {
+  if (l0 + kWtTile > queries || s0 + kWtTile > keys) return false;
+  if (p.causal && s0 + kWtTile - 1 > l0) return false;
+  const bool sinks = s0 + kWtTile <= p.sinks;
+  return sinks || (l0 + kWtTile - 1 - s0 < p.window && s0 + kWtTile - 1 - l0 < p.window);
+}
+
+}  // namespace lb2
