@@ -14,7 +14,9 @@ namespace lb2 {
 
 namespace {
 
-constexpr int kWtFwdThreads = 320;           // warp 0: TMA, warp 1: MMA, warps 2-5 and 6-9: one softmax group each
+// warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: one softmax group each. The softmax keeps a row of S in registers: the first four
+// warps give up theirs (56 + 2 x 224 = 3 x 168 per thread at launch).
+constexpr int kWtFwdThreads = 384, kWtFwdFew = 56, kWtFwdMany = 224;
 
 template <int NB> struct WtFwd {
   static constexpr int TILE = NB * kWtBox;
@@ -81,78 +83,82 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
-    if (n > 0) {
-      if (elect_one()) {
-        mbar_expect_tx(q_full, (uint32_t)(2 * p.boxes_d * kWtBox));
-        for (int i = 0; i < 2; ++i)
-          for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sQ + i * C::TILE + x * kWtBox, &tmQ, x * 64, head[i], min(l0[i], w.L - 1), b, q_full);
-      }
-      __syncwarp();
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      for (int i = 0; i < 2 * n && ok; ++i) {
-        if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) { ok = false; break; }
+  if (warp < 4) {
+    regs_less<kWtFwdFew>();
+    if (warp == 0) {
+      if (n > 0) {
         if (elect_one()) {
-          const bool is_k = (i & 1) == 0;
-          const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = all.at(i >> 1) * kWtTile;
-          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
-          for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, g, s0, b, &full[stage]);
+          mbar_expect_tx(q_full, (uint32_t)(2 * p.boxes_d * kWtBox));
+          for (int i = 0; i < 2; ++i)
+            for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sQ + i * C::TILE + x * kWtBox, &tmQ, x * 64, head[i], min(l0[i], w.L - 1), b, q_full);
         }
         __syncwarp();
-        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-      }
-    }
-  } else if (warp == 1) {
-    // in order: S0 S1 of the first tile; then per tile, O of it and S of the next for each group in turn
-    bool ok = n == 0 || mbar_wait_uniform(q_full, 0, p.status, 0x200u);
-    uint32_t ready[2] = {0, 0};              // phases of p_ready
-    bool begun[2] = {false, false};
-    auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
-    auto scores = [&](int i, int grp) {
-      if (elect_one()) {
-        const uint32_t k = sKV + (2 * i % C::STAGES) * C::TILE, q = sQ + grp * C::TILE, d = tmem + grp * 128;
-        if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(d, q, k);
-        else wt_mma_features<1>(d, q, k);
-        umma_commit(&s_full[grp]);
-      }
-      __syncwarp();
-    };
-    auto release = [&](int i) {
-      if (elect_one()) umma_commit(&empty[i % C::STAGES]);
-      __syncwarp();
-    };
-    for (int i = -1; i < n && ok; ++i) {
-      const bool next = i + 1 < n;
-      if (next && !wait_stage(2 * (i + 1))) { ok = false; break; }
-      if (i >= 0 && !wait_stage(2 * i + 1)) { ok = false; break; }
-      tc_fence_after();
-#pragma unroll
-      for (int grp = 0; grp < 2; ++grp) {
-        if (!ok) break;
-        if (i >= 0 && own[grp].has(all.at(i))) {
-          if (!mbar_wait_uniform(&p_ready[grp], ready[grp], p.status, 0x800u)) { ok = false; break; }
-          ready[grp] ^= 1u;
-          tc_fence_after();
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (int i = 0; i < 2 * n && ok; ++i) {
+          if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) { ok = false; break; }
           if (elect_one()) {
-            const uint32_t v = sKV + ((2 * i + 1) % C::STAGES) * C::TILE, d = tmem + 256 + grp * 128, a = tmem + grp * 128;
-            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens<NB>(d, a, v, begun[grp]);
-            else wt_mma_tokens<1>(d, a, v, begun[grp]);
+            const bool is_k = (i & 1) == 0;
+            const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = all.at(i >> 1) * kWtTile;
+            mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
+            for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, g, s0, b, &full[stage]);
           }
           __syncwarp();
-          begun[grp] = true;
+          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
-        if (next && own[grp].has(all.at(i + 1))) scores(i + 1, grp);
       }
-      if (!ok) break;
-      if (i >= 0) release(2 * i + 1);
-      if (next) release(2 * (i + 1));
+    } else if (warp == 1) {
+      // in order: S0 S1 of the first tile; then per tile, O of it and S of the next for each group in turn
+      bool ok = n == 0 || mbar_wait_uniform(q_full, 0, p.status, 0x200u);
+      uint32_t ready[2] = {0, 0};              // phases of p_ready
+      bool begun[2] = {false, false};
+      auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
+      auto scores = [&](int i, int grp) {
+        if (elect_one()) {
+          const uint32_t k = sKV + (2 * i % C::STAGES) * C::TILE, q = sQ + grp * C::TILE, d = tmem + grp * 128;
+          if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(d, q, k);
+          else wt_mma_features<1>(d, q, k);
+          umma_commit(&s_full[grp]);
+        }
+        __syncwarp();
+      };
+      auto release = [&](int i) {
+        if (elect_one()) umma_commit(&empty[i % C::STAGES]);
+        __syncwarp();
+      };
+      for (int i = -1; i < n && ok; ++i) {
+        const bool next = i + 1 < n;
+        if (next && !wait_stage(2 * (i + 1))) { ok = false; break; }
+        if (i >= 0 && !wait_stage(2 * i + 1)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int grp = 0; grp < 2; ++grp) {
+          if (!ok) break;
+          if (i >= 0 && own[grp].has(all.at(i))) {
+            if (!mbar_wait_uniform(&p_ready[grp], ready[grp], p.status, 0x800u)) { ok = false; break; }
+            ready[grp] ^= 1u;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t v = sKV + ((2 * i + 1) % C::STAGES) * C::TILE, d = tmem + 256 + grp * 128, a = tmem + grp * 128;
+              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens<NB>(d, a, v, begun[grp]);
+              else wt_mma_tokens<1>(d, a, v, begun[grp]);
+            }
+            __syncwarp();
+            begun[grp] = true;
+          }
+          if (next && own[grp].has(all.at(i + 1))) scores(i + 1, grp);
+        }
+        if (!ok) break;
+        if (i >= 0) release(2 * i + 1);
+        if (next) release(2 * (i + 1));
+      }
+      if (ok && elect_one()) { umma_commit(&o_full[0]); umma_commit(&o_full[1]); }
+      __syncwarp();
     }
-    if (ok && elect_one()) { umma_commit(&o_full[0]); umma_commit(&o_full[1]); }
-    __syncwarp();
   } else {
-    const int grp = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane, l = l0[grp] + row, h = head[grp];
-    const int gt = threadIdx.x - 64 - grp * 128;
+    regs_more<kWtFwdMany>();
+    const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, l = l0[grp] + row, h = head[grp];
+    const int gt = threadIdx.x - 128 - grp * 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + grp * 128, tO = tmem + lanes + 256 + grp * 128;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
@@ -181,60 +187,71 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (!mbar_wait_warp(&s_full[grp], phase, p.status, 0x1000u)) { ok = false; break; }
       phase ^= 1u;
       tc_fence_after();
+      // logits = mul * z + flat, mul > 0; what a row does not see is -inf
       float z[128];
-      {
+      const float mul = bias == nullptr && c2 > 0.f ? c2 : 1.f;
+      const bool whole = wt_all_seen(w, l0[grp], queries, s0, keys);
+      const WtSeen seen = wt_seen(w, l, queries, s0, keys);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
         uint32_t v[32];
+        tmem_ld32(tS + q * 32, v);
+        tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tmem_ld32(tS + q * 32, v);
-          tmem_ld_wait();
+        for (int j = 0; j < 32; ++j) z[q * 32 + j] = __uint_as_float(v[j]);
+        if (bias != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(__uint_as_float(v[j]), c2, flat);
+          for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(z[q * 32 + j], c2, bias[q * 32 + j]);
+        } else if (!(c2 > 0.f)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[q * 32 + j] *= c2;
         }
-      }
-      if (bias != nullptr) {
+        if (!whole) {
 #pragma unroll
-        for (int j = 0; j < 128; ++j) z[j] += bias[j];
-      }
-      if (!wt_all_seen(w, l0[grp], queries, s0, keys)) {
-        const WtSeen seen = wt_seen(w, l, queries, s0, keys);
-#pragma unroll
-        for (int j = 0; j < 128; ++j) z[j] = wt_sees(w, seen, l, s0, j) ? z[j] : -INFINITY;
+          for (int j = 0; j < 32; ++j) z[q * 32 + j] = wt_sees(w, seen, l, s0, q * 32 + j) ? z[q * 32 + j] : -INFINITY;
+        }
       }
       float top[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
       for (int j = 4; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], z[j]);
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      const bool grow = mx > m2 + 8.f || (m2 == -INFINITY && mx > m2);
+      const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, flat);
+      const bool grow = mx > m2 + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float keep = grow ? ex2(m2 - mx) : 1.f;
         if (grow) { m2 = mx; sum *= keep; }
         if (begun) {
-#pragma unroll
-          for (int q = 0; q < 2 * NB; ++q) {
-            uint32_t v[32];
-            tmem_ld32(tO + q * 32, v);
+#pragma unroll 1
+          for (int q = 0; q < 4 * NB; ++q) {
+            uint32_t v[16];
+            tmem_ld16(tO + q * 16, v);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * keep);
-            tmem_st32(tO + q * 32, v);
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * keep);
+            tmem_st16(tO + q * 16, v);
           }
         }
       }
       const float ref = m2 == -INFINITY ? 0.f : m2;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t mul_2 = pack2(mul, mul), off_2 = pack2(flat - ref, flat - ref);
+      uint64_t part[2] = {0, 0};
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
+      for (int q = 0; q < 4; ++q) {
+        uint32_t v[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float a = ex2(z[q * 64 + 2 * j] - ref), c = ex2(z[q * 64 + 2 * j + 1] - ref);
-          part[j & 3] += a + c;
+        for (int j = 0; j < 16; ++j) {
+          float a, c;
+          unpack2(fma2(pack2(z[q * 32 + 2 * j], z[q * 32 + 2 * j + 1]), mul_2, off_2), a, c);
+          a = ex2(a); c = ex2(c);
+          part[j & 1] = add2(part[j & 1], pack2(a, c));
           v[j] = pack_bf16(a, c);
         }
-        tmem_st32(tS + q * 32, v);
+        tmem_st16(tS + q * 16, v);
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      {
+        float a, c;
+        unpack2(add2(part[0], part[1]), a, c);
+        sum += a + c;
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
