@@ -571,6 +571,15 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   const int64_t qt = win_tiles(d->queries, tile), kt = win_tiles(d->keys, tile);
   LB2_REQUIRE(qt * d->heads * d->batch <= 0x7FFFFFFF && kt * d->kv_heads * d->batch <= 0x7FFFFFFF && (rows + 7) / 8 <= 0x7FFFFFFF, LB2_BAD_SHAPE,
               "too many rows");
+  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(q, 16) &&
+      aligned_to(k, 16) && aligned_to(v, 16)) {
+    win_delta_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(delta, (const __nv_bfloat16*)dx, (const __nv_bfloat16*)x, p.E, p.H, p.L, rows);
+    LB2_CHECK_LAUNCH("windowed attention delta");
+    if ((rc = win_tc_bwd(p, dq, dk, dv, partial, dx, reinterpret_cast<const float2*>(stats), delta, st)) != LB2_OK || columns == 0) return rc;
+    win_dtable_kernel<<<(unsigned)((p.H * columns + 7) / 8), 256, 0, st>>>((__nv_bfloat16*)dtable, partial, p.H, columns, win_tc_partials(d) * d->batch);
+    LB2_CHECK_LAUNCH("windowed attention dtable");
+    return LB2_OK;
+  }
   LB2_DISPATCH_DTYPE(dtype, LB2_WIN_DISPATCH(d, {
     using C = WinTile<DP>;
     if (nq) {

@@ -187,9 +187,10 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (!mbar_wait_warp(&s_full[grp], phase, p.status, 0x1000u)) { ok = false; break; }
       phase ^= 1u;
       tc_fence_after();
-      // logits = mul * z + flat, mul > 0; what a row does not see is -inf
+      // logits = mul * z + add, mul > 0; what a row does not see is -inf
       float z[128];
-      const float mul = bias == nullptr && c2 > 0.f ? c2 : 1.f;
+      const bool apart = bias == nullptr && wt_apart(c2, flat);
+      const float mul = apart ? c2 : 1.f, add = apart ? flat : 0.f;
       const bool whole = wt_all_seen(w, l0[grp], queries, s0, keys);
       const WtSeen seen = wt_seen(w, l, queries, s0, keys);
 #pragma unroll
@@ -202,9 +203,9 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (bias != nullptr) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(z[q * 32 + j], c2, bias[q * 32 + j]);
-        } else if (!(c2 > 0.f)) {
+        } else if (!apart) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[q * 32 + j] *= c2;
+          for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(z[q * 32 + j], c2, flat);
         }
         if (!whole) {
 #pragma unroll
@@ -214,7 +215,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       float top[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
       for (int j = 4; j < 128; ++j) top[j & 3] = fmaxf(top[j & 3], z[j]);
-      const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, flat);
+      const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
       const bool grow = mx > m2 + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
         const float keep = grow ? ex2(m2 - mx) : 1.f;
@@ -232,7 +233,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       const float ref = m2 == -INFINITY ? 0.f : m2;
-      const uint64_t mul_2 = pack2(mul, mul), off_2 = pack2(flat - ref, flat - ref);
+      const uint64_t mul_2 = pack2(mul, mul), off_2 = pack2(add - ref, add - ref);
       uint64_t part[2] = {0, 0};
 #pragma unroll
       for (int q = 0; q < 4; ++q) {

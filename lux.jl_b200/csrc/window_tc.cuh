@@ -9,6 +9,9 @@ constexpr int kWtTile = 128;                 // queries and keys of a tile
 constexpr int kWtBox = kWtTile * 128;        // bytes of a TMA box: 128 tokens x 64 features
 // what the tensor-core kernels serve: rows of whole 16-byte vectors for TMA, at most two boxes of features
 bool win_tc_serves(const lb2_window_dims* d, int32_t dtype);
+int64_t win_tc_partials(const lb2_window_dims* d);      // blocks that leave a partial sum of dtable per head and sample
+int32_t win_tc_bwd(const WinParams& p, void* dq, void* dk, void* dv, float* partial, const void* dx, const float2* stats, const float* delta,
+                   cudaStream_t st);
 int32_t win_tc_fwd(const WinParams& p, void* x, float2* stats, cudaStream_t st);
 
 // token arrays (features, heads, tokens, batch) in boxes of 64 features x 128 tokens of one head
@@ -55,15 +58,12 @@ template <int NB> __device__ __forceinline__ void wt_mma_tokens(uint32_t d, uint
 #pragma unroll
   for (int ks = 0; ks < 8; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
-template <int N> __device__ __forceinline__ void tmem_ld_row(uint32_t taddr, float (&z)[N]) {
+// as wt_mma_tokens with P in two halves 64 columns apart, each over the columns that its own threads have read
+template <int NB> __device__ __forceinline__ void wt_mma_tokens_halves(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
+  const uint64_t vd = wt_desc_mn(v);
 #pragma unroll
-  for (int q = 0; q < N / 32; ++q) {
-    uint32_t v[32];
-    tmem_ld32(taddr + q * 32, v);
-    tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 32; ++j) z[q * 32 + j] = __uint_as_float(v[j]);
-  }
+  for (int ks = 0; ks < 8; ++ks)
+    umma_ts(d, p + (ks >> 2) * 64 + (ks & 3) * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -88,6 +88,8 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A tile's one bias may join the reference instead of every logit while it does not swallow them.
+__device__ __forceinline__ bool wt_apart(float c2, float flat) { return c2 > 0.f && fabsf(flat) < 65536.f; }
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;

@@ -1,0 +1,664 @@
+// Windowed attention on the tensor cores, pullback: BFloat16, up to 128 features.
+//
+// Two kernels form the weights anew from the stats of the forward pass, so that no result is summed by more than one block:
+//   dq: a tile of 128 queries walks its tiles of keys;        S = Q K', dP = dX V', dS = p (dP - delta), dQ += dS K
+//   dk, dv: a tile of 128 keys walks its tiles of queries;    S' = K Q', dP' = V dX', dV += p' dX, dK += dS' Q
+// Rows are the block's own tokens, a thread holds half a row; p and dS go back to TMEM as bf16, over the columns of S and dP that
+// the same threads have read, and are the A operand of the next product, whose B operand is the tile that is in shared memory
+// already (tokens as the contraction). Two warpgroups share the exponentials of a tile.
+//
+// The bias table's gradient: sums of dS (fp32) by bucket. A tile of one bucket is summed in registers; in the others each warp adds
+// along its diagonals with shuffles, then joins neighbouring diagonals of a bucket; per-warp sums, fixed order.
+#include "common.cuh"
+#include "window_tc.cuh"
+
+namespace lb2 {
+
+namespace {
+
+// warp 0: TMA, warp 1: MMA, warps 4-11: softmax; registers 56 + 2 x 224 = 3 x 168 per thread at launch
+constexpr int kWtBwdThreads = 384, kWtBwdFew = 56, kWtBwdMany = 224, kWtSoft = 256;
+
+struct WtBwdParams {
+  WinParams w;
+  void *dq, *dk, *dv;
+  const void* dx;
+  const float2* stats;
+  const float* delta;
+  float* partial;
+  int tiles, columns, boxes_d, boxes_e;
+  unsigned int* status;
+};
+
+template <int NB> struct WtBwd {
+  static constexpr int TILE = NB * kWtBox;
+  static constexpr int STAGES = NB == 1 ? 6 : 4;
+  // dq: bias and bucket of the diagonals (two tiles), diagonal sums of 8 warps, bucket sums of 8 warps; dk, dv: bias, columns' stats
+  static constexpr int EXTRA = 2 * 256 * 4 + 2 * 256 + 8 * 4 * 48 * 4 + 8 * 2 * kWinMaxBuckets * 4 + 128 * 4;
+  static constexpr int SMEM = (2 + STAGES) * TILE + EXTRA + 256 + 1024;
+};
+
+__device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
+template <int NB>
+__global__ void __launch_bounds__(kWtBwdThreads, 1)
+win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WtBwdParams p) {
+  using C = WtBwd<NB>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
+  float* diag = lut + 2 * 256;                                                     // [warp][4][48]
+  float* bsum = diag + 8 * 4 * 48;                                                 // [warp][buckets]
+  int* bad = reinterpret_cast<int*>(bsum + 8 * 2 * kWinMaxBuckets);                // [128]
+  uint8_t* of = reinterpret_cast<uint8_t*>(bad + 128);                             // [parity][256]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(of + 2 * 256);
+  uint64_t *q_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 2, *ds_ready = dp_full + 1,
+           *o_full = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  const uint32_t sQ = base, sG = base + C::TILE, sKV = base + 2 * C::TILE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WinParams& w = p.w;
+  const int tile = blockIdx.x % p.tiles, hb = blockIdx.x / p.tiles, h = hb % w.H, b = hb / w.H, g = h / w.rep, l0 = tile * kWtTile;
+  const int queries = win_tokens(w, b, w.L), keys = win_tokens(w, b, w.S);
+  const WtTiles own = wt_key_tiles(w, l0, queries, keys);
+  const int n = own.count();
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(o_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x < 128) bad[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < 8 * 2 * kWinMaxBuckets; i += kWtBwdThreads) bsum[i] = 0.f;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tDP = tmem + 256, tDQ = tmem + 384;            // S of even and odd tiles at 0 and 128
+
+  if (warp < 4) {
+    regs_less<kWtBwdFew>();
+    if (warp == 0 && n > 0) {
+      if (elect_one()) {
+        mbar_expect_tx(q_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
+        for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sQ + x * kWtBox, &tmQ, x * 64, h, l0, b, q_full);
+        for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sG + x * kWtBox, &tmG, x * 64, h, l0, b, q_full);
+      }
+      __syncwarp();
+      uint32_t stage = 0, phase = 0;
+      for (int i = 0; i < 2 * n; ++i) {
+        if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) break;
+        if (elect_one()) {
+          const bool is_k = (i & 1) == 0;
+          const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = own.at(i >> 1) * kWtTile;
+          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
+          for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, g, s0, b, &full[stage]);
+        }
+        __syncwarp();
+        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+      }
+    } else if (warp == 1 && n > 0) {
+      bool ok = mbar_wait_uniform(q_full, 0, p.status, 0x200u);
+      auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
+      auto slot = [&](int i) { return sKV + (uint32_t)(i % C::STAGES) * C::TILE; };
+      auto scores = [&](int i) {
+        if (elect_one()) {
+          if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem + (i & 1) * 128, sQ, slot(2 * i));
+          else wt_mma_features<1>(tmem + (i & 1) * 128, sQ, slot(2 * i));
+          umma_commit(&s_full[i & 1]);
+        }
+        __syncwarp();
+      };
+      auto grads = [&](int i) {
+        if (elect_one()) {
+          if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, slot(2 * i + 1));
+          else wt_mma_features<1>(tDP, sG, slot(2 * i + 1));
+          umma_commit(dp_full);
+          umma_commit(&empty[(2 * i + 1) % C::STAGES]);
+        }
+        __syncwarp();
+      };
+      for (int i = -1; i < n && ok; ++i) {
+        const bool next = i + 1 < n;
+        if (next) {
+          if (!wait_stage(2 * (i + 1))) { ok = false; break; }
+          tc_fence_after();
+          scores(i + 1);
+        }
+        if (i >= 0) {
+          if (!mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
+          tc_fence_after();
+        }
+        if (next) {
+          if (!wait_stage(2 * (i + 1) + 1)) { ok = false; break; }
+          tc_fence_after();
+          grads(i + 1);
+        }
+        if (i >= 0) {
+          if (elect_one()) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDQ, tmem + (i & 1) * 128, slot(2 * i), i > 0);
+            else wt_mma_tokens_halves<1>(tDQ, tmem + (i & 1) * 128, slot(2 * i), i > 0);
+            umma_commit(&empty[(2 * i) % C::STAGES]);
+            if (!next) umma_commit(o_full);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    regs_more<kWtBwdMany>();
+    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, l = l0 + row, st = threadIdx.x - 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const float c2 = w.scale2;
+    const bool biased = w.buckets.count > 0;
+    const int64_t at = ((int64_t)b * w.H + h) * w.L + l;
+    const float2 stat = l < queries ? p.stats[at] : make_float2(0.f, INFINITY);
+    const float delta = l < queries ? p.delta[at] : 0.f;
+    const uint64_t nm = pack2(-stat.x, -stat.x), nl = pack2(-stat.y, -stat.y), nd = pack2(-delta, -delta);
+    float* my_bsum = bsum + sw * 2 * kWinMaxBuckets;
+    float* my_diag = diag + sw * 4 * 48;
+    float flat_sum = 0.f;
+    int flat_bucket = -1;
+    auto flush = [&]() {
+      const float t = warp_sum(flat_sum);
+      if (flat_bucket >= 0 && lane == 0) my_bsum[flat_bucket] += t;
+      __syncwarp();
+      flat_sum = 0.f;
+    };
+    bool ok = true;
+    int turn = 0;                       // of the tiles with more than one bucket: each has a barrier, two tables are enough
+    for (int i = 0; i < n; ++i) {
+      const int s0 = own.at(i) * kWtTile;
+      float flat = 0.f;
+      const float* bias = nullptr;
+      const uint8_t* bucket = nullptr;
+      if (biased) {
+        const int low = s0 - l0 - (kWtTile - 1), bl = win_bucket(w.buckets, low);
+        if (bl == win_bucket(w.buckets, low + 2 * (kWtTile - 1))) {
+          flat = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bl]));
+          if (bl != flat_bucket) { flush(); flat_bucket = bl; }
+        } else {
+          float* to = lut + turn * 256;
+          if (st < 255) {
+            const int bk = win_bucket(w.buckets, low + st);
+            to[st] = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bk]));
+            of[turn * 256 + st] = (uint8_t)bk;
+          }
+          bar_group(1, kWtSoft);
+          bias = to + (kWtTile - 1 - row) + half * 64;
+          bucket = of + turn * 256;
+          turn ^= 1;
+        }
+      }
+      if (!mbar_wait_warp(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, p.status, 0x1000u)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t tS = tmem + lanes + (i & 1) * 128 + half * 64;
+      float d[64];
+      const bool apart = bias == nullptr && wt_apart(c2, flat);
+      const float off = (flat - stat.x) - stat.y;
+      const uint64_t mul2_ = pack2(c2, c2), off2_ = pack2(off, off), flat2_ = pack2(flat, flat);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_ld32(tS + q * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const uint64_t s2 = pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+          uint64_t y;
+          if (apart) y = fma2(s2, mul2_, off2_);
+          else if (bias != nullptr) y = add2(add2(fma2(s2, mul2_, pack2(bias[q * 32 + j], bias[q * 32 + j + 1])), nm), nl);
+          else y = add2(add2(fma2(s2, mul2_, flat2_), nm), nl);
+          float e0, e1;
+          unpack2(y, e0, e1);
+          d[q * 32 + j] = ex2(e0); d[q * 32 + j + 1] = ex2(e1);
+        }
+      }
+      if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
+      tc_fence_after();
+      const bool whole = wt_all_seen(w, l0, queries, s0, keys);
+      const WtSeen seen = wt_seen(w, l, queries, s0, keys);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_ld32(tDP + lanes + half * 64 + q * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const uint64_t y = mul2(add2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), nd), pack2(d[q * 32 + j], d[q * 32 + j + 1]));
+          unpack2(y, d[q * 32 + j], d[q * 32 + j + 1]);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (!wt_sees(w, seen, l, s0, half * 64 + q * 32 + j)) d[q * 32 + j] = 0.f;
+        }
+      }
+      {
+        uint32_t v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+        tmem_st32(tS, v);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+      if (biased) {
+        if (bucket == nullptr) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 64; ++j) part[j & 3] += d[j];
+          flat_sum += (part[0] + part[1]) + (part[2] + part[3]);
+        } else {
+          // 16 columns at a time: a lane hands the sum of its diagonal r - j on to the next lane's column; lane 31's is complete
+          float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              a[c] += d[16 * c + j];
+              if (j < 15) {
+                if (lane == 31) my_diag[c * 48 + 46 - j] = a[c];                // diagonal d at d + 15
+                const float up = __shfl_up_sync(0xffffffffu, a[c], 1);
+                a[c] = lane == 0 ? 0.f : up;
+              }
+            }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) my_diag[c * 48 + lane] = a[c];            // r - 15
+          __syncwarp();
+#pragma unroll
+          for (int part = 0; part < 3; ++part) {
+            const int D = part * 32 + lane;                                     // r - j + 63 over the warp's 64 columns, 95 of them
+            float t = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int k = D - 63 + 16 * c + 15;
+              if (k >= 0 && k < 47 && D < 95) t += my_diag[c * 48 + k];
+            }
+            // rel - low = j_tile - r_tile + 127
+            const int bk = bucket[min(254, max(0, (63 - D) + half * 64 - quarter * 32 + 127))];
+            const int mine = D < 95 ? bk : -1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const float up = __shfl_up_sync(0xffffffffu, t, o);
+              const int other = __shfl_up_sync(0xffffffffu, mine, o);
+              if (lane >= o && other == mine) t += up;
+            }
+            const int following = __shfl_down_sync(0xffffffffu, mine, 1);
+            if (mine >= 0 && (lane == 31 || following != mine)) my_bsum[mine] += t;
+            __syncwarp();
+          }
+        }
+      }
+    }
+    if (ok && biased) {
+      flush();
+      bar_group(1, kWtSoft);
+      if (st < p.columns) {
+        float t = 0.f;
+        for (int x = 0; x < 8; ++x) t += bsum[x * 2 * kWinMaxBuckets + st];
+        p.partial[((int64_t)tile * w.B * w.H + (int64_t)b * w.H + h) * p.columns + st] = t;
+      }
+    }
+    if (ok && n > 0) ok = mbar_wait_warp(o_full, 0, p.status, 0x4000u);
+    if (ok) {
+      tc_fence_after();
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.dq) + (((int64_t)b * w.L + l) * w.H + h) * w.D;
+      bool fine = true;
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        const int c0 = half * NB * 32 + q * 32;
+        if (c0 >= w.D) break;
+        uint32_t v[32] = {};
+        if (n > 0) {
+          tmem_ld32(tDQ + lanes + c0, v);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float a = __uint_as_float(v[j + 2 * k]) * w.scale, c = __uint_as_float(v[j + 2 * k + 1]) * w.scale;
+            if (c0 + j < w.D) fine = fine && isfinite(a) && isfinite(c);
+            o[k] = l < queries ? pack_bf16(a, c) : 0u;
+          }
+          if (l < w.L && c0 + j < w.D) *reinterpret_cast<uint4*>(out + c0 + j) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      if (l < queries && !fine) bad[row] = 1;
+      bar_group(1, kWtSoft);
+      for (int r = sw; r < kWtTile; r += 8)
+        if (bad[r]) {
+          const int64_t ar = ((int64_t)b * w.H + h) * w.L + l0 + r;
+          win_row_dq<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dq), p.dx, p.stats[ar], p.delta[ar], l0 + r, h, b, keys);
+        }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0) drain_after_abort();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int NB>
+__global__ void __launch_bounds__(kWtBwdThreads, 1)
+win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WtBwdParams p) {
+  using C = WtBwd<NB>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
+  float* cols = lut + 2 * 256;                                                     // [parity][-m2, -log2 sum, -delta][128]
+  int* bad = reinterpret_cast<int*>(cols + 2 * 3 * 128);                           // [128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bad + 128);
+  uint64_t *k_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 1, *p_ready = dp_full + 1,
+           *ds_ready = p_ready + 1, *o_full = ds_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  const uint32_t sK = base, sV = base + C::TILE, sQG = base + 2 * C::TILE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WinParams& w = p.w;
+  const int tile = blockIdx.x % p.tiles, gb = blockIdx.x / p.tiles, g = gb % w.Hkv, b = gb / w.Hkv, s0 = tile * kWtTile;
+  const int queries = win_tokens(w, b, w.L), keys = win_tokens(w, b, w.S);
+  int lo, hi;
+  win_query_range(w, s0, min(s0 + kWtTile, keys), queries, &lo, &hi);
+  const int first = lo / kWtTile, per_head = s0 < keys && lo < hi ? (hi + kWtTile - 1) / kWtTile - first : 0, n = per_head * w.rep;
+
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(o_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x < 128) bad[threadIdx.x] = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tDP = tmem + 128, tDV = tmem + 256, tDK = tmem + 384;
+
+  if (warp < 4) {
+    regs_less<kWtBwdFew>();
+    if (warp == 0 && n > 0) {
+      if (elect_one()) {
+        mbar_expect_tx(k_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
+        for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sK + x * kWtBox, &tmK, x * 64, g, s0, b, k_full);
+        for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sV + x * kWtBox, &tmV, x * 64, g, s0, b, k_full);
+      }
+      __syncwarp();
+      uint32_t stage = 0, phase = 0;
+      for (int i = 0; i < 2 * n; ++i) {
+        if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) break;
+        if (elect_one()) {
+          const bool is_q = (i & 1) == 0;
+          const int boxes = is_q ? p.boxes_d : p.boxes_e, it = i >> 1, h = g * w.rep + it / per_head, l0 = (first + it % per_head) * kWtTile;
+          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
+          for (int x = 0; x < boxes; ++x) tma_load_4d(sQG + stage * C::TILE + x * kWtBox, is_q ? &tmQ : &tmG, x * 64, h, l0, b, &full[stage]);
+        }
+        __syncwarp();
+        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+      }
+    } else if (warp == 1 && n > 0) {
+      bool ok = mbar_wait_uniform(k_full, 0, p.status, 0x200u);
+      auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
+      auto slot = [&](int i) { return sQG + (uint32_t)(i % C::STAGES) * C::TILE; };
+      for (int i = -1; i < n && ok; ++i) {
+        const bool next = i + 1 < n;
+        if (i >= 0) {
+          if (!mbar_wait_uniform(p_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, slot(2 * i + 1), i > 0);
+            else wt_mma_tokens_halves<1>(tDV, tmem, slot(2 * i + 1), i > 0);
+            umma_commit(&empty[(2 * i + 1) % C::STAGES]);
+          }
+          __syncwarp();
+        }
+        if (next) {
+          if (!wait_stage(2 * (i + 1))) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, slot(2 * (i + 1)));
+            else wt_mma_features<1>(tmem, sK, slot(2 * (i + 1)));
+            umma_commit(s_full);
+          }
+          __syncwarp();
+        }
+        if (i >= 0) {
+          if (!mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x8000u)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, slot(2 * i), i > 0);
+            else wt_mma_tokens_halves<1>(tDK, tDP, slot(2 * i), i > 0);
+            umma_commit(&empty[(2 * i) % C::STAGES]);
+            if (!next) umma_commit(o_full);
+          }
+          __syncwarp();
+        }
+        if (next) {
+          if (!wait_stage(2 * (i + 1) + 1)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, slot(2 * (i + 1) + 1));
+            else wt_mma_features<1>(tDP, sV, slot(2 * (i + 1) + 1));
+            umma_commit(dp_full);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    regs_more<kWtBwdMany>();
+    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, s = s0 + row, st = threadIdx.x - 128;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tD = tDP + lanes + half * 64;
+    const float c2 = w.scale2;
+    const bool biased = w.buckets.count > 0;
+    // the stats of a tile's queries: threads 0-127 bring the softmax's two, the others delta
+    auto fetch = [&](int i) {
+      float2 f = make_float2(0.f, INFINITY);
+      const int h = g * w.rep + i / per_head, l = (first + i % per_head) * kWtTile + (st & 127);
+      const int64_t at = ((int64_t)b * w.H + h) * w.L + l;
+      if (st < 128) { if (l < queries) f = p.stats[at]; }
+      else f.x = l < queries ? p.delta[at] : 0.f;
+      return f;
+    };
+    float2 coming = n > 0 ? fetch(0) : make_float2(0.f, 0.f);
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int h = g * w.rep + i / per_head, l0 = (first + i % per_head) * kWtTile;
+      float* col = cols + (i & 1) * 3 * 128;
+      if (st < 128) { col[st] = -coming.x; col[128 + st] = -coming.y; }
+      else col[256 + st - 128] = -coming.x;
+      float flat = 0.f;
+      const float* bias = nullptr;
+      if (biased) {
+        const int low = s0 - l0 - (kWtTile - 1), bl = win_bucket(w.buckets, low);
+        if (bl == win_bucket(w.buckets, low + 2 * (kWtTile - 1))) {
+          flat = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bl]));
+        } else {                                   // index (column - row) + 127: rel = low + 254 - index
+          float* to = lut + (i & 1) * 256;
+          if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, h, low + 254 - st);
+          bias = to + (kWtTile - 1 - row) + half * 64;
+        }
+      }
+      bar_group(1, kWtSoft);
+      if (i + 1 < n) coming = fetch(i + 1);
+      // the queries that see key s: columns from..to
+      int from = w.causal ? s - l0 : (s < w.sinks ? 0 : s - w.window + 1 - l0);
+      int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
+      if (s >= keys) to = -1;
+      const bool whole = wt_all_seen(w, l0, queries, s0, keys);
+      if (!mbar_wait_warp(s_full, (uint32_t)i & 1u, p.status, 0x1000u)) { ok = false; break; }
+      tc_fence_after();
+      float d[64];
+      const bool apart = bias == nullptr && wt_apart(c2, flat);
+      const uint64_t mul2_ = pack2(c2, c2), flat2_ = pack2(flat, flat);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_ld32(tS + q * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 m = lds4(col + half * 64 + q * 32 + j), e = lds4(col + 128 + half * 64 + q * 32 + j);
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const uint64_t s2 = pack2(__uint_as_float(v[j + k]), __uint_as_float(v[j + k + 1]));
+            const uint64_t nm = k == 0 ? pack2(m.x, m.y) : pack2(m.z, m.w), nl = k == 0 ? pack2(e.x, e.y) : pack2(e.z, e.w);
+            uint64_t y;
+            if (apart) y = add2(fma2(s2, mul2_, add2(flat2_, nm)), nl);
+            else if (bias != nullptr) y = add2(add2(fma2(s2, mul2_, pack2(bias[q * 32 + j + k], bias[q * 32 + j + k + 1])), nm), nl);
+            else y = add2(add2(fma2(s2, mul2_, flat2_), nm), nl);
+            float e0, e1;
+            unpack2(y, e0, e1);
+            d[q * 32 + j + k] = ex2(e0); d[q * 32 + j + k + 1] = ex2(e1);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int c = half * 64 + q * 32 + j;
+            if (c < from || c > to) d[q * 32 + j] = 0.f;
+          }
+        }
+      }
+      {
+        uint32_t v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+        tmem_st32(tS, v);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_ready);
+      if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t o[32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_ld32(tD + q * 32, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 e = lds4(col + 256 + half * 64 + q * 32 + j);
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const uint64_t y = mul2(add2(pack2(__uint_as_float(v[j + k]), __uint_as_float(v[j + k + 1])), k == 0 ? pack2(e.x, e.y) : pack2(e.z, e.w)),
+                                    pack2(d[q * 32 + j + k], d[q * 32 + j + k + 1]));
+            unpack2(y, d[q * 32 + j + k], d[q * 32 + j + k + 1]);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int c = half * 64 + q * 32 + j;
+            if (c < from || c > to) d[q * 32 + j] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[q * 16 + j] = pack_bf16(d[q * 32 + 2 * j], d[q * 32 + 2 * j + 1]);
+      }
+      tmem_st32(tD, o);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) ok = mbar_wait_warp(o_full, 0, p.status, 0x4000u);
+    if (ok) {
+      tc_fence_after();
+      bool fine = true;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const int width = which == 0 ? w.D : w.E;
+        const float f = which == 0 ? w.scale : 1.f;
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * w.S + s) * w.Hkv + g) * width;
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+          const int c0 = half * NB * 32 + q * 32;
+          if (c0 >= width) break;
+          uint32_t v[32] = {};
+          if (n > 0) {
+            tmem_ld32((which == 0 ? tDK : tDV) + lanes + c0, v);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a = __uint_as_float(v[j + 2 * k]) * f, c = __uint_as_float(v[j + 2 * k + 1]) * f;
+              if (c0 + j < width) fine = fine && isfinite(a) && isfinite(c);
+              x[k] = s < keys ? pack_bf16(a, c) : 0u;
+            }
+            if (s < w.S && c0 + j < width) *reinterpret_cast<uint4*>(out + c0 + j) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+      if (s < keys && !fine) bad[row] = 1;
+      bar_group(1, kWtSoft);
+      for (int r = sw; r < kWtTile; r += 8)
+        if (bad[r])
+          win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s0 + r, g, b, queries);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*reinterpret_cast<volatile unsigned int*>(p.status) != 0) drain_after_abort();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+int64_t win_tc_partials(const lb2_window_dims* d) { return (d->queries + kWtTile - 1) / kWtTile; }
+
+int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* partial, const void* dx, const float2* stats, const float* delta,
+                   cudaStream_t st) {
+  WtBwdParams p{};
+  p.w = w; p.dq = dq; p.dk = dk; p.dv = dv; p.dx = dx; p.stats = stats; p.delta = delta; p.partial = partial;
+  p.columns = w.buckets.count * (w.buckets.bidirectional ? 2 : 1);
+  p.boxes_d = (w.D + 63) / 64; p.boxes_e = (w.E + 63) / 64;
+  p.status = device_status_word();
+  LB2_REQUIRE(p.status != nullptr, LB2_LAUNCH_FAIL, "windowed attention: device status word unavailable");
+  CUtensorMap mq, mg, mk, mv;
+  if (!wt_encode(&mq, w.q, w.D, w.H, w.L, w.B) || !wt_encode(&mg, dx, w.E, w.H, w.L, w.B) || !wt_encode(&mk, w.k, w.D, w.Hkv, w.S, w.B) ||
+      !wt_encode(&mv, w.v, w.E, w.Hkv, w.S, w.B))
+    return fail(LB2_LAUNCH_FAIL, "windowed attention: cuTensorMapEncodeTiled failed");
+  const int64_t qt = (w.L + kWtTile - 1) / kWtTile, kt = (w.S + kWtTile - 1) / kWtTile;
+  LB2_REQUIRE(qt * w.H * w.B <= 0x7FFFFFFF && kt * w.Hkv * w.B <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
+  auto launch = [&](auto kernel, int smem, int64_t tiles, int64_t blocks) -> int32_t {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+    p.tiles = (int)tiles;
+    kernel<<<(unsigned)blocks, kWtBwdThreads, smem, st>>>(mq, mg, mk, mv, p);
+    LB2_CHECK_LAUNCH("windowed attention pullback");
+    return LB2_OK;
+  };
+  const bool one = p.boxes_d == 1 && p.boxes_e == 1;
+  int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, qt * w.H * w.B) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, qt * w.H * w.B);
+  if (rc != LB2_OK) return rc;
+  return one ? launch(win_tc_dkv_kernel<1>, WtBwd<1>::SMEM, kt, kt * w.Hkv * w.B) : launch(win_tc_dkv_kernel<2>, WtBwd<2>::SMEM, kt, kt * w.Hkv * w.B);
+}
+
+}  // namespace lb2
