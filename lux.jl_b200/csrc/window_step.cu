@@ -4,8 +4,10 @@
 // A cache of `capacity` slots holds position p in slot p while p < sinks, and later ones in
 // sinks + (p - sinks) mod (capacity - sinks): the sinks stay, the rest is overwritten oldest first. With
 // capacity >= sinks + window all that the new token sees is there.
+#include <type_traits>
+
 #include "common.cuh"
-#include "window.cuh"
+#include "window_tc.cuh"
 
 namespace lb2 {
 
@@ -22,7 +24,363 @@ struct StepParams {
   lb2_rel_buckets buckets;
 };
 
-// a block per (sequence, head); its warps take the keys in turn
+// The keys that the new token at position n sees: n - lo + 1 of the window, `early` sinks before them. Key i lies in slot(i).
+struct StepKeys {
+  int count, early, first, capacity, ring;        // first: slot of the window's oldest key
+  __device__ __forceinline__ StepKeys(const StepParams& p, int n) {
+    const int lo = max(0, n - p.window + 1);
+    capacity = p.C; ring = p.C - p.sinks;
+    early = min(p.sinks, lo);
+    count = early + (n - lo + 1);
+    first = (int)ring_slot(lo, p.sinks, ring);
+  }
+  // lo < sinks: no slot has been taken twice among the visible ones, and key i is position and slot i
+  __device__ __forceinline__ int64_t slot(int i) const {
+    if (i < early) return i;
+    const int s = first + (i - early);
+    return s < capacity ? s : s - ring;
+  }
+  __device__ __forceinline__ int distance(int i, int n) const { return i < early ? n - i : count - 1 - i; }
+};
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// ---- the kernels of long caches ----------------------------------------------------------------
+// A cluster of blocks per (sequence, key head, up to R of its query heads) splits the visible keys; every key and value is read once
+// for all R heads. Each warp (Float32: part of a warp) keeps its own running maximum, sum and accumulators; the block joins its
+// warps', the cluster its blocks' through distributed shared memory, so there is no workspace and the order is fixed.
+// Bounded by the cache's bytes: see the measured figures below.
+constexpr int kStepThreads = 128, kStepWarps = 4;
+
+template <int R, int DV, int PARTS> struct StepJoin {
+  float o[PARTS][R][DV], m[PARTS][R], s[PARTS][R];
+  float bias[R][2 * kWinMaxBuckets];
+};
+template <typename T, int R, int DV, int PARTS>
+__device__ __forceinline__ void step_join(StepJoin<R, DV, PARTS>& j, const StepParams& p, T* x, int heads) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < R * DV; i += kStepThreads) {
+    const int r = i / DV, c = i % DV;
+    float top = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) top = fmaxf(top, j.m[q][r]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float a = 0.f;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) a = fmaf(j.o[q][r][c], exp2f(j.m[q][r] - ref), a);
+    j.o[0][r][c] = a;                              // read and written by this thread alone
+  }
+  __syncthreads();
+  if (tid < R) {
+    float top = -INFINITY, t = 0.f;
+    for (int q = 0; q < PARTS; ++q) top = fmaxf(top, j.m[q][tid]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int q = 0; q < PARTS; ++q) t = fmaf(j.s[q][tid], exp2f(j.m[q][tid] - ref), t);
+    j.m[0][tid] = top; j.s[0][tid] = t;
+  }
+  uint32_t blocks;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(blocks));
+  __syncthreads();                                 // warps converge before the aligned barrier
+  cluster_sync_all();
+  const uint32_t rank = cluster_cta_rank(), mo = smem_u32(&j.m[0][0]), so = smem_u32(&j.s[0][0]), oo = smem_u32(&j.o[0][0][0]);
+  for (int i = tid + (int)rank * kStepThreads; i < heads * DV; i += kStepThreads * (int)blocks) {
+    const int r = i / DV, c = i % DV;
+    float top = -INFINITY;
+    for (uint32_t q = 0; q < blocks; ++q) top = fmaxf(top, ld_cluster_f32(map_to_cta(mo + 4 * r, q)));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float a = 0.f, t = 0.f;
+    for (uint32_t q = 0; q < blocks; ++q) {
+      const float f = exp2f(ld_cluster_f32(map_to_cta(mo + 4 * r, q)) - ref);
+      t = fmaf(ld_cluster_f32(map_to_cta(so + 4 * r, q)), f, t);
+      a = fmaf(ld_cluster_f32(map_to_cta(oo + 4 * i, q)), f, a);
+    }
+    if (c < p.E) x[r * p.E + c] = from_f32<T>(a / t);
+  }
+  __syncthreads();
+  cluster_sync_all();                              // nobody leaves while its shared memory is read
+}
+
+// What the kernels below have in common; `head0` is the first of up to R heads, `rank` of `blocks` the block's place in its cluster.
+struct StepPlace {
+  int b, g, head0, heads, n;
+  uint32_t rank, blocks;
+};
+template <int R> __device__ __forceinline__ StepPlace step_place(const StepParams& p) {
+  StepPlace w;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(w.blocks));
+  w.rank = cluster_cta_rank();
+  const int groups = (p.rep + R - 1) / R;
+  int item = blockIdx.x / w.blocks;
+  const int hg = item % groups;
+  item /= groups;
+  w.g = item % p.Hkv; w.b = item / p.Hkv;
+  w.head0 = w.g * p.rep + hg * R;
+  w.heads = min(R, p.rep - hg * R);
+  w.n = p.lengths[w.b];
+  return w;
+}
+// zeros where there is no sequence; the new row into the cache; the heads' bias per bucket
+template <typename T, int R> __device__ __forceinline__ void step_edges(const StepParams& p, const StepPlace& w, float (*bias)[2 * kWinMaxBuckets]) {
+  if (w.n < 0) {
+    T* x = static_cast<T*>(p.x) + ((int64_t)w.b * p.H + w.head0) * p.E;
+    if (w.rank == 0)
+      for (int i = threadIdx.x; i < w.heads * p.E; i += kStepThreads) x[i] = from_f32<T>(0.f);
+    return;
+  }
+  if (w.rank == 0 && w.head0 % p.rep == 0) {       // the slot holds nothing that is seen: no block reads it
+    const int64_t row = ((int64_t)w.b * p.C + ring_slot(w.n, p.sinks, p.C - p.sinks)) * p.Hkv + w.g, in = (int64_t)w.b * p.Hkv + w.g;
+    for (int i = threadIdx.x; i < p.D; i += kStepThreads) static_cast<T*>(p.kcache)[row * p.D + i] = static_cast<const T*>(p.k)[in * p.D + i];
+    for (int i = threadIdx.x; i < p.E; i += kStepThreads) static_cast<T*>(p.vcache)[row * p.E + i] = static_cast<const T*>(p.v)[in * p.E + i];
+  }
+  const int columns = p.buckets.count * (p.buckets.bidirectional ? 2 : 1);
+  for (int i = threadIdx.x; i < w.heads * columns; i += kStepThreads)
+    bias[i % w.heads][i / w.heads] = win_bias2(to_f32(static_cast<const T*>(p.table)[w.head0 + i % w.heads + (int64_t)p.H * (i / w.heads)]));
+}
+// the share of `count` keys, in groups of `unit`, of a block
+__device__ __forceinline__ void step_share(int count, int unit, const StepPlace& w, int* from, int* to) {
+  const int groups = (count + unit - 1) / unit;
+  *from = (int)((int64_t)groups * w.rank / w.blocks) * unit;
+  *to = min(count, (int)((int64_t)groups * (w.rank + 1) / w.blocks) * unit);
+}
+
+// ---- BFloat16 -----------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// A warp takes 16 keys at a time. S[heads][keys] = Q K' and O[heads][features] += P V as m16n8k16 products (too small and too ragged for
+// the TMEM path, and the cache's bytes bound them). The features of a contraction may come in any order, so a lane takes eight
+// neighbouring ones of a key's row with one 16-byte load as its share of two steps; for V it joins two keys' rows by halves.
+template <int DC, int R>
+__global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __grid_constant__ StepParams p) {
+  using T = __nv_bfloat16;
+  static_assert(R == 8 || R == 16, "rows of an m16 tile");
+  __shared__ StepJoin<R, DC, kStepWarps> j;
+  const StepPlace w = step_place<R>(p);
+  step_edges<T, R>(p, w, j.bias);
+  if (w.n < 0) return;                             // the whole cluster
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, u = lane >> 2, t = lane & 3;
+  const StepKeys keys(p, w.n);
+  const int64_t in = (int64_t)w.b * p.Hkv + w.g, row0 = (int64_t)w.b * p.C * p.Hkv + w.g;
+  const T* kc = static_cast<const T*>(p.kcache) + row0 * p.D;
+  const T* vc = static_cast<const T*>(p.vcache) + row0 * p.E;
+  const T* kn = static_cast<const T*>(p.k) + in * p.D;
+  const T* vn = static_cast<const T*>(p.v) + in * p.E;
+  const int64_t ks = (int64_t)p.Hkv * p.D, vs = (int64_t)p.Hkv * p.E;
+  constexpr int KC = DC / 32, VC = DC / 64;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 q[R / 8][KC];
+#pragma unroll
+  for (int a = 0; a < R / 8; ++a)
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+      q[a][c] = u + 8 * a < w.heads && c * 32 + t * 8 < p.D
+                    ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + ((int64_t)w.b * p.H + w.head0 + u + 8 * a) * p.D + c * 32 + t * 8)
+                    : zero;
+  float o[VC][8][R / 4];
+#pragma unroll
+  for (int c = 0; c < VC; ++c)
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+      for (int k = 0; k < R / 4; ++k) o[c][f][k] = 0.f;
+  float m[R / 8], sum[R / 8];
+#pragma unroll
+  for (int a = 0; a < R / 8; ++a) { m[a] = -INFINITY; sum[a] = 0.f; }
+
+  int from, to;
+  step_share(keys.count, 16, w, &from, &to);
+  for (int i0 = from + warp * 16; i0 < to; i0 += kStepWarps * 16) {
+    uint4 kv[2][KC], vv[4][VC];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      const int i = i0 + tile * 8 + u;
+      const T* at = i == keys.count - 1 ? kn : kc + keys.slot(i) * ks;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kv[tile][c] = i < to && c * 32 + t * 8 < p.D ? *reinterpret_cast<const uint4*>(at + c * 32 + t * 8) : zero;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = i0 + (r >> 1) * 8 + 2 * t + (r & 1);
+      const T* at = i == keys.count - 1 ? vn : vc + keys.slot(i) * vs;
+#pragma unroll
+      for (int c = 0; c < VC; ++c) vv[r][c] = i < to && c * 64 + u * 8 < p.E ? *reinterpret_cast<const uint4*>(at + c * 64 + u * 8) : zero;
+    }
+    float s[2][4];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+      s[tile][0] = s[tile][1] = s[tile][2] = s[tile][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 lo = q[0][c], hi = R == 16 ? q[R / 8 - 1][c] : zero;
+        mma_bf16(s[tile], lo.x, hi.x, lo.y, hi.y, kv[tile][c].x, kv[tile][c].y);
+        mma_bf16(s[tile], lo.z, hi.z, lo.w, hi.w, kv[tile][c].z, kv[tile][c].w);
+      }
+    }
+    float z[R / 8][4], top[R / 8];                 // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+    for (int a = 0; a < R / 8; ++a) top[a] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + (k >> 1) * 8 + 2 * t + (k & 1);
+      const int bk = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, -keys.distance(i, w.n)) : 0;
+#pragma unroll
+      for (int a = 0; a < R / 8; ++a) {
+        float v = s[k >> 1][2 * a + (k & 1)] * p.scale2;
+        if (p.buckets.count > 0 && u + 8 * a < w.heads) v += j.bias[u + 8 * a][bk];
+        z[a][k] = i < to ? v : -INFINITY;
+        top[a] = fmaxf(top[a], z[a][k]);
+      }
+    }
+    bool grow = false;
+#pragma unroll
+    for (int a = 0; a < R / 8; ++a) {
+      top[a] = fmaxf(top[a], __shfl_xor_sync(0xffffffffu, top[a], 1));
+      top[a] = fmaxf(top[a], __shfl_xor_sync(0xffffffffu, top[a], 2));
+      grow = grow || top[a] > m[a] + 8.f;
+    }
+    if (__any_sync(0xffffffffu, grow)) {           // weights up to 2^8 are as exact in bf16
+#pragma unroll
+      for (int a = 0; a < R / 8; ++a) {
+        const float to_m = top[a] > m[a] + 8.f ? top[a] : m[a], keep = to_m == m[a] ? 1.f : ex2(m[a] - to_m);
+        m[a] = to_m;
+        sum[a] *= keep;
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+          for (int f = 0; f < 8; ++f) { o[c][f][2 * a] *= keep; o[c][f][2 * a + 1] *= keep; }
+      }
+    }
+    uint32_t pa[R / 8][2];
+#pragma unroll
+    for (int a = 0; a < R / 8; ++a) {
+      const float ref = m[a] == -INFINITY ? 0.f : m[a];
+      float e[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e[k] = ex2(z[a][k] - ref);
+      sum[a] += (e[0] + e[1]) + (e[2] + e[3]);
+      pa[a][0] = pack_bf16(e[0], e[1]);
+      pa[a][1] = pack_bf16(e[2], e[3]);
+    }
+#pragma unroll
+    for (int c = 0; c < VC; ++c) {
+      const uint32_t w0[4] = {vv[0][c].x, vv[0][c].y, vv[0][c].z, vv[0][c].w}, w1[4] = {vv[1][c].x, vv[1][c].y, vv[1][c].z, vv[1][c].w};
+      const uint32_t w2[4] = {vv[2][c].x, vv[2][c].y, vv[2][c].z, vv[2][c].w}, w3[4] = {vv[3][c].x, vv[3][c].y, vv[3][c].z, vv[3][c].w};
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        const uint32_t b0 = __byte_perm(w0[f >> 1], w1[f >> 1], f & 1 ? 0x7632 : 0x5410), b1 = __byte_perm(w2[f >> 1], w3[f >> 1], f & 1 ? 0x7632 : 0x5410);
+        float d[4] = {o[c][f][0], o[c][f][1], R == 16 ? o[c][f][R / 4 - 2] : 0.f, R == 16 ? o[c][f][R / 4 - 1] : 0.f};
+        mma_bf16(d, pa[0][0], R == 16 ? pa[R / 8 - 1][0] : 0u, pa[0][1], R == 16 ? pa[R / 8 - 1][1] : 0u, b0, b1);
+#pragma unroll
+        for (int k = 0; k < R / 4; ++k) o[c][f][k] = d[k];
+      }
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < R / 8; ++a) {
+    sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 1);
+    sum[a] += __shfl_xor_sync(0xffffffffu, sum[a], 2);
+    if (t == 0) { j.m[warp][u + 8 * a] = m[a]; j.s[warp][u + 8 * a] = sum[a]; }
+#pragma unroll
+    for (int c = 0; c < VC; ++c)
+#pragma unroll
+      for (int f = 0; f < 8; ++f)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) j.o[warp][u + 8 * a][c * 64 + (2 * t + k) * 8 + f] = o[c][f][2 * a + k];
+  }
+  step_join<T>(j, p, static_cast<T*>(p.x) + ((int64_t)w.b * p.H + w.head0) * p.E, w.heads);
+}
+
+// ---- Float32 ------------------------------------------------------------------------------------
+// LPR lanes share a key's row, four features each; 32 / LPR keys per warp and load, four loads at a time.
+template <int LPR, int R>
+__global__ void __launch_bounds__(kStepThreads) win_step_f32_kernel(const __grid_constant__ StepParams p) {
+  constexpr int DC = LPR * 4, PER = 32 / LPR, PARTS = kStepWarps * PER, U = 4;
+  extern __shared__ __align__(16) uint8_t raw[];
+  auto& j = *reinterpret_cast<StepJoin<R, DC, PARTS>*>(raw);
+  const StepPlace w = step_place<R>(p);
+  step_edges<float, R>(p, w, j.bias);
+  if (w.n < 0) return;
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp * PER + lane / LPR, c = (lane % LPR) * 4;
+  const StepKeys keys(p, w.n);
+  const int64_t in = (int64_t)w.b * p.Hkv + w.g, row0 = (int64_t)w.b * p.C * p.Hkv + w.g;
+  const float* kc = static_cast<const float*>(p.kcache) + row0 * p.D;
+  const float* vc = static_cast<const float*>(p.vcache) + row0 * p.E;
+  const float* kn = static_cast<const float*>(p.k) + in * p.D;
+  const float* vn = static_cast<const float*>(p.v) + in * p.E;
+  const int64_t ks = (int64_t)p.Hkv * p.D, vs = (int64_t)p.Hkv * p.E;
+  const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 q[R], o[R];
+  float m[R], sum[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    q[r] = r < w.heads && c < p.D ? *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + ((int64_t)w.b * p.H + w.head0 + r) * p.D + c) : zero;
+    o[r] = zero; m[r] = -INFINITY; sum[r] = 0.f;
+  }
+  int from, to;
+  step_share(keys.count, PARTS, w, &from, &to);
+  for (int i0 = from; i0 < to; i0 += PARTS * U) {      // all lanes of a warp together
+    float4 kv[U], vv[U];
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int i = i0 + x * PARTS + part;
+      const bool fresh = i == keys.count - 1;
+      const int64_t slot = keys.slot(i);
+      kv[x] = i < to && c < p.D ? *reinterpret_cast<const float4*>((fresh ? kn : kc + slot * ks) + c) : zero;
+      vv[x] = i < to && c < p.E ? *reinterpret_cast<const float4*>((fresh ? vn : vc + slot * vs) + c) : zero;
+    }
+    int bk[U];
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int i = i0 + x * PARTS + part;
+      bk[x] = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, -keys.distance(i, w.n)) : 0;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (r >= w.heads) break;
+      float z[U], top = m[r];
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        float d = q[r].x * kv[x].x;
+        d = fmaf(q[r].y, kv[x].y, d);
+        d = fmaf(q[r].z, kv[x].z, d);
+        d = fmaf(q[r].w, kv[x].w, d);
+#pragma unroll
+        for (int s = LPR / 2; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+        d *= p.scale2;
+        if (p.buckets.count > 0) d += j.bias[r][bk[x]];
+        z[x] = i0 + x * PARTS + part < to ? d : -INFINITY;
+        top = fmaxf(top, z[x]);
+      }
+      const float ref = top == -INFINITY ? 0.f : top, keep = exp2f(m[r] - ref);
+      m[r] = top;
+      sum[r] *= keep;
+      o[r].x *= keep; o[r].y *= keep; o[r].z *= keep; o[r].w *= keep;
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const float e = exp2f(z[x] - ref);
+        sum[r] += e;
+        o[r].x = fmaf(e, vv[x].x, o[r].x); o[r].y = fmaf(e, vv[x].y, o[r].y);
+        o[r].z = fmaf(e, vv[x].z, o[r].z); o[r].w = fmaf(e, vv[x].w, o[r].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    *reinterpret_cast<float4*>(&j.o[part][r][c]) = o[r];
+    if (lane % LPR == 0) { j.m[part][r] = m[r]; j.s[part][r] = sum[r]; }
+  }
+  step_join<float>(j, p, static_cast<float*>(p.x) + ((int64_t)w.b * p.H + w.head0) * p.E, w.heads);
+}
+
+// ---- any features: a block per (sequence, head); its warps take the keys in turn -----------------
 template <typename T> __global__ void __launch_bounds__(256) win_step_kernel(const __grid_constant__ StepParams p) {
   __shared__ float so[8][kWinMaxDim], sm[8], ss[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -41,7 +399,7 @@ template <typename T> __global__ void __launch_bounds__(256) win_step_kernel(con
   float q[kWinLaneDims], t[kWinLaneDims], o[kWinLaneDims] = {};
   win_load_lane(static_cast<const T*>(p.q) + ((int64_t)b * p.H + h) * p.D, p.D, lane, q);
   float m = -INFINITY, sum = 0.f;
-  const int lo = max(0, n - p.window + 1), early = min(p.sinks, lo), count = early + (n + 1 - lo);
+  const int lo = max(0, n - p.window + 1), early = min(p.sinks, lo), count = early + (n - lo + 1);
   for (int i = warp; i < count; i += 8) {
     const int s = i < early ? i : lo + (i - early);
     const int64_t slot = ring_slot(s, p.sinks, ring);
@@ -111,6 +469,31 @@ int32_t step_check(const lb2_window_dims* d, const lb2_rel_buckets* t, const voi
   return t == nullptr ? LB2_OK : check_rel_buckets(t);
 }
 
+// Clusters: enough blocks for the device (six per SM even out sequences of different lengths) while each keeps 64 keys or more.
+template <typename K> int32_t step_launch(K kernel, const StepParams& p, const lb2_window_dims* d, int heads_per_block, int smem, cudaStream_t st) {
+  const int64_t items = d->batch * d->kv_heads * ((p.rep + heads_per_block - 1) / heads_per_block), seen = d->window + d->sinks;
+  int blocks = 1;
+  while (blocks < 8 && items * blocks < (int64_t)sm_count() * 6 && seen >= (int64_t)blocks * 2 * 64) blocks *= 2;
+  LB2_REQUIRE(items * blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
+  if (smem > 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention step: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(items * blocks));
+  cfg.blockDim = dim3(kStepThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)blocks; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention step: %s", cudaGetErrorString(e));
+  return LB2_OK;
+}
+
 }  // namespace
 
 }  // namespace lb2
@@ -142,6 +525,23 @@ int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, const voi
   p.scale2 = (float)(scale * 1.4426950408889634);
   if (buckets != nullptr) p.buckets = *buckets;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t per16 = 16 / (int64_t)es;
+  if (d->head_dim > 0 && d->value_dim > 0 && d->head_dim <= 128 && d->value_dim <= 128 && d->head_dim % per16 == 0 && d->value_dim % per16 == 0 &&
+      aligned_to(kcache, 16) && aligned_to(vcache, 16) && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16)) {
+    const int most = p.D > p.E ? p.D : p.E;
+    if (dtype == LB2_BF16) {
+      if (p.rep <= 8) return most <= 64 ? step_launch(win_step_bf16_kernel<64, 8>, p, d, 8, 0, st) : step_launch(win_step_bf16_kernel<128, 8>, p, d, 8, 0, st);
+      return most <= 64 ? step_launch(win_step_bf16_kernel<64, 16>, p, d, 16, 0, st) : step_launch(win_step_bf16_kernel<128, 16>, p, d, 16, 0, st);
+    }
+    auto rows = [&](auto lpr) -> int32_t {
+      constexpr int LPR = decltype(lpr)::value, PARTS = kStepWarps * 32 / LPR;
+      if (p.rep == 1) return step_launch(win_step_f32_kernel<LPR, 1>, p, d, 1, (int)sizeof(StepJoin<1, LPR * 4, PARTS>), st);
+      if (p.rep <= 4) return step_launch(win_step_f32_kernel<LPR, 4>, p, d, 4, (int)sizeof(StepJoin<4, LPR * 4, PARTS>), st);
+      return step_launch(win_step_f32_kernel<LPR, 8>, p, d, 8, (int)sizeof(StepJoin<8, LPR * 4, PARTS>), st);
+    };
+    if (most <= 32) return rows(std::integral_constant<int, 8>{});
+    return most <= 64 ? rows(std::integral_constant<int, 16>{}) : rows(std::integral_constant<int, 32>{});
+  }
   LB2_DISPATCH_DTYPE(dtype, { win_step_kernel<T><<<(unsigned)(d->heads * d->batch), 256, 0, st>>>(p); });
   LB2_CHECK_LAUNCH("windowed attention step");
   return LB2_OK;
