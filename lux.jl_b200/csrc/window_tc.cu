@@ -188,28 +188,26 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       phase ^= 1u;
       tc_fence_after();
       // logits = mul * z + add, mul > 0; what a row does not see is -inf
-      float z[128];
       const bool apart = bias == nullptr && wt_apart(c2, flat);
       const float mul = apart ? c2 : 1.f, add = apart ? flat : 0.f;
-      const bool whole = wt_all_seen(w, l0[grp], queries, s0, keys);
-      const WtSeen seen = wt_seen(w, l, queries, s0, keys);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t v[32];
-        tmem_ld32(tS + q * 32, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) z[q * 32 + j] = __uint_as_float(v[j]);
+      float z[128];
+      tmem_row128<0>(tS, z);
+      if (!apart) {
         if (bias != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(z[q * 32 + j], c2, bias[q * 32 + j]);
-        } else if (!apart) {
+          for (int j = 0; j < 128; ++j) z[j] = fmaf(z[j], c2, bias[j]);
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[q * 32 + j] = fmaf(z[q * 32 + j], c2, flat);
+          for (int j = 0; j < 128; ++j) z[j] = fmaf(z[j], c2, flat);
         }
-        if (!whole) {
+      }
+      if (!wt_all_seen(w, l0[grp], queries, s0, keys)) {
+        const WtSeen seen(w, l, queries, s0, keys);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[q * 32 + j] = wt_sees(w, seen, l, s0, q * 32 + j) ? z[q * 32 + j] : -INFINITY;
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t bits = seen.bits(q * 32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[q * 32 + j] = bits >> j & 1u ? z[q * 32 + j] : -INFINITY;
         }
       }
       float top[4] = {z[0], z[1], z[2], z[3]};

@@ -65,6 +65,57 @@ template <int NB> __device__ __forceinline__ void wt_mma_tokens_halves(uint32_t 
   for (int ks = 0; ks < 8; ++ks)
     umma_ts(d, p + (ks >> 2) * 64 + (ks & 3) * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
+// `N` columns of a row and the wait for them in one statement, so that nothing reads the registers in between
+template <int O, int M> __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&z)[M]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(z[O + 0]), "=f"(z[O + 1]), "=f"(z[O + 2]), "=f"(z[O + 3]), "=f"(z[O + 4]), "=f"(z[O + 5]), "=f"(z[O + 6]), "=f"(z[O + 7]),
+        "=f"(z[O + 8]), "=f"(z[O + 9]), "=f"(z[O + 10]), "=f"(z[O + 11]), "=f"(z[O + 12]), "=f"(z[O + 13]), "=f"(z[O + 14]), "=f"(z[O + 15]),
+        "=f"(z[O + 16]), "=f"(z[O + 17]), "=f"(z[O + 18]), "=f"(z[O + 19]), "=f"(z[O + 20]), "=f"(z[O + 21]), "=f"(z[O + 22]), "=f"(z[O + 23]),
+        "=f"(z[O + 24]), "=f"(z[O + 25]), "=f"(z[O + 26]), "=f"(z[O + 27]), "=f"(z[O + 28]), "=f"(z[O + 29]), "=f"(z[O + 30]), "=f"(z[O + 31]),
+        "=f"(z[O + 32]), "=f"(z[O + 33]), "=f"(z[O + 34]), "=f"(z[O + 35]), "=f"(z[O + 36]), "=f"(z[O + 37]), "=f"(z[O + 38]), "=f"(z[O + 39]),
+        "=f"(z[O + 40]), "=f"(z[O + 41]), "=f"(z[O + 42]), "=f"(z[O + 43]), "=f"(z[O + 44]), "=f"(z[O + 45]), "=f"(z[O + 46]), "=f"(z[O + 47]),
+        "=f"(z[O + 48]), "=f"(z[O + 49]), "=f"(z[O + 50]), "=f"(z[O + 51]), "=f"(z[O + 52]), "=f"(z[O + 53]), "=f"(z[O + 54]), "=f"(z[O + 55]),
+        "=f"(z[O + 56]), "=f"(z[O + 57]), "=f"(z[O + 58]), "=f"(z[O + 59]), "=f"(z[O + 60]), "=f"(z[O + 61]), "=f"(z[O + 62]), "=f"(z[O + 63])
+      : "r"(taddr)
+      : "memory");
+}
+template <int O, int M> __device__ __forceinline__ void tmem_row128(uint32_t taddr, float (&z)[M]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63, "
+      "%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, "
+      "%80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95, "
+      "%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, "
+      "%112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%128];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(z[O + 0]), "=f"(z[O + 1]), "=f"(z[O + 2]), "=f"(z[O + 3]), "=f"(z[O + 4]), "=f"(z[O + 5]), "=f"(z[O + 6]), "=f"(z[O + 7]),
+        "=f"(z[O + 8]), "=f"(z[O + 9]), "=f"(z[O + 10]), "=f"(z[O + 11]), "=f"(z[O + 12]), "=f"(z[O + 13]), "=f"(z[O + 14]), "=f"(z[O + 15]),
+        "=f"(z[O + 16]), "=f"(z[O + 17]), "=f"(z[O + 18]), "=f"(z[O + 19]), "=f"(z[O + 20]), "=f"(z[O + 21]), "=f"(z[O + 22]), "=f"(z[O + 23]),
+        "=f"(z[O + 24]), "=f"(z[O + 25]), "=f"(z[O + 26]), "=f"(z[O + 27]), "=f"(z[O + 28]), "=f"(z[O + 29]), "=f"(z[O + 30]), "=f"(z[O + 31]),
+        "=f"(z[O + 32]), "=f"(z[O + 33]), "=f"(z[O + 34]), "=f"(z[O + 35]), "=f"(z[O + 36]), "=f"(z[O + 37]), "=f"(z[O + 38]), "=f"(z[O + 39]),
+        "=f"(z[O + 40]), "=f"(z[O + 41]), "=f"(z[O + 42]), "=f"(z[O + 43]), "=f"(z[O + 44]), "=f"(z[O + 45]), "=f"(z[O + 46]), "=f"(z[O + 47]),
+        "=f"(z[O + 48]), "=f"(z[O + 49]), "=f"(z[O + 50]), "=f"(z[O + 51]), "=f"(z[O + 52]), "=f"(z[O + 53]), "=f"(z[O + 54]), "=f"(z[O + 55]),
+        "=f"(z[O + 56]), "=f"(z[O + 57]), "=f"(z[O + 58]), "=f"(z[O + 59]), "=f"(z[O + 60]), "=f"(z[O + 61]), "=f"(z[O + 62]), "=f"(z[O + 63]),
+        "=f"(z[O + 64]), "=f"(z[O + 65]), "=f"(z[O + 66]), "=f"(z[O + 67]), "=f"(z[O + 68]), "=f"(z[O + 69]), "=f"(z[O + 70]), "=f"(z[O + 71]),
+        "=f"(z[O + 72]), "=f"(z[O + 73]), "=f"(z[O + 74]), "=f"(z[O + 75]), "=f"(z[O + 76]), "=f"(z[O + 77]), "=f"(z[O + 78]), "=f"(z[O + 79]),
+        "=f"(z[O + 80]), "=f"(z[O + 81]), "=f"(z[O + 82]), "=f"(z[O + 83]), "=f"(z[O + 84]), "=f"(z[O + 85]), "=f"(z[O + 86]), "=f"(z[O + 87]),
+        "=f"(z[O + 88]), "=f"(z[O + 89]), "=f"(z[O + 90]), "=f"(z[O + 91]), "=f"(z[O + 92]), "=f"(z[O + 93]), "=f"(z[O + 94]), "=f"(z[O + 95]),
+        "=f"(z[O + 96]), "=f"(z[O + 97]), "=f"(z[O + 98]), "=f"(z[O + 99]), "=f"(z[O + 100]), "=f"(z[O + 101]), "=f"(z[O + 102]), "=f"(z[O + 103]),
+        "=f"(z[O + 104]), "=f"(z[O + 105]), "=f"(z[O + 106]), "=f"(z[O + 107]), "=f"(z[O + 108]), "=f"(z[O + 109]), "=f"(z[O + 110]), "=f"(z[O + 111]),
+        "=f"(z[O + 112]), "=f"(z[O + 113]), "=f"(z[O + 114]), "=f"(z[O + 115]), "=f"(z[O + 116]), "=f"(z[O + 117]), "=f"(z[O + 118]), "=f"(z[O + 119]),
+        "=f"(z[O + 120]), "=f"(z[O + 121]), "=f"(z[O + 122]), "=f"(z[O + 123]), "=f"(z[O + 124]), "=f"(z[O + 125]), "=f"(z[O + 126]), "=f"(z[O + 127])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -149,21 +200,20 @@ __device__ __forceinline__ WtTiles wt_union(const WtTiles& a, const WtTiles& b) 
   r.first = max(r.first, r.nsink);
   return r;
 }
-// Which columns of a tile a row sees: s = s0 + j with j <= hi and (j >= lo or j < sink).
-struct WtSeen { int lo, hi, sink; };
-__device__ __forceinline__ WtSeen wt_seen(const WinParams& p, int l, int queries, int s0, int keys) {
-  WtSeen w;
-  w.lo = l - p.window + 1 - s0;
-  w.sink = p.sinks - s0;
-  w.hi = (p.causal ? min(l, keys - 1) : keys - 1) - s0;
-  if (!p.causal && w.sink <= 0) w.hi = min(w.hi, l + p.window - 1 - s0);
-  if (l >= queries) w.hi = -1;
-  return w;
-}
-// non-causal tiles with sinks: the sink columns are seen beyond the window's end, the others are not
-__device__ __forceinline__ bool wt_sees(const WinParams& p, const WtSeen& w, int l, int s0, int j) {
-  return j <= w.hi && (j < w.sink || (j >= w.lo && (p.causal || s0 + j < l + p.window)));
-}
+__device__ __forceinline__ uint32_t wt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+// Which keys of a tile a row of queries sees, 32 columns at a time: s = s0 + j with j < end and (j < sink or from <= j < past).
+struct WtSeen {
+  int from, past, sink, end;
+  __device__ __forceinline__ WtSeen(const WinParams& p, int l, int queries, int s0, int keys) {
+    from = l - p.window + 1 - s0;
+    past = l + p.window - s0;
+    sink = p.sinks - s0;
+    end = l >= queries ? 0 : (p.causal ? min(l + 1, keys) : keys) - s0;
+  }
+  __device__ __forceinline__ uint32_t bits(int j) const {
+    return wt_below(end - j) & (wt_below(sink - j) | (wt_below(past - j) & ~wt_below(from - j)));
+  }
+};
 // every row of the tile sees every key of it
 __device__ __forceinline__ bool wt_all_seen(const WinParams& p, int l0, int queries, int s0, int keys) {
   if (l0 + kWtTile > queries || s0 + kWtTile > keys) return false;

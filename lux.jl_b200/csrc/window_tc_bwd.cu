@@ -203,41 +203,42 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool apart = bias == nullptr && wt_apart(c2, flat);
       const float off = (flat - stat.x) - stat.y;
       const uint64_t mul2_ = pack2(c2, c2), off2_ = pack2(off, off), flat2_ = pack2(flat, flat);
+      tmem_row64<0>(tS, d);
+      if (apart) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_ld32(tS + q * 32, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const uint64_t s2 = pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
-          uint64_t y;
-          if (apart) y = fma2(s2, mul2_, off2_);
-          else if (bias != nullptr) y = add2(add2(fma2(s2, mul2_, pack2(bias[q * 32 + j], bias[q * 32 + j + 1])), nm), nl);
-          else y = add2(add2(fma2(s2, mul2_, flat2_), nm), nl);
+        for (int j = 0; j < 64; j += 2) {
           float e0, e1;
-          unpack2(y, e0, e1);
-          d[q * 32 + j] = ex2(e0); d[q * 32 + j + 1] = ex2(e1);
+          unpack2(fma2(pack2(d[j], d[j + 1]), mul2_, off2_), e0, e1);
+          d[j] = ex2(e0); d[j + 1] = ex2(e1);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 64; j += 2) {
+          const uint64_t add = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_;
+          float e0, e1;
+          unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add), nm), nl), e0, e1);
+          d[j] = ex2(e0); d[j + 1] = ex2(e1);
         }
       }
       if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
       tc_fence_after();
       const bool whole = wt_all_seen(w, l0, queries, s0, keys);
-      const WtSeen seen = wt_seen(w, l, queries, s0, keys);
+      {
+        float e[64];
+        tmem_row64<0>(tDP + lanes + half * 64, e);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_ld32(tDP + lanes + half * 64 + q * 32, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          const uint64_t y = mul2(add2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), nd), pack2(d[q * 32 + j], d[q * 32 + j + 1]));
-          unpack2(y, d[q * 32 + j], d[q * 32 + j + 1]);
+        for (int j = 0; j < 64; j += 2) {
+          const uint64_t y = mul2(add2(pack2(e[j], e[j + 1]), nd), pack2(d[j], d[j + 1]));
+          unpack2(y, d[j], d[j + 1]);
         }
-        if (!whole) {
+      }
+      if (!whole) {
+        const WtSeen seen(w, l, queries, s0, keys);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (!wt_sees(w, seen, l, s0, half * 64 + q * 32 + j)) d[q * 32 + j] = 0.f;
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t bits = seen.bits(half * 64 + q * 32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
         }
       }
       {
@@ -508,33 +509,35 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       float d[64];
       const bool apart = bias == nullptr && wt_apart(c2, flat);
       const uint64_t mul2_ = pack2(c2, c2), flat2_ = pack2(flat, flat);
+      tmem_row64<0>(tS, d);
+      if (apart) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_ld32(tS + q * 32, v);
-        tmem_ld_wait();
+        for (int j = 0; j < 64; j += 4) {
+          const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
+          float y[4];
+          unpack2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add2(flat2_, pack2(m.x, m.y))), pack2(e.x, e.y)), y[0], y[1]);
+          unpack2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add2(flat2_, pack2(m.z, m.w))), pack2(e.z, e.w)), y[2], y[3]);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 m = lds4(col + half * 64 + q * 32 + j), e = lds4(col + 128 + half * 64 + q * 32 + j);
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const uint64_t s2 = pack2(__uint_as_float(v[j + k]), __uint_as_float(v[j + k + 1]));
-            const uint64_t nm = k == 0 ? pack2(m.x, m.y) : pack2(m.z, m.w), nl = k == 0 ? pack2(e.x, e.y) : pack2(e.z, e.w);
-            uint64_t y;
-            if (apart) y = add2(fma2(s2, mul2_, add2(flat2_, nm)), nl);
-            else if (bias != nullptr) y = add2(add2(fma2(s2, mul2_, pack2(bias[q * 32 + j + k], bias[q * 32 + j + k + 1])), nm), nl);
-            else y = add2(add2(fma2(s2, mul2_, flat2_), nm), nl);
-            float e0, e1;
-            unpack2(y, e0, e1);
-            d[q * 32 + j + k] = ex2(e0); d[q * 32 + j + k + 1] = ex2(e1);
-          }
+          for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
         }
-        if (!whole) {
+      } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int c = half * 64 + q * 32 + j;
-            if (c < from || c > to) d[q * 32 + j] = 0.f;
-          }
+        for (int j = 0; j < 64; j += 4) {
+          const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
+          const uint64_t add0 = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_, add1 = bias != nullptr ? pack2(bias[j + 2], bias[j + 3]) : flat2_;
+          float y[4];
+          unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add0), pack2(m.x, m.y)), pack2(e.x, e.y)), y[0], y[1]);
+          unpack2(add2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add1), pack2(m.z, m.w)), pack2(e.z, e.w)), y[2], y[3]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
         }
       }
       {
@@ -550,31 +553,26 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
       tc_fence_after();
       uint32_t o[32];
+      {
+        float e[64];
+        tmem_row64<0>(tD, e);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t v[32];
-        tmem_ld32(tD + q * 32, v);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 e = lds4(col + 256 + half * 64 + q * 32 + j);
-#pragma unroll
-          for (int k = 0; k < 4; k += 2) {
-            const uint64_t y = mul2(add2(pack2(__uint_as_float(v[j + k]), __uint_as_float(v[j + k + 1])), k == 0 ? pack2(e.x, e.y) : pack2(e.z, e.w)),
-                                    pack2(d[q * 32 + j + k], d[q * 32 + j + k + 1]));
-            unpack2(y, d[q * 32 + j + k], d[q * 32 + j + k + 1]);
-          }
+        for (int j = 0; j < 64; j += 4) {
+          const float4 nd = lds4(col + 256 + half * 64 + j);
+          unpack2(mul2(add2(pack2(e[j], e[j + 1]), pack2(nd.x, nd.y)), pack2(d[j], d[j + 1])), d[j], d[j + 1]);
+          unpack2(mul2(add2(pack2(e[j + 2], e[j + 3]), pack2(nd.z, nd.w)), pack2(d[j + 2], d[j + 3])), d[j + 2], d[j + 3]);
         }
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int c = half * 64 + q * 32 + j;
-            if (c < from || c > to) d[q * 32 + j] = 0.f;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[q * 16 + j] = pack_bf16(d[q * 32 + 2 * j], d[q * 32 + 2 * j + 1]);
       }
+      if (!whole) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
       tmem_st32(tD, o);
       tmem_st_wait();
       tc_fence_before();
