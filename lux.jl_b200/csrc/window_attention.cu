@@ -238,19 +238,30 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
     if (bad[r]) win_row_fwd<T>(p, x, lb != nullptr ? lb + l0 + r : nullptr, l0 + r, h, b, keys);
 }
 
-// delta[batch][head][query] = dx . x, a warp per row
-template <typename T>
+// delta[batch][head][query] = dx . x; LR lanes share a row and take a 16-byte vector each, or (LR = 0) a warp walks it
+template <typename T, int LR>
 __global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delta, const T* __restrict__ dx, const T* __restrict__ x, int E, int H,
                                                         int L, int64_t rows) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);      // (batch, query, head)
-  if (row >= rows) return;
-  const T *a = dx + row * E, *c = x + row * E;
+  constexpr int LANES = LR == 0 ? 32 : LR, V = Vec16<T>::N;
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;      // (batch, query, head)
   float s = 0.f;
-  for (int e = lane; e < E; e += 32) s = fmaf(to_f32(a[e]), to_f32(c[e]), s);
-  s = warp_sum(s);
-  const int64_t h = row % H, bl = row / H, b = bl / L, l = bl % L;
-  if (lane == 0) delta[(b * H + h) * L + l] = s;
+  if (row < rows) {
+    const T *a = dx + row * E, *c = x + row * E;
+    if constexpr (LR == 0) {
+      for (int e = lane; e < E; e += 32) s = fmaf(to_f32(a[e]), to_f32(c[e]), s);
+    } else if (lane * V < E) {
+      const Vec16<T> u = load16(a + lane * V), v = load16(c + lane * V);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s = fmaf(u.get(i), v.get(i), s);
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0 && row < rows) {
+    const int64_t h = row % H, bl = row / H, b = bl / L, l = bl - b * L;
+    delta[(b * H + h) * L + l] = s;
+  }
 }
 
 // dq, and partial[tile][batch][head][bucket] of dtable
@@ -480,6 +491,9 @@ WinParams win_params(const lb2_window_dims* d, const void* q, const void* k, con
 int win_columns(const lb2_rel_buckets* t) { return t == nullptr ? 0 : t->count * (t->bidirectional ? 2 : 1); }
 int win_simt_tile(const lb2_window_dims* d) { return d->head_dim <= 128 && d->value_dim <= 128 ? 64 : 32; }
 int64_t win_tiles(int64_t n, int tile) { return (n + tile - 1) / tile; }
+size_t win_partial_bytes(const lb2_window_dims* d, const lb2_rel_buckets* t) {
+  return align_up((size_t)(win_tiles(d->queries, win_simt_tile(d)) * d->batch * d->heads * win_columns(t)) * sizeof(float), 256);
+}
 // four features at a time: rows and bases of whole vectors
 bool win_vec(int64_t n, const void* a, const void* b, size_t es) { return n % 4 == 0 && aligned_to(a, 4 * es) && aligned_to(b, 4 * es); }
 
@@ -494,6 +508,20 @@ bool win_vec(int64_t n, const void* a, const void* b, size_t es) { return n % 4 
 template <typename K> int32_t win_smem(K kernel, int bytes) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(e));
+  return LB2_OK;
+}
+
+template <typename T> int32_t win_delta(float* delta, const T* dx, const T* x, const WinParams& p, int64_t rows, cudaStream_t st) {
+  const int lanes = p.E / Vec16<T>::N;
+  const bool vec = p.E > 0 && p.E % Vec16<T>::N == 0 && lanes <= 32 && aligned_to(dx, 16) && aligned_to(x, 16);
+  auto launch = [&](auto kernel, int per_row) {
+    kernel<<<(unsigned)((rows * per_row + 255) / 256), 256, 0, st>>>(delta, dx, x, p.E, p.H, p.L, rows);
+  };
+  if (!vec) launch(win_delta_kernel<T, 0>, 32);
+  else if (lanes <= 8) launch(win_delta_kernel<T, 8>, 8);
+  else if (lanes <= 16) launch(win_delta_kernel<T, 16>, 16);
+  else launch(win_delta_kernel<T, 32>, 32);
+  LB2_CHECK_LAUNCH("windowed attention delta");
   return LB2_OK;
 }
 
@@ -535,9 +563,9 @@ int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const voi
 
 size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* d, const lb2_rel_buckets* buckets, int32_t dtype) {
   if (d == nullptr || !valid_dtype(dtype) || d->queries <= 0 || d->heads <= 0 || d->batch <= 0) return 0;
+  if (d->kv_heads <= 0 || d->heads % d->kv_heads != 0) return 0;
   const size_t rows = (size_t)(d->queries * d->heads * d->batch);
-  return align_up(rows * sizeof(float), 256) +
-         align_up((size_t)(win_tiles(d->queries, win_simt_tile(d)) * d->batch * d->heads * win_columns(buckets)) * sizeof(float), 256);
+  return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + (win_tc_serves(d, dtype) ? align_up(win_tc_sink_bytes(d), 256) : 0);
 }
 
 int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const float* stats, const void* q,
@@ -567,15 +595,15 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   const int64_t rows = d->queries * d->heads * d->batch;
   float* delta = static_cast<float*>(workspace);
   float* partial = delta + align_up((size_t)rows * sizeof(float), 256) / sizeof(float);
+  float* sink_sums = partial + win_partial_bytes(d, buckets) / sizeof(float);
   const int vecq = win_vec(d->head_dim, q, k, es), vecv = win_vec(d->value_dim, v, dx, es);
   const int64_t qt = win_tiles(d->queries, tile), kt = win_tiles(d->keys, tile);
   LB2_REQUIRE(qt * d->heads * d->batch <= 0x7FFFFFFF && kt * d->kv_heads * d->batch <= 0x7FFFFFFF && (rows + 7) / 8 <= 0x7FFFFFFF, LB2_BAD_SHAPE,
               "too many rows");
   if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(q, 16) &&
       aligned_to(k, 16) && aligned_to(v, 16)) {
-    win_delta_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(delta, (const __nv_bfloat16*)dx, (const __nv_bfloat16*)x, p.E, p.H, p.L, rows);
-    LB2_CHECK_LAUNCH("windowed attention delta");
-    if ((rc = win_tc_bwd(p, dq, dk, dv, partial, dx, reinterpret_cast<const float2*>(stats), delta, st)) != LB2_OK || columns == 0) return rc;
+    if ((rc = win_delta(delta, (const __nv_bfloat16*)dx, (const __nv_bfloat16*)x, p, rows, st)) != LB2_OK) return rc;
+    if ((rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, dx, reinterpret_cast<const float2*>(stats), delta, st)) != LB2_OK || columns == 0) return rc;
     win_dtable_kernel<<<(unsigned)((p.H * columns + 7) / 8), 256, 0, st>>>((__nv_bfloat16*)dtable, partial, p.H, columns, win_tc_partials(d) * d->batch);
     LB2_CHECK_LAUNCH("windowed attention dtable");
     return LB2_OK;
@@ -583,8 +611,7 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   LB2_DISPATCH_DTYPE(dtype, LB2_WIN_DISPATCH(d, {
     using C = WinTile<DP>;
     if (nq) {
-      win_delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(delta, (const T*)dx, (const T*)x, p.E, p.H, p.L, rows);
-      LB2_CHECK_LAUNCH("windowed attention delta");
+      if ((rc = win_delta(delta, (const T*)dx, (const T*)x, p, rows, st)) != LB2_OK) return rc;
       if ((rc = win_smem(win_dq_kernel<T, DP>, C::DQ_BYTES)) != LB2_OK) return rc;
       win_dq_kernel<T, DP><<<(unsigned)(qt * d->heads * d->batch), kWinThreads, C::DQ_BYTES, st>>>((T*)dq, partial, (const T*)dx, (const float2*)stats, delta, p, (int)qt,
                                                                                                    vecq, vecv);

@@ -10,7 +10,8 @@ constexpr int kWtBox = kWtTile * 128;        // bytes of a TMA box: 128 tokens x
 // what the tensor-core kernels serve: rows of whole 16-byte vectors for TMA, at most two boxes of features
 bool win_tc_serves(const lb2_window_dims* d, int32_t dtype);
 int64_t win_tc_partials(const lb2_window_dims* d);      // blocks that leave a partial sum of dtable per head and sample
-int32_t win_tc_bwd(const WinParams& p, void* dq, void* dk, void* dv, float* partial, const void* dx, const float2* stats, const float* delta,
+size_t win_tc_sink_bytes(const lb2_window_dims* d);    // scratch for the keys that all later queries see
+int32_t win_tc_bwd(const WinParams& p, void* dq, void* dk, void* dv, float* partial, float* sink_sums, const void* dx, const float2* stats, const float* delta,
                    cudaStream_t st);
 int32_t win_tc_fwd(const WinParams& p, void* x, float2* stats, cudaStream_t st);
 
