@@ -118,6 +118,7 @@ template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& 
     for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(w, t[i], o[i] * keep);
     sum = sum * keep + w;
     m = mn;
+    if (isnan(sum)) break;                // so is the whole row
   }
 #pragma unroll
   for (int i = 0; i < kWinLaneDims; ++i) o[i] /= sum;

@@ -45,6 +45,15 @@ template <int NB> __device__ __forceinline__ void wt_mma_features(uint32_t d, ui
     umma<false>(d, ad + at, bd + at, wt_idesc(kWtTile, false), ks != 0 ? 1u : 0u);
   }
 }
+// D[128][64] = A . B', B the 64 tokens at `b`
+template <int NB> __device__ __forceinline__ void wt_mma_features64(uint32_t d, uint32_t a, uint32_t b) {
+  const uint64_t ad = wt_desc_k(a), bd = wt_desc_k(b);
+#pragma unroll
+  for (int ks = 0; ks < 4 * NB; ++ks) {
+    const uint32_t at = (ks >> 2) * (kWtBox >> 4) + (ks & 3) * 2;
+    umma<false>(d, ad + at, bd + at, wt_idesc(64, false), ks != 0 ? 1u : 0u);
+  }
+}
 // A operand in TMEM: 128 lanes x 128 values, two bf16 per column
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -53,13 +62,13 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D[128][64 NB] (+)= P . V: P from TMEM, V a tile of 128 tokens
-template <int NB> __device__ __forceinline__ void wt_mma_tokens(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
+// D[128][64 NB] (+)= P . V: P from TMEM, V 64 tokens of a tile
+template <int NB> __device__ __forceinline__ void wt_mma_tokens64(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
   const uint64_t vd = wt_desc_mn(v);
 #pragma unroll
-  for (int ks = 0; ks < 8; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
+  for (int ks = 0; ks < 4; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
-// as wt_mma_tokens with P in two halves 64 columns apart, each over the columns that its own threads have read
+// over 128 tokens, with P in two halves 64 columns apart, each over the columns that its own threads have read
 template <int NB> __device__ __forceinline__ void wt_mma_tokens_halves(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
   const uint64_t vd = wt_desc_mn(v);
 #pragma unroll
@@ -201,6 +210,40 @@ __device__ __forceinline__ WtTiles wt_union(const WtTiles& a, const WtTiles& b) 
   r.first = max(r.first, r.nsink);
   return r;
 }
+__device__ __forceinline__ int warp_uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }   // the same in all lanes, and known to be
+// Where a tile of 128 queries from l0 on stands to `N` keys from s0 on: some row sees some of them; every row sees all of them.
+template <int N> struct WtView {
+  int sinks, lo, hi, whole_sinks, whole_lo, whole_hi, whole_end;
+  __device__ __forceinline__ WtView(const WinParams& p, int l0, int queries, int keys) {
+    sinks = lo = hi = whole_sinks = whole_lo = 0;
+    whole_hi = whole_end = -1;
+    if (l0 >= queries) return;
+    win_key_range(p, l0, min(l0 + kWtTile, queries), keys, &sinks, &lo, &hi);
+    if (lo >= hi) lo = hi = 0;
+    if (l0 + kWtTile > queries) return;
+    whole_sinks = p.sinks - N;
+    whole_lo = l0 + kWtTile - p.window;
+    whole_end = min(keys, p.causal ? l0 + 1 : keys) - N;
+    whole_hi = min(whole_end, l0 + p.window - N);
+  }
+  __device__ __forceinline__ bool some(int s0) const { return s0 < sinks || (s0 < hi && s0 + N > lo); }
+  __device__ __forceinline__ bool whole(int s0) const { return s0 <= whole_end && (s0 <= whole_sinks || (s0 >= whole_lo && s0 <= whole_hi)); }
+};
+// The bias of N keys from s0 on for a tile of queries from l0 on: one value where all pairs lie in a side's last bucket.
+struct WtFlat {
+  float left, right;
+  int last;                               // where the last bucket starts; no bias: out of reach
+  template <typename T> __device__ __forceinline__ WtFlat(const WinParams& p, const T* table, int h) {
+    left = right = 0.f; last = 0;
+    if (p.buckets.count == 0) return;
+    last = p.buckets.first[p.buckets.count - 1];
+    left = win_bias2(to_f32(table[h + (int64_t)p.H * (p.buckets.count - 1)]));
+    right = p.buckets.bidirectional ? win_bias2(to_f32(table[h + (int64_t)p.H * (2 * p.buckets.count - 1)])) : win_bias2(to_f32(table[h]));
+  }
+  // low, high: of key - query over the pairs
+  __device__ __forceinline__ bool is_left(int high) const { return high <= 0 && -high >= last; }
+  __device__ __forceinline__ bool is_right(const WinParams& p, int low) const { return low > 0 && (!p.buckets.bidirectional || low >= last); }
+};
 __device__ __forceinline__ uint32_t wt_below(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
 // Which keys of a tile a row of queries sees, 32 columns at a time: s = s0 + j with j < end and (j < sink or from <= j < past).
 struct WtSeen {
@@ -215,12 +258,23 @@ struct WtSeen {
     return wt_below(end - j) & (wt_below(sink - j) | (wt_below(past - j) & ~wt_below(from - j)));
   }
 };
-// every row of the tile sees every key of it
-__device__ __forceinline__ bool wt_all_seen(const WinParams& p, int l0, int queries, int s0, int keys) {
-  if (l0 + kWtTile > queries || s0 + kWtTile > keys) return false;
-  if (p.causal && s0 + kWtTile - 1 > l0) return false;
-  const bool sinks = s0 + kWtTile <= p.sinks;
-  return sinks || (l0 + kWtTile - 1 - s0 < p.window && s0 + kWtTile - 1 - l0 < p.window);
+// every one of 128 queries from l0 on sees every one of `n` keys from s0 on
+__device__ __forceinline__ bool wt_all_seen(const WinParams& p, int l0, int queries, int s0, int keys, int n = kWtTile) {
+  if (l0 + kWtTile > queries || s0 + n > keys) return false;
+  if (p.causal && s0 + n - 1 > l0) return false;
+  const bool sinks = s0 + n <= p.sinks;
+  return sinks || (l0 + kWtTile - 1 - s0 < p.window && s0 + n - 1 - l0 < p.window);
+}
+// 16 columns of a row as bf16, 32 bytes in one store where rows allow it
+__device__ __forceinline__ void wt_store16(__nv_bfloat16* to, const uint32_t (&v)[8], int columns, bool wide) {
+  if (wide && columns >= 16) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    if (columns >= 8) *reinterpret_cast<uint4*>(to) = make_uint4(v[0], v[1], v[2], v[3]);
+    if (columns >= 16) *reinterpret_cast<uint4*>(to + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+  }
 }
 
 }  // namespace lb2
