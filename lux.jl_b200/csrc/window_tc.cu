@@ -1,16 +1,15 @@
 // Windowed attention on the tensor cores, forward: BFloat16, up to 128 features.
 //
 // A block owns two tiles of 128 queries that read the same keys: the tiles of two heads that share a key head, or two
-// neighbouring tiles of one head; each has its softmax group of four warps, a thread per row. Per 64 keys: S = Q K' into TMEM, the
-// group turns S into weights 2^(z2 - m2), which go back to TMEM as bf16 over S, O += P V with P taken from TMEM. A group has two S
-// buffers: the next 64 keys' logits are there when it has finished a step, so that neither the group nor the tensor cores wait
-// for one another's latency. O is rescaled only when a row's maximum has grown by more than 2^8 (the reference m2 may lag behind
+// neighbouring tiles of one head; each has its softmax group of four warps, a thread per row, and a warp that issues its products.
+// Per tile of 128 keys: S = Q K' into TMEM, the group turns S into weights 2^(z2 - m2), which go back to TMEM as bf16 over S,
+// O += P V with P taken from TMEM. While one group is in its softmax the tensor cores work for the other. O is rescaled only when a row's maximum has grown by more than 2^8 (the reference m2 may lag behind
 // the maximum by that: weights up to 256 are as exact in bf16 as weights up to 1).
 //
 // Blocks stay on their SM and take pairs of tiles in turn: the next pair's Q and keys are loaded, and its first logits formed, while
 // the groups finish and store this one's.
 //
-// TMEM columns: S of group 0 (2 x 64) | S of group 1 | O0 (128) | O1. Shared memory: both tiles of Q, a ring of key and value tiles in turn.
+// TMEM columns: S0 | S1 | O0 | O1, 128 each. Shared memory: both tiles of Q, a ring of key and value tiles in turn.
 #include "common.cuh"
 #include "window_tc.cuh"
 
@@ -18,8 +17,8 @@ namespace lb2 {
 
 namespace {
 
-// warp 0: TMA, warps 1 and 2: MMA, warps 4-7 and 8-11: one softmax group each; registers 104 + 2 x 200 = 3 x 168 per thread at launch
-constexpr int kWtFwdThreads = 384, kWtFwdFew = 104, kWtFwdMany = 200;
+// warp 0: TMA, warps 1 and 2: MMA, warps 4-7 and 8-11: one softmax group each; registers 56 + 2 x 224 = 3 x 168 per thread at launch
+constexpr int kWtFwdThreads = 384, kWtFwdFew = 56, kWtFwdMany = 224;
 
 template <int NB> struct WtFwd {
   static constexpr int TILE = NB * kWtBox;
@@ -55,9 +54,6 @@ struct WtPair {
     queries = warp_uniform(win_tokens(w, b, w.L)); keys = warp_uniform(win_tokens(w, b, w.S));
     all = wt_union(wt_key_tiles(w, l0[0], queries, keys), wt_key_tiles(w, l0[1], queries, keys));
   }
-  __device__ __forceinline__ int steps() const { return 2 * all.count(); }
-  // the first key of step j + 1, s0 that of step j
-  __device__ __forceinline__ int next_key(int j, int s0) const { return j + 1 == 2 * all.nsink ? all.first * kWtTile : s0 + 64; }
 };
 
 template <int NB>
@@ -70,11 +66,9 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);      // [group][parity][256]
   uint64_t* bars = reinterpret_cast<uint64_t*>(lut + 2 * 2 * 256);
-  // [group][buffer]: S is there, P is there, its product is in O (a warp may be a step ahead of the others of its group, and the
-  // products two behind: a barrier of their buffer is at the phase asked for or one before, which its parity tells apart).
-  // o_empty: O has been read
-  uint64_t *q_full = bars, *q_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *p_ready = s_full + 4,
-           *pv_done = p_ready + 4, *o_empty = pv_done + 4;
+  // [group]: S is there, P is there, its product is in O, O has been read
+  uint64_t *q_full = bars, *q_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *p_ready = s_full + 2,
+           *pv_done = p_ready + 2, *o_empty = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 2);
   const uint32_t sQ = base, sKV = base + 2 * C::TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -84,8 +78,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
     mbar_init(q_full, 1); mbar_init(q_empty, 2);
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
-    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1); }
-    for (int i = 0; i < 2; ++i) mbar_init(&o_empty[i], 4);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1); mbar_init(&o_empty[i], 4); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -130,46 +123,43 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // a warp per group: while one waits for its weights the other's products run
       const int grp = warp - 1;
       uint32_t turn = 0, kst = 0, kph = 0, vst = 0, vph = 0;               // pairs; the ring's next key and value tile
-      uint32_t made = 0, used = 0, outs = 0;                               // S formed, P consumed, O begun
+      uint32_t used = 0, outs = 0;                                         // P consumed, O begun
       const uint32_t tS = tmem + grp * 128, tO = tmem + 256 + grp * 128, q = sQ + grp * C::TILE;
       bool ok = true;
       for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
         const WtPair t(p, item);
-        const int n = t.steps();
+        const int n = t.all.count();
         if (n == 0) continue;
-        const WtView<64> view(w, grp == 0 ? t.l0[0] : t.l0[1], t.queries, t.keys);
+        const WtView<128> view(w, grp == 0 ? t.l0[0] : t.l0[1], t.queries, t.keys);
         if (!mbar_wait_uniform(q_full, turn & 1u, p.status, 0x200u)) break;
         ++turn;
         bool begun = false;
-        int s0 = 0, s2 = t.all.at(0) * kWtTile;  // of step j and of step j + 2
-        // two steps ahead: logits of step j + 2 after the product of step j, whose buffer they take
-        for (int j = -2; j < n; ++j) {
-          const int ahead = j + 2;
-          if (j == 0) s0 = t.all.at(0) * kWtTile;
-          const bool use = j >= 0 && view.some(s0), make = ahead < n && view.some(s2), k_last = ahead < n && (ahead & 1) == 1, v_last = j >= 0 && (j & 1) == 1;
-          if (ahead < n && (ahead & 1) == 0 && !mbar_wait_uniform(&full[2 * kst], kph, p.status, 0x400u)) ok = false;
-          if (j >= 0 && (j & 1) == 0 && !mbar_wait_uniform(&full[2 * vst + 1], vph, p.status, 0x400u)) ok = false;
+        // the next tile's logits after this one's product, whose weights they overwrite
+        for (int j = -1; j < n; ++j) {
+          const bool next = j + 1 < n, use = j >= 0 && view.some(t.all.at(j) * kWtTile), make = next && view.some(t.all.at(j + 1) * kWtTile);
+          if (next && !mbar_wait_uniform(&full[2 * kst], kph, p.status, 0x400u)) ok = false;
+          if (j >= 0 && !mbar_wait_uniform(&full[2 * vst + 1], vph, p.status, 0x400u)) ok = false;
           if (use) {
             if (!begun && !mbar_wait_uniform(&o_empty[grp], (outs & 1u) ^ 1u, p.status, 0x4000u)) ok = false;
-            if (!mbar_wait_uniform(&p_ready[grp * 2 + (used & 1u)], (used >> 1) & 1u, p.status, 0x800u)) ok = false;
+            if (!mbar_wait_uniform(&p_ready[grp], used & 1u, p.status, 0x800u)) ok = false;
           }
           if (!ok) break;
           tc_fence_after();
-          const uint32_t k = sKV + 2 * kst * C::TILE + (ahead & 1) * 64 * 128, v = sKV + (2 * vst + 1) * C::TILE + (j & 1) * 64 * 128;
+          const uint32_t k = sKV + 2 * kst * C::TILE, v = sKV + (2 * vst + 1) * C::TILE;
           if (elect_one()) {
             if (use) {
-              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens64<NB>(tO, tS + (used & 1u) * 64, v, begun);
-              else wt_mma_tokens64<1>(tO, tS + (used & 1u) * 64, v, begun);
-              umma_commit(&pv_done[grp * 2 + (used & 1u)]);
+              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens<NB>(tO, tS, v, begun);
+              else wt_mma_tokens<1>(tO, tS, v, begun);
+              umma_commit(&pv_done[grp]);
             }
             if (make) {
-              if (NB == 2 && p.boxes_d == 2) wt_mma_features64<NB>(tS + (made & 1u) * 64, q, k);
-              else wt_mma_features64<1>(tS + (made & 1u) * 64, q, k);
-              umma_commit(&s_full[grp * 2 + (made & 1u)]);
+              if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tS, q, k);
+              else wt_mma_features<1>(tS, q, k);
+              umma_commit(&s_full[grp]);
             }
-            if (v_last) umma_commit(&empty[2 * vst + 1]);
-            if (k_last) umma_commit(&empty[2 * kst]);
-            if (ahead == n - 1) umma_commit(q_empty);
+            if (j >= 0) umma_commit(&empty[2 * vst + 1]);
+            if (next) umma_commit(&empty[2 * kst]);
+            if (j + 1 == n - 1) umma_commit(q_empty);
           }
           __syncwarp();
           if (use) {
@@ -177,11 +167,8 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             ++used;
             begun = true;
           }
-          if (make) ++made;
-          if (v_last && ++vst == C::STAGES / 2) { vst = 0; vph ^= 1u; }
-          if (k_last && ++kst == C::STAGES / 2) { kst = 0; kph ^= 1u; }
-          if (j >= 0) s0 = t.next_key(j, s0);
-          s2 = t.next_key(ahead, s2);
+          if (j >= 0 && ++vst == C::STAGES / 2) { vst = 0; vph ^= 1u; }
+          if (next && ++kst == C::STAGES / 2) { kst = 0; kph ^= 1u; }
         }
       }
     }
@@ -194,53 +181,52 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     bool ok = true, redo = false;
     uint32_t made = 0;                           // steps so far
     int turn = 0;                                // of the bias tables: each use has a barrier of the group, two are enough
-    auto last_product = [&](uint32_t k) { return mbar_wait_warp(&pv_done[grp * 2 + (k & 1u)], (k >> 1) & 1u, p.status, 0x2000u); };
     for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
       const WtPair t(p, item);
-      const int h = t.head[grp], l0 = t.l0[grp], l = l0 + row, n = t.steps();
-      const WtView<64> view(w, l0, t.queries, t.keys);
+      const int h = t.head[grp], l0 = t.l0[grp], l = l0 + row, n = t.all.count();
+      const WtView<128> view(w, l0, t.queries, t.keys);
       const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
       float m2 = -INFINITY, sum = 0.f;
       bool begun = false;
-      for (int j = 0, s0 = t.all.at(0) * kWtTile; j < n; s0 = t.next_key(j, s0), ++j) {
+      for (int j = 0; j < n; ++j) {
+        const int s0 = t.all.at(j) * kWtTile;
         if (!view.some(s0)) continue;
         float flat = 0.f;
         const float* bias = nullptr;
         if (biased) {
           const int low = s0 - l0 - (kWtTile - 1);
-          if (tail.is_left(low + kWtTile + 62)) {
+          if (tail.is_left(low + 2 * (kWtTile - 1))) {
             flat = tail.left;
           } else if (tail.is_right(w, low)) {
             flat = tail.right;
           } else {                               // index j - row + 127: rel = low + index
             float* at = lut + (grp * 2 + turn) * 256;
             turn ^= 1;
-            for (int x = gt; x < kWtTile + 63; x += 128) at[x] = win_bias<__nv_bfloat16>(w, h, low + x);
+            for (int x = gt; x < 2 * kWtTile - 1; x += 128) at[x] = win_bias<__nv_bfloat16>(w, h, low + x);
             bar_group(1 + grp, 128);
             bias = at + (kWtTile - 1 - row);
           }
         }
-        const uint32_t buf = made & 1u;
-        if (!mbar_wait_warp(&s_full[grp * 2 + buf], (made >> 1) & 1u, p.status, 0x1000u)) { ok = false; break; }
+        if (!mbar_wait_warp(&s_full[grp], made & 1u, p.status, 0x1000u)) { ok = false; break; }
         tc_fence_after();
         // logits = mul * z + add, mul > 0; what a row does not see is -inf
         const bool apart = bias == nullptr && wt_apart(c2, flat);
         const float mul = apart ? c2 : 1.f, add = apart ? flat : 0.f;
-        float z[64];
-        tmem_row64<0>(tS + buf * 64, z);
+        float z[128];
+        tmem_row128<0>(tS, z);
         if (!apart) {
           if (bias != nullptr) {
 #pragma unroll
-            for (int x = 0; x < 64; ++x) z[x] = fmaf(z[x], c2, bias[x]);
+            for (int x = 0; x < 128; ++x) z[x] = fmaf(z[x], c2, bias[x]);
           } else {
 #pragma unroll
-            for (int x = 0; x < 64; ++x) z[x] = fmaf(z[x], c2, flat);
+            for (int x = 0; x < 128; ++x) z[x] = fmaf(z[x], c2, flat);
           }
         }
         if (!view.whole(s0)) {
           const WtSeen seen(w, l, t.queries, s0, t.keys);
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
+          for (int q = 0; q < 4; ++q) {
             const uint32_t bits = seen.bits(q * 32);
 #pragma unroll
             for (int x = 0; x < 32; ++x) z[q * 32 + x] = bits >> x & 1u ? z[q * 32 + x] : -INFINITY;
@@ -248,15 +234,13 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         float top[4] = {z[0], z[1], z[2], z[3]};
 #pragma unroll
-        for (int x = 4; x < 64; ++x) top[x & 3] = fmaxf(top[x & 3], z[x]);
+        for (int x = 4; x < 128; ++x) top[x & 3] = fmaxf(top[x & 3], z[x]);
         const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
         const bool grow = mx > m2 + 8.f;
         if (__any_sync(0xffffffffu, grow)) {
           const float keep = grow ? ex2(m2 - mx) : 1.f;
           if (grow) { m2 = mx; sum *= keep; }
-          if (begun) {                           // O is still while this step's P is not ready
-            if (!last_product(made - 1)) { ok = false; break; }
-            tc_fence_after();
+          if (begun) {                           // the logits came after the last product: O is still
 #pragma unroll 1
             for (int q = 0; q < 4 * NB; ++q) {
               uint32_t v[16];
@@ -271,16 +255,19 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float ref = m2 == -INFINITY ? 0.f : m2;
         const uint64_t mul_2 = pack2(mul, mul), off_2 = pack2(add - ref, add - ref);
         uint64_t part[2] = {0, 0};
-        uint32_t v[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          float a, c;
-          unpack2(fma2(pack2(z[2 * x], z[2 * x + 1]), mul_2, off_2), a, c);
-          a = ex2(a); c = ex2(c);
-          part[x & 1] = add2(part[x & 1], pack2(a, c));
-          v[x] = pack_bf16(a, c);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t v[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            float a, c;
+            unpack2(fma2(pack2(z[q * 64 + 2 * x], z[q * 64 + 2 * x + 1]), mul_2, off_2), a, c);
+            a = ex2(a); c = ex2(c);
+            part[x & 1] = add2(part[x & 1], pack2(a, c));
+            v[x] = pack_bf16(a, c);
+          }
+          tmem_st32(tS + q * 32, v);
         }
-        tmem_st32(tS + buf * 64, v);
         {
           float a, c;
           unpack2(add2(part[0], part[1]), a, c);
@@ -289,7 +276,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[grp * 2 + buf]);
+        if (lane == 0) mbar_arrive(&p_ready[grp]);
         ++made;
         begun = true;
       }
@@ -300,7 +287,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __nv_bfloat16* xr = static_cast<__nv_bfloat16*>(p.x) + (((int64_t)t.b * w.L + l) * w.H + h) * w.E;
       float o[64 * NB];
       if (begun) {
-        if (!last_product(made - 1)) { ok = false; continue; }
+        if (!mbar_wait_warp(&pv_done[grp], (made - 1) & 1u, p.status, 0x2000u)) { ok = false; continue; }
         tc_fence_after();
         tmem_row64<0>(tO, o);
         if constexpr (NB == 2) tmem_row64<64>(tO + 64, o);

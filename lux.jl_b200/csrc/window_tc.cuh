@@ -45,15 +45,6 @@ template <int NB> __device__ __forceinline__ void wt_mma_features(uint32_t d, ui
     umma<false>(d, ad + at, bd + at, wt_idesc(kWtTile, false), ks != 0 ? 1u : 0u);
   }
 }
-// D[128][64] = A . B', B the 64 tokens at `b`
-template <int NB> __device__ __forceinline__ void wt_mma_features64(uint32_t d, uint32_t a, uint32_t b) {
-  const uint64_t ad = wt_desc_k(a), bd = wt_desc_k(b);
-#pragma unroll
-  for (int ks = 0; ks < 4 * NB; ++ks) {
-    const uint32_t at = (ks >> 2) * (kWtBox >> 4) + (ks & 3) * 2;
-    umma<false>(d, ad + at, bd + at, wt_idesc(64, false), ks != 0 ? 1u : 0u);
-  }
-}
 // A operand in TMEM: 128 lanes x 128 values, two bf16 per column
 __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -62,13 +53,13 @@ __device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D[128][64 NB] (+)= P . V: P from TMEM, V 64 tokens of a tile
-template <int NB> __device__ __forceinline__ void wt_mma_tokens64(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
+// D[128][64 NB] (+)= P . V: P from TMEM, V a tile of 128 tokens
+template <int NB> __device__ __forceinline__ void wt_mma_tokens(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
   const uint64_t vd = wt_desc_mn(v);
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
+  for (int ks = 0; ks < 8; ++ks) umma_ts(d, p + ks * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
-// over 128 tokens, with P in two halves 64 columns apart, each over the columns that its own threads have read
+// with P in two halves 64 columns apart, each over the columns that its own threads have read
 template <int NB> __device__ __forceinline__ void wt_mma_tokens_halves(uint32_t d, uint32_t p, uint32_t v, bool accumulate) {
   const uint64_t vd = wt_desc_mn(v);
 #pragma unroll
