@@ -178,10 +178,10 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + grp * 128, tO = tmem + lanes + 256 + grp * 128;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
-    bool ok = true, redo = false;
+    bool ok = true, redo = false;                // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
     uint32_t made = 0;                           // steps so far
     int turn = 0;                                // of the bias tables: each use has a barrier of the group, two are enough
-    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
       const WtPair t(p, item);
       const int h = t.head[grp], l0 = t.l0[grp], l = l0 + row, n = t.all.count();
       const WtView<128> view(w, l0, t.queries, t.keys);
@@ -207,7 +207,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             bias = at + (kWtTile - 1 - row);
           }
         }
-        if (!mbar_wait_warp(&s_full[grp], made & 1u, p.status, 0x1000u)) { ok = false; break; }
+        ok = ok && mbar_wait_warp(&s_full[grp], made & 1u, p.status, 0x1000u);
         tc_fence_after();
         // logits = mul * z + add, mul > 0; what a row does not see is -inf
         const bool apart = bias == nullptr && wt_apart(c2, flat);
@@ -280,14 +280,14 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ++made;
         begun = true;
       }
-      if (!ok || l0 >= w.L) continue;
+      if (l0 >= w.L) continue;
       const bool any = l < t.queries && win_any(w, l, t.keys), in = l < w.L;
       const float inv = 1.f / sum;
       bool fine = isfinite(inv);
       __nv_bfloat16* xr = static_cast<__nv_bfloat16*>(p.x) + (((int64_t)t.b * w.L + l) * w.H + h) * w.E;
       float o[64 * NB];
       if (begun) {
-        if (!mbar_wait_warp(&pv_done[grp], (made - 1) & 1u, p.status, 0x2000u)) { ok = false; continue; }
+        ok = ok && mbar_wait_warp(&pv_done[grp], (made - 1) & 1u, p.status, 0x2000u);
         tc_fence_after();
         tmem_row64<0>(tO, o);
         if constexpr (NB == 2) tmem_row64<64>(tO + 64, o);

@@ -67,6 +67,19 @@ template <int NB> __device__ __forceinline__ void wt_mma_tokens_halves(uint32_t 
     umma_ts(d, p + (ks >> 2) * 64 + (ks & 3) * 8, vd + ks * ((16 * 128) >> 4), wt_idesc(64 * NB, true), (accumulate || ks != 0) ? 1u : 0u);
 }
 // `N` columns of a row and the wait for them in one statement, so that nothing reads the registers in between
+template <int O, int M> __device__ __forceinline__ void tmem_row32(uint32_t taddr, float (&z)[M]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(z[O + 0]), "=f"(z[O + 1]), "=f"(z[O + 2]), "=f"(z[O + 3]), "=f"(z[O + 4]), "=f"(z[O + 5]), "=f"(z[O + 6]), "=f"(z[O + 7]),
+        "=f"(z[O + 8]), "=f"(z[O + 9]), "=f"(z[O + 10]), "=f"(z[O + 11]), "=f"(z[O + 12]), "=f"(z[O + 13]), "=f"(z[O + 14]), "=f"(z[O + 15]),
+        "=f"(z[O + 16]), "=f"(z[O + 17]), "=f"(z[O + 18]), "=f"(z[O + 19]), "=f"(z[O + 20]), "=f"(z[O + 21]), "=f"(z[O + 22]), "=f"(z[O + 23]),
+        "=f"(z[O + 24]), "=f"(z[O + 25]), "=f"(z[O + 26]), "=f"(z[O + 27]), "=f"(z[O + 28]), "=f"(z[O + 29]), "=f"(z[O + 30]), "=f"(z[O + 31])
+      : "r"(taddr)
+      : "memory");
+}
 template <int O, int M> __device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&z)[M]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"

@@ -18,8 +18,8 @@ namespace lb2 {
 
 namespace {
 
-// warp 0: TMA, warp 1: MMA, warps 4-11: softmax; registers 56 + 2 x 224 = 3 x 168 per thread at launch
-constexpr int kWtBwdThreads = 384, kWtBwdFew = 56, kWtBwdMany = 224, kWtSoft = 256;
+// warp 0: TMA, warp 1: MMA, warps 4-11: softmax; registers 88 + 2 x 208 = 3 x 168 per thread at launch
+constexpr int kWtBwdThreads = 384, kWtBwdFew = 88, kWtBwdMany = 208, kWtSoft = 256;
 
 struct WtBwdParams {
   WinParams w;
@@ -29,7 +29,7 @@ struct WtBwdParams {
   const float* delta;
   float* partial;
   float* sink_sums;                          // [split][tile][batch][kv head][128][D + E], fp32
-  int tiles, columns, boxes_d, boxes_e;
+  int tiles, items, columns, boxes_d, boxes_e, wide_d;
   int sink_tiles, splits;                    // dk, dv: the first tiles, whose keys all later queries see, are shared by `splits` blocks
   unsigned int* status;
 };
@@ -42,6 +42,59 @@ template <int NB> struct WtBwd {
   static constexpr int SMEM = (2 + STAGES) * TILE + EXTRA + 256 + 1024;
 };
 
+// a tile of queries and the tiles of keys that it visits; the longest (last) tiles first
+struct WtQueries {
+  int l0, h, b, queries, keys;
+  WtTiles own;
+  __device__ __forceinline__ WtQueries(const WtBwdParams& p, int item) {
+    const int rest = item / p.tiles;
+    l0 = (p.tiles - 1 - item % p.tiles) * kWtTile;
+    h = rest % p.w.H; b = rest / p.w.H;
+    queries = warp_uniform(win_tokens(p.w, b, p.w.L)); keys = warp_uniform(win_tokens(p.w, b, p.w.S));
+    own = wt_key_tiles(p.w, l0, queries, keys);
+  }
+};
+// Adds 32 rows x 64 columns of d to the warp's sums by bucket. 16 columns at a time a lane hands the sum of its diagonal r - j on to the
+// next lane's column; lane 31's is complete. Then neighbouring diagonals of one bucket join.
+__device__ __forceinline__ void wt_diagonals(const float (&d)[64], float* my_diag, float* my_bsum, const uint8_t* bucket, int half, int quarter, int lane) {
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      a[c] += d[16 * c + j];
+      if (j < 15) {
+        if (lane == 31) my_diag[c * 48 + 46 - j] = a[c];                // diagonal d at d + 15
+        const float up = __shfl_up_sync(0xffffffffu, a[c], 1);
+        a[c] = lane == 0 ? 0.f : up;
+      }
+    }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) my_diag[c * 48 + lane] = a[c];            // r - 15
+  __syncwarp();
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    const int D = part * 32 + lane;                                     // r - j + 63 over the 64 columns, 95 of them
+    float t = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = D - 63 + 16 * c + 15;
+      if (k >= 0 && k < 47 && D < 95) t += my_diag[c * 48 + k];
+    }
+    // key - query, from the tile's lowest: j_tile - r_tile + 127
+    const int bk = bucket[min(254, max(0, (63 - D) + half * 64 - quarter * 32 + 127))];
+    const int mine = D < 95 ? bk : -1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float up = __shfl_up_sync(0xffffffffu, t, o);
+      const int other = __shfl_up_sync(0xffffffffu, mine, o);
+      if (lane >= o && other == mine) t += up;
+    }
+    const int following = __shfl_down_sync(0xffffffffu, mine, 1);
+    if (mine >= 0 && (lane == 31 || following != mine)) my_bsum[mine] += t;
+    __syncwarp();
+  }
+}
 __device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 template <int NB>
@@ -55,31 +108,28 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
   float* diag = lut + 2 * 256;                                                     // [warp][4][48]
   float* bsum = diag + 8 * 4 * 48;                                                 // [warp][buckets]
-  int* bad = reinterpret_cast<int*>(bsum + 8 * 2 * kWinMaxBuckets);                // [128]
+  int* bad = reinterpret_cast<int*>(bsum + 8 * 2 * kWinMaxBuckets);
   uint8_t* of = reinterpret_cast<uint8_t*>(bad + 128);                             // [parity][256]
   uint64_t* bars = reinterpret_cast<uint64_t*>(of + 2 * 256);
-  uint64_t *q_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 2, *ds_ready = dp_full + 1,
-           *o_full = ds_ready + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  uint64_t *q_full = bars, *q_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 2,
+           *ds_ready = dp_full + 1, *o_full = ds_ready + 1, *o_empty = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
   const uint32_t sQ = base, sG = base + C::TILE, sKV = base + 2 * C::TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinParams& w = p.w;
-  const int tile = blockIdx.x % p.tiles, hb = blockIdx.x / p.tiles, h = hb % w.H, b = hb / w.H, g = h / w.rep, l0 = tile * kWtTile;
-  const int queries = win_tokens(w, b, w.L), keys = win_tokens(w, b, w.S);
-  const WtTiles own = wt_key_tiles(w, l0, queries, keys);
-  const int n = own.count();
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
+    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmG); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+    mbar_init(q_full, 1); mbar_init(q_empty, 1);
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(o_full, 1);
+    mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(o_full, 1); mbar_init(o_empty, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (threadIdx.x < 128) bad[threadIdx.x] = 0;
+  if (threadIdx.x == 0) *bad = 0;
   for (int i = threadIdx.x; i < 8 * 2 * kWinMaxBuckets; i += kWtBwdThreads) bsum[i] = 0.f;
   tc_fence_before();
   __syncthreads();
@@ -88,263 +138,263 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   if (warp < 4) {
     regs_less<kWtBwdFew>();
-    if (warp == 0 && n > 0) {
-      if (elect_one()) {
-        mbar_expect_tx(q_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
-        for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sQ + x * kWtBox, &tmQ, x * 64, h, l0, b, q_full);
-        for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sG + x * kWtBox, &tmG, x * 64, h, l0, b, q_full);
-      }
-      __syncwarp();
-      uint32_t stage = 0, phase = 0;
-      for (int i = 0; i < 2 * n; ++i) {
-        if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) break;
+    if (warp == 0) {
+      uint32_t stage = 0, phase = 0, turn = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        const WtQueries t(p, item);
+        const int n = t.own.count();
+        if (n == 0) continue;
+        if (!mbar_wait_uniform(q_empty, (turn & 1u) ^ 1u, p.status, 0x80u)) break;
+        ++turn;
         if (elect_one()) {
-          const bool is_k = (i & 1) == 0;
-          const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = own.at(i >> 1) * kWtTile;
-          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
-          for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, g, s0, b, &full[stage]);
+          mbar_expect_tx(q_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
+          for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sQ + x * kWtBox, &tmQ, x * 64, t.h, t.l0, t.b, q_full);
+          for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sG + x * kWtBox, &tmG, x * 64, t.h, t.l0, t.b, q_full);
         }
         __syncwarp();
-        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-      }
-    } else if (warp == 1 && n > 0) {
-      bool ok = mbar_wait_uniform(q_full, 0, p.status, 0x200u);
-      auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
-      auto slot = [&](int i) { return sKV + (uint32_t)(i % C::STAGES) * C::TILE; };
-      auto scores = [&](int i) {
-        if (elect_one()) {
-          if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem + (i & 1) * 128, sQ, slot(2 * i));
-          else wt_mma_features<1>(tmem + (i & 1) * 128, sQ, slot(2 * i));
-          umma_commit(&s_full[i & 1]);
-        }
-        __syncwarp();
-      };
-      auto grads = [&](int i) {
-        if (elect_one()) {
-          if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, slot(2 * i + 1));
-          else wt_mma_features<1>(tDP, sG, slot(2 * i + 1));
-          umma_commit(dp_full);
-          umma_commit(&empty[(2 * i + 1) % C::STAGES]);
-        }
-        __syncwarp();
-      };
-      for (int i = -1; i < n && ok; ++i) {
-        const bool next = i + 1 < n;
-        if (next) {
-          if (!wait_stage(2 * (i + 1))) { ok = false; break; }
-          tc_fence_after();
-          scores(i + 1);
-        }
-        if (i >= 0) {
-          if (!mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
-          tc_fence_after();
-        }
-        if (next) {
-          if (!wait_stage(2 * (i + 1) + 1)) { ok = false; break; }
-          tc_fence_after();
-          grads(i + 1);
-        }
-        if (i >= 0) {
+        for (int i = 0; i < 2 * n; ++i) {
+          if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) { ok = false; break; }
           if (elect_one()) {
-            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDQ, tmem + (i & 1) * 128, slot(2 * i), i > 0);
-            else wt_mma_tokens_halves<1>(tDQ, tmem + (i & 1) * 128, slot(2 * i), i > 0);
-            umma_commit(&empty[(2 * i) % C::STAGES]);
-            if (!next) umma_commit(o_full);
+            const bool is_k = (i & 1) == 0;
+            const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = t.own.at(i >> 1) * kWtTile;
+            mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
+            for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, t.h / w.rep, s0, t.b, &full[stage]);
           }
           __syncwarp();
+          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
+      }
+    } else if (warp == 1) {
+      uint32_t turn = 0, kst = 0, vst = 0, ph_k = 0, ph_v = 0, done = 0;   // items; the ring's next tiles; tiles so far
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        const WtQueries t(p, item);
+        const int n = t.own.count();
+        if (n == 0) continue;
+        if (!mbar_wait_uniform(q_full, turn & 1u, p.status, 0x200u)) break;
+        uint32_t kprev = 0;                                                // where tile i's keys are
+        for (int i = -1; i < n; ++i) {
+          const bool next = i + 1 < n;
+          const uint32_t cur = (done + (uint32_t)i) & 1u, nxt = cur ^ 1u, k = sKV + 2 * kst * C::TILE, v = sKV + (2 * vst + 1) * C::TILE;
+          if (next) {
+            if (!mbar_wait_uniform(&full[2 * kst], ph_k, p.status, 0x400u)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+              if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem + nxt * 128, sQ, k);
+              else wt_mma_features<1>(tmem + nxt * 128, sQ, k);
+              umma_commit(&s_full[nxt]);
+            }
+            __syncwarp();
+          }
+          if (i >= 0) {
+            if (!mbar_wait_uniform(ds_ready, cur, p.status, 0x800u)) { ok = false; break; }
+            if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
+            tc_fence_after();
+          }
+          if (next && !mbar_wait_uniform(&full[2 * vst + 1], ph_v, p.status, 0x400u)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (next) {
+              if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, v);
+              else wt_mma_features<1>(tDP, sG, v);
+              umma_commit(dp_full);
+              umma_commit(&empty[2 * vst + 1]);
+              if (i + 2 == n) umma_commit(q_empty);
+            }
+            if (i >= 0) {
+              const uint32_t kc = sKV + 2 * kprev * C::TILE;
+              if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDQ, tmem + cur * 128, kc, i > 0);
+              else wt_mma_tokens_halves<1>(tDQ, tmem + cur * 128, kc, i > 0);
+              umma_commit(&empty[2 * kprev]);
+              if (!next) umma_commit(o_full);
+            }
+          }
+          __syncwarp();
+          kprev = kst;
+          if (next) {
+            if (++kst == C::STAGES / 2) { kst = 0; ph_k ^= 1u; }
+            if (++vst == C::STAGES / 2) { vst = 0; ph_v ^= 1u; }
+          }
+        }
+        ++turn;
+        done += (uint32_t)n;
       }
     }
   } else {
     regs_more<kWtBwdMany>();
-    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, l = l0 + row, st = threadIdx.x - 128;
+    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, st = threadIdx.x - 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
-    const int64_t at = ((int64_t)b * w.H + h) * w.L + l;
-    const float2 stat = l < queries ? p.stats[at] : make_float2(0.f, INFINITY);
-    const float delta = l < queries ? p.delta[at] : 0.f;
-    const uint64_t nm = pack2(-stat.x, -stat.x), nl = pack2(-stat.y, -stat.y), nd = pack2(-delta, -delta);
     float* my_bsum = bsum + sw * 2 * kWinMaxBuckets;
     float* my_diag = diag + sw * 4 * 48;
-    float flat_sum = 0.f;
-    int flat_bucket = -1;
-    auto flush = [&]() {
-      const float t = warp_sum(flat_sum);
-      if (flat_bucket >= 0 && lane == 0) my_bsum[flat_bucket] += t;
-      __syncwarp();
-      flat_sum = 0.f;
-    };
-    bool ok = true;
-    int turn = 0;                       // of the tiles with more than one bucket: each has a barrier, two tables are enough
-    for (int i = 0; i < n; ++i) {
-      const int s0 = own.at(i) * kWtTile;
-      float flat = 0.f;
-      const float* bias = nullptr;
-      const uint8_t* bucket = nullptr;
-      if (biased) {
-        const int low = s0 - l0 - (kWtTile - 1), bl = win_bucket(w.buckets, low);
-        if (bl == win_bucket(w.buckets, low + 2 * (kWtTile - 1))) {
-          flat = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bl]));
-          if (bl != flat_bucket) { flush(); flat_bucket = bl; }
-        } else {
-          float* to = lut + turn * 256;
-          if (st < 255) {
-            const int bk = win_bucket(w.buckets, low + st);
-            to[st] = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bk]));
-            of[turn * 256 + st] = (uint8_t)bk;
+    bool ok = true;                     // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
+    uint32_t done = 0, turn = 0;        // tiles and items so far
+    int table = 0;                      // of the tiles with more than one bucket: each has a barrier, two tables are enough
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+      const WtQueries t(p, item);
+      const int l0 = t.l0, l = l0 + row, n = t.own.count(), h = t.h;
+      const WtView<kWtTile> view(w, l0, t.queries, t.keys);
+      const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
+      const int64_t at = ((int64_t)t.b * w.H + h) * w.L + l;
+      const float2 stat = l < t.queries ? p.stats[at] : make_float2(0.f, INFINITY);
+      const float delta = l < t.queries ? p.delta[at] : 0.f;
+      const uint64_t nm = pack2(-stat.x, -stat.x), nl = pack2(-stat.y, -stat.y), nd = pack2(-delta, -delta);
+      float left_sum = 0.f, right_sum = 0.f;
+      for (int i = 0; i < n; ++i) {
+        const int s0 = t.own.at(i) * kWtTile, low = s0 - l0 - (kWtTile - 1);
+        const uint32_t cur = (done + (uint32_t)i) & 1u;
+        float flat = 0.f;
+        const float* bias = nullptr;
+        const uint8_t* bucket = nullptr;
+        const bool in_left = biased && tail.is_left(low + 2 * (kWtTile - 1));
+        if (biased) {
+          if (in_left) {
+            flat = tail.left;
+          } else if (tail.is_right(w, low)) {
+            flat = tail.right;
+          } else {
+            float* to = lut + table * 256;
+            if (st < 255) {
+              const int bk = win_bucket(w.buckets, low + st);
+              to[st] = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bk]));
+              of[table * 256 + st] = (uint8_t)bk;
+            }
+            bar_group(1, kWtSoft);
+            bias = to + (kWtTile - 1 - row) + half * 64;
+            bucket = of + table * 256;
+            table ^= 1;
           }
-          bar_group(1, kWtSoft);
-          bias = to + (kWtTile - 1 - row) + half * 64;
-          bucket = of + turn * 256;
-          turn ^= 1;
+        }
+        ok = ok && mbar_wait_warp(&s_full[cur], ((done + (uint32_t)i) >> 1) & 1u, p.status, 0x1000u);
+        tc_fence_after();
+        const uint32_t tS = tmem + lanes + cur * 128 + half * 64;
+        float d[64];
+        tmem_row64<0>(tS, d);
+        const uint64_t mul2_ = pack2(c2, c2);
+        if (bias == nullptr && wt_apart(c2, flat)) {
+          const float off = (flat - stat.x) - stat.y;
+          const uint64_t off2_ = pack2(off, off);
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            float e0, e1;
+            unpack2(fma2(pack2(d[j], d[j + 1]), mul2_, off2_), e0, e1);
+            d[j] = ex2(e0); d[j + 1] = ex2(e1);
+          }
+        } else {
+          const uint64_t flat2_ = pack2(flat, flat);
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const uint64_t add = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_;
+            float e0, e1;
+            unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add), nm), nl), e0, e1);
+            d[j] = ex2(e0); d[j + 1] = ex2(e1);
+          }
+        }
+        ok = ok && mbar_wait_warp(dp_full, cur, p.status, 0x2000u);
+        tc_fence_after();
+        {
+          float e[64];
+          tmem_row64<0>(tDP + lanes + half * 64, e);
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const uint64_t y = mul2(add2(pack2(e[j], e[j + 1]), nd), pack2(d[j], d[j + 1]));
+            unpack2(y, d[j], d[j + 1]);
+          }
+        }
+        if (!view.whole(s0)) {
+          const WtSeen seen(w, l, t.queries, s0, t.keys);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t bits = seen.bits(half * 64 + q * 32);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
+          }
+        }
+        {
+          uint32_t v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+          tmem_st32(tS, v);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+        if (biased) {
+          if (bucket == nullptr) {
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 64; ++j) part[j & 3] += d[j];
+            (in_left ? left_sum : right_sum) += (part[0] + part[1]) + (part[2] + part[3]);
+          } else {
+            wt_diagonals(d, my_diag, my_bsum, bucket, half, quarter, lane);
+          }
         }
       }
-      if (!mbar_wait_warp(&s_full[i & 1], (uint32_t)(i >> 1) & 1u, p.status, 0x1000u)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t tS = tmem + lanes + (i & 1) * 128 + half * 64;
-      float d[64];
-      const bool apart = bias == nullptr && wt_apart(c2, flat);
-      const float off = (flat - stat.x) - stat.y;
-      const uint64_t mul2_ = pack2(c2, c2), off2_ = pack2(off, off), flat2_ = pack2(flat, flat);
-      tmem_row64<0>(tS, d);
-      if (apart) {
-#pragma unroll
-        for (int j = 0; j < 64; j += 2) {
-          float e0, e1;
-          unpack2(fma2(pack2(d[j], d[j + 1]), mul2_, off2_), e0, e1);
-          d[j] = ex2(e0); d[j + 1] = ex2(e1);
+      done += (uint32_t)n;
+      if (biased) {
+        const float a = warp_sum(left_sum), c = warp_sum(right_sum);
+        if (lane == 0) {
+          my_bsum[w.buckets.count - 1] += a;
+          my_bsum[w.buckets.bidirectional ? 2 * w.buckets.count - 1 : 0] += c;
         }
+        bar_group(1, kWtSoft);
+        if (st < p.columns) {
+          float sum = 0.f;
+          for (int x = 0; x < 8; ++x) {
+            sum += bsum[x * 2 * kWinMaxBuckets + st];
+            bsum[x * 2 * kWinMaxBuckets + st] = 0.f;
+          }
+          p.partial[((int64_t)(l0 / kWtTile) * w.B * w.H + (int64_t)t.b * w.H + h) * p.columns + st] = sum;
+        }
+        bar_group(1, kWtSoft);
+      }
+      float o[32 * NB];
+      if (n > 0) {
+        ok = ok && mbar_wait_warp(o_full, turn & 1u, p.status, 0x4000u);
+        ++turn;
+        tc_fence_after();
+        if constexpr (NB == 2) tmem_row64<0>(tDQ + lanes + half * 64, o);
+        else tmem_row32<0>(tDQ + lanes + half * 32, o);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty);
       } else {
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) {
-          const uint64_t add = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_;
-          float e0, e1;
-          unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add), nm), nl), e0, e1);
-          d[j] = ex2(e0); d[j + 1] = ex2(e1);
-        }
+        for (int j = 0; j < 32 * NB; ++j) o[j] = 0.f;
       }
-      if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
-      tc_fence_after();
-      const bool whole = wt_all_seen(w, l0, queries, s0, keys);
-      {
-        float e[64];
-        tmem_row64<0>(tDP + lanes + half * 64, e);
-#pragma unroll
-        for (int j = 0; j < 64; j += 2) {
-          const uint64_t y = mul2(add2(pack2(e[j], e[j + 1]), nd), pack2(d[j], d[j + 1]));
-          unpack2(y, d[j], d[j + 1]);
-        }
-      }
-      if (!whole) {
-        const WtSeen seen(w, l, queries, s0, keys);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t bits = seen.bits(half * 64 + q * 32);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
-        }
-      }
-      {
-        uint32_t v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
-        tmem_st32(tS, v);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
-      if (biased) {
-        if (bucket == nullptr) {
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 64; ++j) part[j & 3] += d[j];
-          flat_sum += (part[0] + part[1]) + (part[2] + part[3]);
-        } else {
-          // 16 columns at a time: a lane hands the sum of its diagonal r - j on to the next lane's column; lane 31's is complete
-          float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              a[c] += d[16 * c + j];
-              if (j < 15) {
-                if (lane == 31) my_diag[c * 48 + 46 - j] = a[c];                // diagonal d at d + 15
-                const float up = __shfl_up_sync(0xffffffffu, a[c], 1);
-                a[c] = lane == 0 ? 0.f : up;
-              }
-            }
-#pragma unroll
-          for (int c = 0; c < 4; ++c) my_diag[c * 48 + lane] = a[c];            // r - 15
-          __syncwarp();
-#pragma unroll
-          for (int part = 0; part < 3; ++part) {
-            const int D = part * 32 + lane;                                     // r - j + 63 over the warp's 64 columns, 95 of them
-            float t = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int k = D - 63 + 16 * c + 15;
-              if (k >= 0 && k < 47 && D < 95) t += my_diag[c * 48 + k];
-            }
-            // rel - low = j_tile - r_tile + 127
-            const int bk = bucket[min(254, max(0, (63 - D) + half * 64 - quarter * 32 + 127))];
-            const int mine = D < 95 ? bk : -1;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const float up = __shfl_up_sync(0xffffffffu, t, o);
-              const int other = __shfl_up_sync(0xffffffffu, mine, o);
-              if (lane >= o && other == mine) t += up;
-            }
-            const int following = __shfl_down_sync(0xffffffffu, mine, 1);
-            if (mine >= 0 && (lane == 31 || following != mine)) my_bsum[mine] += t;
-            __syncwarp();
-          }
-        }
-      }
-    }
-    if (ok && biased) {
-      flush();
-      bar_group(1, kWtSoft);
-      if (st < p.columns) {
-        float t = 0.f;
-        for (int x = 0; x < 8; ++x) t += bsum[x * 2 * kWinMaxBuckets + st];
-        p.partial[((int64_t)tile * w.B * w.H + (int64_t)b * w.H + h) * p.columns + st] = t;
-      }
-    }
-    if (ok && n > 0) ok = mbar_wait_warp(o_full, 0, p.status, 0x4000u);
-    if (ok) {
-      tc_fence_after();
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.dq) + (((int64_t)b * w.L + l) * w.H + h) * w.D;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.dq) + (((int64_t)t.b * w.L + l) * w.H + h) * w.D;
       bool fine = true;
 #pragma unroll
-      for (int q = 0; q < NB; ++q) {
-        const int c0 = half * NB * 32 + q * 32;
-        if (c0 >= w.D) break;
-        uint32_t v[32] = {};
-        if (n > 0) {
-          tmem_ld32(tDQ + lanes + c0, v);
-          tmem_ld_wait();
+      for (int q = 0; q < 2 * NB; ++q) {
+        const int c0 = half * NB * 32 + q * 16;
+        uint32_t v[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float a = o[q * 16 + 2 * x] * w.scale, c = o[q * 16 + 2 * x + 1] * w.scale;
+          if (c0 + 2 * x < w.D) fine = fine && isfinite(a) && isfinite(c);
+          v[x] = l < t.queries ? pack_bf16(a, c) : 0u;
         }
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint32_t o[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float a = __uint_as_float(v[j + 2 * k]) * w.scale, c = __uint_as_float(v[j + 2 * k + 1]) * w.scale;
-            if (c0 + j < w.D) fine = fine && isfinite(a) && isfinite(c);
-            o[k] = l < queries ? pack_bf16(a, c) : 0u;
-          }
-          if (l < w.L && c0 + j < w.D) *reinterpret_cast<uint4*>(out + c0 + j) = make_uint4(o[0], o[1], o[2], o[3]);
+        if (l < w.L) wt_store16(out + c0, v, w.D - c0, p.wide_d != 0);
+      }
+      if (l < t.queries && !fine) *bad = 1;
+    }
+    // rows that an infinity or NaN reached, once the pipeline no longer waits for these warps
+    bar_group(1, kWtSoft);
+    if (*bad != 0 && ok) {
+      for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+        const WtQueries t(p, item);
+        for (int r = sw; r < kWtTile && t.l0 + r < t.queries; r += 8) {
+          const int64_t at = ((int64_t)t.b * w.H + t.h) * w.L + t.l0 + r;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.dq) + (((int64_t)t.b * w.L + t.l0 + r) * w.H + t.h) * w.D;
+          bool fine = true;
+          for (int e = lane; e < w.D; e += 32) fine = fine && isfinite(__bfloat162float(out[e]));
+          if (!__all_sync(0xffffffffu, fine))
+            win_row_dq<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dq), p.dx, p.stats[at], p.delta[at], t.l0 + r, t.h, t.b, t.keys);
         }
       }
-      if (l < queries && !fine) bad[row] = 1;
-      bar_group(1, kWtSoft);
-      for (int r = sw; r < kWtTile; r += 8)
-        if (bad[r]) {
-          const int64_t ar = ((int64_t)b * w.H + h) * w.L + l0 + r;
-          win_row_dq<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dq), p.dx, p.stats[ar], p.delta[ar], l0 + r, h, b, keys);
-        }
     }
   }
 
@@ -387,7 +437,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tile = p.sink_tiles + r % per; gb = r / per;
   }
   const int g = gb % w.Hkv, b = gb / w.Hkv, s0 = tile * kWtTile;
-  const int queries = win_tokens(w, b, w.L), keys = win_tokens(w, b, w.S);
+  const int queries = warp_uniform(win_tokens(w, b, w.L)), keys = warp_uniform(win_tokens(w, b, w.S));
   int lo, hi;
   win_query_range(w, s0, min(s0 + kWtTile, keys), queries, &lo, &hi);
   const int first = lo / kWtTile, per_head = s0 < keys && lo < hi ? (hi + kWtTile - 1) / kWtTile - first : 0;
@@ -432,50 +482,47 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     } else if (warp == 1 && n > 0) {
       bool ok = mbar_wait_uniform(k_full, 0, p.status, 0x200u);
-      auto wait_stage = [&](int i) { return mbar_wait_uniform(&full[i % C::STAGES], (uint32_t)(i / C::STAGES) & 1u, p.status, 0x400u); };
-      auto slot = [&](int i) { return sQG + (uint32_t)(i % C::STAGES) * C::TILE; };
+      uint32_t qst = 0, gst = 0, ph_q = 0, ph_g = 0, qprev = 0, gprev = 0;
       for (int i = -1; i < n && ok; ++i) {
         const bool next = i + 1 < n;
-        if (i >= 0) {
-          if (!mbar_wait_uniform(p_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, slot(2 * i + 1), i > 0);
-            else wt_mma_tokens_halves<1>(tDV, tmem, slot(2 * i + 1), i > 0);
-            umma_commit(&empty[(2 * i + 1) % C::STAGES]);
+        const uint32_t qn = sQG + 2 * qst * C::TILE, gn = sQG + (2 * gst + 1) * C::TILE, qc = sQG + 2 * qprev * C::TILE, gc = sQG + (2 * gprev + 1) * C::TILE;
+        if (i >= 0 && !mbar_wait_uniform(p_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
+        if (next && !mbar_wait_uniform(&full[2 * qst], ph_q, p.status, 0x400u)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          if (i >= 0) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, gc, i > 0);
+            else wt_mma_tokens_halves<1>(tDV, tmem, gc, i > 0);
+            umma_commit(&empty[2 * gprev + 1]);
           }
-          __syncwarp();
-        }
-        if (next) {
-          if (!wait_stage(2 * (i + 1))) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, slot(2 * (i + 1)));
-            else wt_mma_features<1>(tmem, sK, slot(2 * (i + 1)));
+          if (next) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, qn);
+            else wt_mma_features<1>(tmem, sK, qn);
             umma_commit(s_full);
           }
-          __syncwarp();
         }
-        if (i >= 0) {
-          if (!mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x8000u)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, slot(2 * i), i > 0);
-            else wt_mma_tokens_halves<1>(tDK, tDP, slot(2 * i), i > 0);
-            umma_commit(&empty[(2 * i) % C::STAGES]);
+        __syncwarp();
+        if (i >= 0 && !mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x8000u)) { ok = false; break; }
+        if (next && !mbar_wait_uniform(&full[2 * gst + 1], ph_g, p.status, 0x400u)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          if (i >= 0) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, qc, i > 0);
+            else wt_mma_tokens_halves<1>(tDK, tDP, qc, i > 0);
+            umma_commit(&empty[2 * qprev]);
             if (!next) umma_commit(o_full);
           }
-          __syncwarp();
-        }
-        if (next) {
-          if (!wait_stage(2 * (i + 1) + 1)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, slot(2 * (i + 1) + 1));
-            else wt_mma_features<1>(tDP, sV, slot(2 * (i + 1) + 1));
+          if (next) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, gn);
+            else wt_mma_features<1>(tDP, sV, gn);
             umma_commit(dp_full);
           }
-          __syncwarp();
+        }
+        __syncwarp();
+        qprev = qst; gprev = gst;
+        if (next) {
+          if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
+          if (++gst == C::STAGES / 2) { gst = 0; ph_g ^= 1u; }
         }
       }
     }
@@ -504,9 +551,12 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       float flat = 0.f;
       const float* bias = nullptr;
       if (biased) {
-        const int low = s0 - l0 - (kWtTile - 1), bl = win_bucket(w.buckets, low);
-        if (bl == win_bucket(w.buckets, low + 2 * (kWtTile - 1))) {
-          flat = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bl]));
+        const int low = s0 - l0 - (kWtTile - 1);
+        const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
+        if (tail.is_left(low + 2 * (kWtTile - 1))) {
+          flat = tail.left;
+        } else if (tail.is_right(w, low)) {
+          flat = tail.right;
         } else {                                   // index (column - row) + 127: rel = low + 254 - index
           float* to = lut + (i & 1) * 256;
           if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, h, low + 254 - st);
@@ -520,7 +570,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
       if (s >= keys) to = -1;
       const bool whole = wt_all_seen(w, l0, queries, s0, keys);
-      if (!mbar_wait_warp(s_full, (uint32_t)i & 1u, p.status, 0x1000u)) { ok = false; break; }
+      ok = ok && mbar_wait_warp(s_full, (uint32_t)i & 1u, p.status, 0x1000u);
       tc_fence_after();
       float d[64];
       const bool apart = bias == nullptr && wt_apart(c2, flat);
@@ -566,7 +616,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_ready);
-      if (!mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u)) { ok = false; break; }
+      ok = ok && mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u);
       tc_fence_after();
       uint32_t o[32];
       {
@@ -595,8 +645,8 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
     }
-    if (ok && n > 0) ok = mbar_wait_warp(o_full, 0, p.status, 0x4000u);
-    if (ok && splits > 1) {
+    if (n > 0) ok = ok && mbar_wait_warp(o_full, 0, p.status, 0x4000u);
+    if (splits > 1) {
       tc_fence_after();
       float* out = p.sink_sums + ((((int64_t)split * p.sink_tiles + tile) * groups + gb) * kWtTile + row) * (w.D + w.E);
 #pragma unroll
@@ -619,7 +669,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                                                                    __uint_as_float(v[j + 2]) * f, __uint_as_float(v[j + 3]) * f);
         }
       }
-    } else if (ok) {
+    } else {
       tc_fence_after();
       bool fine = true;
 #pragma unroll
@@ -736,7 +786,11 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
     return LB2_OK;
   };
   const bool one = p.boxes_d == 1 && p.boxes_e == 1;
-  int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, qt * w.H * w.B) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, qt * w.H * w.B);
+  LB2_REQUIRE(qt * w.H * w.B <= 0x7FFF0000, LB2_BAD_SHAPE, "too many rows");           // and a grid more
+  p.items = (int)(qt * w.H * w.B);
+  p.wide_d = aligned_to(dq, 32) && w.D % 16 == 0;
+  const int64_t resident = std::min(p.items, sm_count());
+  int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, resident);
   if (rc != LB2_OK) return rc;
   const int64_t groups = (int64_t)w.Hkv * w.B, blocks = (kt - p.sink_tiles + (int64_t)p.sink_tiles * p.splits) * groups;
   LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
