@@ -16,59 +16,148 @@ int32_t check_rel_buckets(const lb2_rel_buckets* t) {
 
 namespace {
 
-constexpr int kRelRows = 64;      // queries per partial sum
+constexpr int kRelRows = 64;      // queries per block
 
+// Forward: a block writes kRelRows x kRelKeys values of a head, all from the kRelRows + kRelKeys - 1 diagonals that it works out once.
+// Shared memory holds the diagonals once per alignment (copy r starts at diagonal r), so that a 16-byte store of neighbouring keys is
+// one aligned 16-byte load whatever the row. Bounded by the stores: LB2_RELPOS_FWD.
+constexpr int kRelKeys = 1024;
 template <typename T>
 __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, const T* __restrict__ table, const __grid_constant__ lb2_rel_buckets t,
-                                                         int S, int L, int H, int offset, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / S;
-    const int s = (int)(i - row * S), h = (int)(row / L), l = (int)(row - (int64_t)h * L);
-    bias[i] = table[h + (int64_t)H * win_bucket(t, s - l - offset)];
+                                                         int S, int L, int H, int offset) {
+  constexpr int V = 16 / sizeof(T), N = kRelRows + kRelKeys;
+  __shared__ __align__(16) T lut[V][N];
+  const int h = blockIdx.z, s0 = blockIdx.x * kRelKeys, l0 = blockIdx.y * kRelRows, keys = min(kRelKeys, S - s0), rows = min(kRelRows, L - l0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // diagonal i: s - l = s0 - l0 - (kRelRows - 1) + i
+  for (int i = threadIdx.x; i < keys + kRelRows - 1; i += 256) {
+    const T v = table[h + (int64_t)H * win_bucket(t, s0 - l0 - (kRelRows - 1) + i - offset)];
+#pragma unroll
+    for (int r = 0; r < V; ++r)
+      if (i >= r) lut[r][i - r] = v;
+  }
+  __syncthreads();
+  for (int row = warp; row < rows; row += 8) {
+    T* out = bias + ((int64_t)h * L + l0 + row) * S + s0;
+    const int first = kRelRows - 1 - row;                                 // diagonal of the row's first key
+    const int head = min(keys, (int)((16 - reinterpret_cast<uintptr_t>(out) % 16) % 16 / sizeof(T))), end = head + (keys - head) / V * V;
+    if (lane < head) out[lane] = lut[0][first + lane];
+    if (end + lane < keys) out[end + lane] = lut[0][first + end + lane];
+    const int r = (first + head) % V;
+    for (int s = head + lane * V; s < end; s += 32 * V) store16_stream(out + s, load16(&lut[r][first + s - r]));
   }
 }
 
-// partial[chunk][h][diagonal]: diagonal i holds s - l = i - (L - 1)
-template <typename T>
-__global__ void __launch_bounds__(256) relpos_diag_kernel(float* __restrict__ partial, const T* __restrict__ dbias, int S, int L, int H, int B) {
-  const int i = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, chunk = blockIdx.z, d = i - (L - 1);
-  if (i >= S + L - 1) return;
-  const int lo = max(chunk * kRelRows, -d), hi = min(min((chunk + 1) * kRelRows, L), S - d);
-  float sum = 0.f;
-  for (int b = 0; b < B; ++b)
-    for (int l = lo; l < hi; ++l) sum += to_f32(dbias[(((int64_t)b * H + h) * L + l) * S + l + d]);
-  partial[((int64_t)chunk * H + h) * (S + L - 1) + i] = sum;
-}
-// a block per (head, bucket): its diagonals of all chunks, 64 bits
-template <typename T>
-__global__ void __launch_bounds__(256) relpos_bucket_kernel(T* __restrict__ dtable, const float* __restrict__ partial,
-                                                            const __grid_constant__ lb2_rel_buckets t, int S, int L, int H, int offset, int chunks) {
-  __shared__ double red[8];
-  const int h = blockIdx.x, j = blockIdx.y, n = S + L - 1;
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256)
-    if (win_bucket(t, i - (L - 1) - offset) == j)
-      for (int c = 0; c < chunks; ++c) sum += partial[((int64_t)c * H + h) * n + i];
+// Backward: a warp takes 32 V neighbouring keys (V per lane, one load) of V queries at a time. A lane's V x V values lie on 2 V - 1
+// diagonals; V of them, complete for this lane, are the next lane's upper ones in the next V queries: they move there with
+// a shuffle, and out of lane 31 to the warp's sums in shared memory. The block joins its warps, then diagonals by bucket;
+// all in a fixed order. Bounded by the loads: LB2_RELPOS_BWD.
+constexpr int kRelWarps = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __restrict__ partial, const T* __restrict__ dbias,
+                                                                    const __grid_constant__ lb2_rel_buckets t, int S, int L, int H, int B, int offset,
+                                                                    int columns) {
+  constexpr int KEYS = 32 * V, N = KEYS + kRelRows;                       // diagonal i: s - l = s0 - l0 - (kRelRows - 1) + i
+  __shared__ __align__(16) float sums[kRelWarps][N];
+  __shared__ uint8_t of[N];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.z, s0 = blockIdx.x * KEYS, l0 = blockIdx.y * kRelRows;
+  for (int i = threadIdx.x; i < N; i += 32 * kRelWarps) {
+    of[i] = (uint8_t)win_bucket(t, s0 - l0 - (kRelRows - 1) + i - offset);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+    for (int w = 0; w < kRelWarps; ++w) sums[w][i] = 0.f;
+  }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; ++w) sum += red[w];
-    dtable[h + (int64_t)H * j] = from_f32<T>((float)sum);
+  // the warps share the samples, or the rows where samples are few
+  const bool by_sample = B >= kRelWarps;
+  const int lo = by_sample ? 0 : warp * (kRelRows / kRelWarps), hi = min(L - l0, by_sample ? kRelRows : lo + kRelRows / kRelWarps);
+  const int s = s0 + lane * V;
+  float* my = sums[warp];
+  for (int b = by_sample ? warp : 0; b < B; b += by_sample ? kRelWarps : 1) {
+    const T* in = dbias + (((int64_t)b * H + h) * L + l0) * S + s;
+    float a[2 * V - 1];                                                   // diagonal s - row + x - (V - 1) of the block of V rows
+#pragma unroll
+    for (int x = 0; x < 2 * V - 1; ++x) a[x] = 0.f;
+    int row = lo;
+    for (; row < hi; row += V) {
+      if (row > lo) {
+#pragma unroll
+        for (int x = 0; x < V; ++x) {
+          const float up = __shfl_up_sync(0xffffffffu, a[V - 1 + x], 1);
+          if (lane == 31) my[31 * V + x + kRelRows - 1 - (row - V)] += a[V - 1 + x];
+          a[V - 1 + x] = (lane == 0 ? 0.f : up) + (x > 0 ? a[x - 1] : 0.f);
+        }
+#pragma unroll
+        for (int x = 0; x < V - 1; ++x) a[x] = 0.f;
+        __syncwarp();
+      }
+      if constexpr (V == 1) {
+        if (s < S) a[0] += to_f32(in[(int64_t)row * S]);
+      } else {
+        Vec16<T> v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          v[k].raw = make_uint4(0, 0, 0, 0);
+          if (row + k < hi && s < S) v[k] = load16_stream(in + (int64_t)(row + k) * S);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+          for (int e = 0; e < V; ++e) a[e - k + V - 1] += v[k].get(e);
+      }
+    }
+    row -= V;                                                             // the last block's first row; empty where lo >= hi
+    if (lo < hi) {
+      // neighbouring lanes share diagonals: the upper ones first, then the lower ones
+#pragma unroll
+      for (int x = 0; x < V; ++x) my[lane * V + x + kRelRows - 1 - row] += a[V - 1 + x];
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < V - 1; ++x) {
+        const int i = lane * V + x - (V - 1) + kRelRows - 1 - row;
+        if (i >= 0) my[i] += a[x];                                        // rows past the last held zeros
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < N; i += 32 * kRelWarps) {
+    float v = sums[0][i];
+#pragma unroll
+    for (int w = 1; w < kRelWarps; ++w) v += sums[w][i];
+    sums[0][i] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x < columns) {
+    float v = 0.f;
+    for (int i = 0; i < N; ++i)
+      if (of[i] == threadIdx.x) v += sums[0][i];
+    partial[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * H + h) * columns + threadIdx.x] = v;
   }
 }
+// dtable[h, bucket]: the blocks' sums, 64 bits, a warp per entry
+template <typename T>
+__global__ void __launch_bounds__(256) relpos_join_kernel(T* __restrict__ dtable, const float* __restrict__ partial, int H, int columns, int64_t n) {
+  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);     // h + H * bucket
+  if (i >= H * columns) return;
+  const int h = i % H, c = i / H;
+  double s = 0.0;
+  for (int64_t j = lane; j < n; j += 32) s += partial[(j * H + h) * columns + c];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) dtable[i] = from_f32<T>((float)s);
+}
+
+int rel_columns(const lb2_rel_buckets* t) { return t->count * (t->bidirectional ? 2 : 1); }
+int64_t rel_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
 
 int32_t relpos_check(const lb2_rel_buckets* t, int64_t S, int64_t L, int64_t H, int64_t offset, int32_t dtype) {
   LB2_REQUIRE(valid_dtype(dtype), LB2_UNSUPPORTED_DTYPE, "dtype %d not supported", (int)dtype);
   LB2_REQUIRE(S >= 0 && L >= 0 && H >= 0, LB2_BAD_SHAPE, "negative extent");
-  const int64_t big = 1 << 22;
+  const int64_t big = 65535 * kRelRows;                 // blocks along a grid's second axis
   LB2_REQUIRE(S <= big && L <= big && H <= 65535, LB2_BAD_SHAPE, "extent too large");
   LB2_REQUIRE(offset >= -(1 << 29) && offset <= (1 << 29), LB2_BAD_ARG, "offset too large");
   return check_rel_buckets(t);
 }
-int rel_columns(const lb2_rel_buckets* t) { return t->count * (t->bidirectional ? 2 : 1); }
-
 }  // namespace
 
 }  // namespace lb2
@@ -85,19 +174,18 @@ int32_t lb2_relpos_bias_fwd(void* bias, const void* table, const lb2_rel_buckets
   LB2_REQUIRE(bias && table, LB2_BAD_ARG, "null tensor pointer");
   const size_t es = dtype_size(dtype);
   LB2_REQUIRE(aligned_to(bias, es) && aligned_to(table, es), LB2_BAD_ALIGN, "pointer not aligned to the element size");
-  const int64_t n = S * L * H, blocks = (n + 255) / 256, cap = (int64_t)sm_count() * 8;
+  const dim3 grid((unsigned)rel_blocks(S, kRelKeys), (unsigned)rel_blocks(L, kRelRows), (unsigned)H);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LB2_DISPATCH_DTYPE(dtype, {
-    relpos_fwd_kernel<T><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, st>>>((T*)bias, (const T*)table, *buckets, (int)S, (int)L, (int)H, (int)offset, n);
+    relpos_fwd_kernel<T><<<grid, 256, 0, st>>>((T*)bias, (const T*)table, *buckets, (int)S, (int)L, (int)H, (int)offset);
   });
   LB2_CHECK_LAUNCH("relative position bias");
   return LB2_OK;
 }
 
 size_t lb2_relpos_bias_bwd_workspace_bytes(const lb2_rel_buckets* buckets, int64_t S, int64_t L, int64_t H, int64_t B) {
-  (void)buckets;
-  if (S <= 0 || L <= 0 || H <= 0 || B <= 0) return 0;
-  return align_up((size_t)((L + kRelRows - 1) / kRelRows * H * (S + L - 1)) * sizeof(float), 256);
+  if (buckets == nullptr || S <= 0 || L <= 0 || H <= 0 || B <= 0) return 0;
+  return align_up((size_t)(rel_blocks(S, 32) * rel_blocks(L, kRelRows) * H * rel_columns(buckets)) * sizeof(float), 256);
 }
 
 int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_buckets* buckets, int64_t S, int64_t L, int64_t H, int64_t B,
@@ -115,19 +203,24 @@ int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_bucke
   const size_t need = lb2_relpos_bias_bwd_workspace_bytes(buckets, S, L, H, B);
   LB2_REQUIRE(none || (workspace != nullptr && workspace_bytes >= need), LB2_WORKSPACE_TOO_SMALL, "workspace of %zu bytes needed", need);
   LB2_REQUIRE(aligned_to(workspace, 256), LB2_BAD_ALIGN, "workspace must be 256-byte aligned");
-  const int chunks = none ? 0 : (int)((L + kRelRows - 1) / kRelRows);
-  LB2_REQUIRE(chunks <= 65535, LB2_BAD_SHAPE, "too many queries");
   float* partial = static_cast<float*>(workspace);
+  const int columns = rel_columns(buckets);
+  int64_t blocks = 0;
   LB2_DISPATCH_DTYPE(dtype, {
     if (!none) {
-      relpos_diag_kernel<T><<<dim3((unsigned)((S + L - 1 + 255) / 256), (unsigned)H, (unsigned)chunks), 256, 0, st>>>(partial, (const T*)dbias, (int)S, (int)L,
-                                                                                                                   (int)H, (int)B);
-      LB2_CHECK_LAUNCH("relative position bias diagonals");
+      constexpr int V = Vec16<T>::N;
+      auto launch = [&](auto kernel, int keys) {       // whole vectors only where every row starts on one
+        const dim3 grid((unsigned)rel_blocks(S, keys), (unsigned)rel_blocks(L, kRelRows), (unsigned)H);
+        blocks = (int64_t)grid.x * grid.y;
+        kernel<<<grid, 32 * kRelWarps, 0, st>>>(partial, (const T*)dbias, *buckets, (int)S, (int)L, (int)H, (int)B, (int)offset, columns);
+      };
+      if (S % V == 0 && aligned_to(dbias, 16)) launch(relpos_bwd_kernel<T, V>, 32 * V);
+      else launch(relpos_bwd_kernel<T, 1>, 32);
+      LB2_CHECK_LAUNCH("relative position bias gradient");
     }
-    relpos_bucket_kernel<T><<<dim3((unsigned)H, (unsigned)rel_columns(buckets)), 256, 0, st>>>((T*)dtable, partial, *buckets, (int)S, (int)L, (int)H,
-                                                                                            (int)offset, chunks);
+    relpos_join_kernel<T><<<(unsigned)rel_blocks(H * columns, 8), 256, 0, st>>>((T*)dtable, partial, (int)H, columns, blocks);
   });
-  LB2_CHECK_LAUNCH("relative position bias buckets");
+  LB2_CHECK_LAUNCH("relative position bias gradient's sums");
   return LB2_OK;
 }
 

@@ -22,7 +22,7 @@ import torch
 
 from . import _cabi
 from ._cabi import ArgumentError, DimensionMismatch
-from .arrays import as_colmajor, current_stream, dtype_code, is_colmajor, jl_empty, jl_reshape, ptr, workspace
+from .arrays import as_colmajor, colmajor_strides, current_stream, dtype_code, jl_empty, jl_reshape, ptr, workspace
 
 # --------------------------------------------------------------------------------------------
 # activations
@@ -888,15 +888,15 @@ def _buckets_struct(buckets: RelativeBuckets):
     return t
 
 
-def _on_one_device(**tensors):
-    """All on one CUDA device, which is returned: a host pointer would be read by the kernels as a device address."""
+def _same_device(**metas):
+    """The one CUDA device of all: a host pointer would be read by the kernels as a device address."""
     device = None
-    for name, t in tensors.items():
-        if t is None:
+    for name, m in metas.items():
+        if m is None:
             continue
-        if t.device.type != "cuda" or (device is not None and t.device != device):
-            raise ArgumentError(f"{name} must be on the CUDA device of the other arrays, not on {t.device}")
-        device = t.device
+        if m[3].type != "cuda" or (device is not None and m[3] != device):
+            raise ArgumentError(f"{name} must be on the CUDA device of the other arrays, not on {m[3]}")
+        device = m[3]
     return device
 
 
@@ -910,15 +910,16 @@ def _launch(device, name, *args):
             _cabi.check(getattr(lib, name)(*args, current_stream(device)))
 
 
-def _table_of(table, buckets, heads: int):
-    """The bias table as the library takes it, and its buckets' descriptor."""
+def _check_table(table, buckets, heads: int):
     if (table is None) != (buckets is None):
         raise ArgumentError("table and buckets must both be given or both be nothing")
-    if table is None:
-        return None, None
-    if tuple(table.shape) != (heads, len(buckets)):
-        raise DimensionMismatch(f"the bias table must have the shape (heads, buckets) = ({heads}, {len(buckets)}), not {tuple(table.shape)}")
-    return as_colmajor(table), C.byref(_buckets_struct(buckets))
+    if table is not None and table[0] != (heads, len(buckets)):
+        raise DimensionMismatch(f"the bias table must have the shape (heads, buckets) = ({heads}, {len(buckets)}), not {table[0]}")
+
+
+def _table_of(table, buckets):
+    """The bias table as the library takes it, and its buckets' descriptor."""
+    return (None, None) if table is None else (as_colmajor(table), C.byref(_buckets_struct(buckets)))
 
 
 def relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: int, *, offset: int = 0):
@@ -927,8 +928,9 @@ def relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: 
     if table.dim() != 2:
         raise DimensionMismatch("the bias table must be a matrix (heads, buckets)")
     S, Lq, H = int(keys), int(queries), table.shape[0]
-    device = _on_one_device(table=table)
-    T, plan = _table_of(table, buckets, H)
+    device = _same_device(table=_meta(table))
+    _check_table(_meta(table), buckets, H)
+    T, plan = _table_of(table, buckets)
     bias = jl_empty((S, Lq, H, 1), T.dtype, device)
     _launch(device, "lb2_relpos_bias_fwd", ptr(bias), ptr(T), plan, S, Lq, H, int(offset), dtype_code(T.dtype))
     return bias
@@ -943,7 +945,7 @@ def rrule_relative_position_bias(table, buckets: RelativeBuckets, keys: int, que
         if tuple(delta.shape[:3]) != (S, Lq, H):
             raise DimensionMismatch(f"the cotangent must have the shape ({S}, {Lq}, {H}, ...)")
         d = _cotangent(delta, bias.dtype)
-        device = _on_one_device(table=bias, cotangent=d)
+        device = _same_device(table=_meta(bias), cotangent=_meta(d))
         plan, Bn = C.byref(_buckets_struct(buckets)), math.prod(d.shape[3:])
         dtable = jl_empty((H, len(buckets)), bias.dtype, device)
         _, wsp, wsn = _ws(_cabi.load().lb2_relpos_bias_bwd_workspace_bytes(plan, S, Lq, H, Bn), device)
@@ -953,34 +955,49 @@ def rrule_relative_position_bias(table, buckets: RelativeBuckets, keys: int, que
     return bias, pullback
 
 
-def _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths, want_stats):
-    if q.dim() < 4 or k.dim() != q.dim() or v.dim() != q.dim():
-        raise AssertionError("N must be at least 4")
-    device = _on_one_device(q=q, k=k, v=v, table=table, lengths=lengths)
-    q, k, v, table = _promote(q, k, v, table)
-    Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
-    D, H, Lq = Q.shape[:3]
-    Hkv, S = Kx.shape[1], Kx.shape[2]
-    E, batch_shape = V.shape[0], tuple(Q.shape[3:])
-    if Kx.shape[0] != D:
+def _meta(t):
+    return None if t is None else (tuple(t.shape), t.stride(), t.dtype, t.device)
+
+
+def _dense(meta) -> bool:
+    """Column-major without gaps: the library takes the array as it is."""
+    return all(s == x or d == 1 for s, x, d in zip(meta[1], colmajor_strides(meta[0]), meta[0])) or 0 in meta[0]
+
+
+@functools.lru_cache(maxsize=4096)
+def _windowed_plan(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths):
+    """The checks of a windowed attention call, which the arrays' shapes, types and devices decide, once per set of them:
+    (dims, scale, dtype code, device, output shape)."""
+    device = _same_device(q=q, k=k, v=v, table=table, lengths=lengths)
+    (D, H, Lq), (Hkv, S), E, batch_shape = q[0][:3], k[0][1:3], v[0][0], q[0][3:]
+    if k[0][0] != D:
         raise AssertionError("`q` and `k` must have the same head dimension")
-    if batch_shape != tuple(Kx.shape[3:]) or batch_shape != tuple(V.shape[3:]):
+    if batch_shape != k[0][3:] or batch_shape != v[0][3:]:
         raise DimensionMismatch("All dimensions (except first 3) of q, k, v must be the same")
-    if V.shape[2] != S or V.shape[1] != Hkv:
+    if v[0][2] != S or v[0][1] != Hkv:
         raise AssertionError("`v` and `k` must have the same number of tokens and heads")
     if Hkv == 0 or H % Hkv != 0:
         raise AssertionError("num_heads must be divisible by num_kv_groups")
     Bn = math.prod(batch_shape)
-    if lengths is not None:
-        if lengths.numel() != Bn:
-            raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {lengths.numel()}")
-        lengths = as_colmajor(lengths.to(torch.int32))
-    Tb, plan = _table_of(table, buckets, H)
+    if lengths is not None and math.prod(lengths[0]) != Bn:
+        raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {math.prod(lengths[0])}")
+    _check_table(table, buckets, H)
     sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
-    dt = dtype_code(Q.dtype)
     dims = _cabi.WindowDims(D, E, H, Hkv, Lq, S, Bn, int(window), int(sinks), int(bool(is_causal)))
-    out = jl_empty((E, H, Lq) + batch_shape, Q.dtype, device)
-    stats = torch.empty(2 * Lq * H * Bn, dtype=torch.float32, device=device) if want_stats else None
+    return dims, sc, dtype_code(q[2]), device, (E, H, Lq) + batch_shape
+
+
+def _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths, want_stats):
+    if q.dim() < 4 or k.dim() != q.dim() or v.dim() != q.dim():
+        raise AssertionError("N must be at least 4")
+    q, k, v, table = _promote(q, k, v, table)
+    dims, sc, dt, device, xshape = _windowed_plan(_meta(q), _meta(k), _meta(v), window, sinks, is_causal, scale, _meta(table), buckets, _meta(lengths))
+    Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
+    if lengths is not None:
+        lengths = as_colmajor(lengths.to(torch.int32))
+    Tb, plan = _table_of(table, buckets)
+    out = jl_empty(xshape, Q.dtype, device)
+    stats = torch.empty(2 * dims.queries * dims.heads * dims.batch, dtype=torch.float32, device=device) if want_stats else None
     _launch(device, "lb2_window_attention_fwd", ptr(out), ptr(stats), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lengths), sc, C.byref(dims), dt)
     return out, (stats, Q, Kx, V, Tb, plan, lengths, sc, dims, dt, device)
 
@@ -1002,7 +1019,7 @@ def rrule_windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal:
         if tuple(dx.shape) != tuple(x.shape):
             raise DimensionMismatch("the cotangent must have the shape of the output")
         G = _cotangent(dx, Q.dtype)
-        _on_one_device(q=Q, cotangent=G)
+        _same_device(q=_meta(Q), cotangent=_meta(G))
         dq, dk, dv = (jl_empty(tuple(t.shape), Q.dtype, device) for t in (Q, Kx, V))
         dtable = jl_empty(tuple(Tb.shape), Q.dtype, device) if Tb is not None else None
         _, wsp, wsn = _ws(_cabi.load().lb2_window_attention_bwd_workspace_bytes(C.byref(dims), plan, dt), device)
@@ -1016,14 +1033,39 @@ def rrule_windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal:
 def _check_caches(kcache, vcache, k, v):
     """The caches are written in place: they are taken as they are or not at all."""
     for name, c, t in (("kcache", kcache, k), ("vcache", vcache, v)):
-        if c.dtype != t.dtype:
-            raise ArgumentError(f"{name} holds {c.dtype}, the new tokens are {t.dtype}")
-        if not is_colmajor(c):
+        if c[2] != t[2]:
+            raise ArgumentError(f"{name} holds {c[2]}, the new tokens are {t[2]}")
+        if not _dense(c):
             raise ArgumentError(f"{name} must be a dense column-major array")
-        if c.dim() < 3 or c.shape[0] != t.shape[0] or c.shape[1] != t.shape[1]:
+        if len(c[0]) < 3 or c[0][:2] != t[0][:2]:
             raise DimensionMismatch(f"{name} must have the shape (features, kv heads, capacity, batch...) of the tokens it takes")
-    if tuple(kcache.shape[2:]) != tuple(vcache.shape[2:]):
+    if kcache[0][2:] != vcache[0][2:]:
         raise DimensionMismatch("kcache and vcache must have the same capacity and batch")
+
+
+@functools.lru_cache(maxsize=4096)
+def _step_plan(q, k, v, kcache, vcache, lengths, window, sinks, scale, table, buckets):
+    """The checks of a step, as _windowed_plan: (dims, scale, dtype code, device, output shape, whether all arrays are dense)."""
+    device = _same_device(q=q, k=k, v=v, kcache=kcache, vcache=vcache, lengths=lengths, table=table)
+    if len(q[0]) < 3 or len(k[0]) != len(q[0]) or len(v[0]) != len(q[0]):
+        raise AssertionError("N must be at least 3")
+    if not q[2] == k[2] == v[2] or (table is not None and table[2] != q[2]):
+        raise ArgumentError("q, k, v and the table must have one element type")
+    _check_caches(kcache, vcache, k, v)
+    (D, H), (E, Hkv), batch_shape = q[0][:2], v[0][:2], q[0][2:]
+    if k[0][:2] != (D, Hkv):
+        raise AssertionError("`q` and `k` must have the same head dimension, `k` and `v` the same heads")
+    if k[0][2:] != batch_shape or v[0][2:] != batch_shape or kcache[0][3:] != batch_shape:
+        raise DimensionMismatch("q, k, v and the caches must have the same batch")
+    if Hkv == 0 or H % Hkv != 0:
+        raise AssertionError("num_heads must be divisible by num_kv_groups")
+    Bn = math.prod(batch_shape)
+    if lengths[2] != torch.int32 or math.prod(lengths[0]) != Bn:
+        raise ArgumentError(f"lengths must hold one Int32 per sample ({Bn})")
+    _check_table(table, buckets, H)
+    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
+    dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache[0][2], Bn, int(window), int(sinks), 1)
+    return dims, sc, dtype_code(q[2]), device, (E, H) + batch_shape, all(_dense(m) for m in (q, k, v, lengths, table) if m is not None)
 
 
 def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, sinks: int = 0, scale=None, table=None, buckets=None):
@@ -1031,40 +1073,24 @@ def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, si
     over the caches kcache (D, Hkv, capacity, B...), vcache (E, Hkv, capacity, B...), which take the token in place: position p goes to
     slot p while p < sinks, then to sinks + (p - sinks) mod (capacity - sinks); capacity >= sinks + window. `lengths` (B..., Int32 on
     the device, not changed) counts the tokens before this one; where it is negative there is no sequence: x is zero, the caches stay."""
-    device = _on_one_device(q=q, k=k, v=v, kcache=kcache, vcache=vcache, lengths=lengths, table=table)
-    if q.dim() < 3 or k.dim() != q.dim() or v.dim() != q.dim():
-        raise AssertionError("N must be at least 3")
-    if not (q.dtype == k.dtype == v.dtype) or (table is not None and table.dtype != q.dtype):
-        raise ArgumentError("q, k, v and the table must have one element type")
-    _check_caches(kcache, vcache, k, v)
-    Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
-    (D, H), (E, Hkv), batch_shape = Q.shape[:2], V.shape[:2], tuple(Q.shape[2:])
-    if Kx.shape[0] != D or Kx.shape[1] != Hkv:
-        raise AssertionError("`q` and `k` must have the same head dimension, `k` and `v` the same heads")
-    if any(tuple(t.shape[-len(batch_shape):]) != batch_shape for t in (Kx, V)) or tuple(kcache.shape[3:]) != batch_shape:
-        raise DimensionMismatch("q, k, v and the caches must have the same batch")
-    if Hkv == 0 or H % Hkv != 0:
-        raise AssertionError("num_heads must be divisible by num_kv_groups")
-    Bn = math.prod(batch_shape)
-    if lengths.dtype != torch.int32 or lengths.numel() != Bn:
-        raise ArgumentError(f"lengths must hold one Int32 per sample ({Bn})")
-    lens = as_colmajor(lengths)
-    Tb, plan = _table_of(table, buckets, H)
-    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
-    dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache.shape[2], Bn, int(window), int(sinks), 1)
-    x = jl_empty((E, H) + batch_shape, Q.dtype, device)
-    _launch(device, "lb2_window_attention_step", ptr(x), ptr(kcache), ptr(vcache), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lens), sc,
-            C.byref(dims), dtype_code(Q.dtype))
+    dims, sc, dt, device, xshape, dense = _step_plan(_meta(q), _meta(k), _meta(v), _meta(kcache), _meta(vcache), _meta(lengths), window, sinks, scale,
+                                                     _meta(table), buckets)
+    if not dense:
+        q, k, v, lengths = (as_colmajor(t) for t in (q, k, v, lengths))
+    table, plan = _table_of(table, buckets)
+    x = jl_empty(xshape, q.dtype, device)
+    _launch(device, "lb2_window_attention_step", ptr(x), ptr(kcache), ptr(vcache), ptr(q), ptr(k), ptr(v), ptr(table), plan, ptr(lengths), sc,
+            C.byref(dims), dt)
     return x
 
 
 def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     """Puts a prompt k (D, Hkv, S, B...), v (E, Hkv, S, B...) into the caches of windowed_attention_step, as if its tokens had come one by
     one; `lengths` (B...) as in windowed_attention. The slots that hold none of them stay as they are."""
-    device = _on_one_device(kcache=kcache, vcache=vcache, k=k, v=v, lengths=lengths)
+    device = _same_device(kcache=_meta(kcache), vcache=_meta(vcache), k=_meta(k), v=_meta(v), lengths=_meta(lengths))
     if k.dim() < 4 or v.dim() != k.dim():
         raise AssertionError("N must be at least 4")
-    _check_caches(kcache, vcache, k, v)
+    _check_caches(_meta(kcache), _meta(vcache), _meta(k), _meta(v))
     Kx, V = as_colmajor(k), as_colmajor(v)
     if tuple(Kx.shape[1:]) != tuple(V.shape[1:]) or tuple(Kx.shape[3:]) != tuple(kcache.shape[3:]):
         raise DimensionMismatch("k, v and the caches must have the same heads, tokens and batch")
