@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
   const int s = s0 + lane * V;
   float* my = sums[warp];
   for (int b = by_sample ? warp : 0; b < B; b += by_sample ? kRelWarps : 1) {
-    const T* in = dbias + (((int64_t)b * H + h) * L + l0) * S + s;
+    const T* in = dbias + (((int64_t)b * H + h) * L + l0) * S + min(s, S - V);
     float a[2 * V - 1];                                                   // diagonal s - row + x - (V - 1) of the block of V rows
 #pragma unroll
     for (int x = 0; x < 2 * V - 1; ++x) a[x] = 0.f;
@@ -91,14 +91,18 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
         __syncwarp();
       }
       if constexpr (V == 1) {
-        if (s < S) a[0] += to_f32(in[(int64_t)row * S]);
+        const float v = to_f32(in[(int64_t)row * S]);
+        a[0] += s < S ? v : 0.f;
       } else {
         Vec16<T> v[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          v[k].raw = make_uint4(0, 0, 0, 0);
-          if (row + k < hi && s < S) v[k] = load16_stream(in + (int64_t)(row + k) * S);
+        for (int k = 0; k < V; ++k) {                                     // volatile: all in flight before the first is used
+          const T* at = in + (int64_t)min(row + k, hi - 1) * S;
+          asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[k].w[0]), "=r"(v[k].w[1]), "=r"(v[k].w[2]), "=r"(v[k].w[3]) : "l"(at));
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (row + k >= hi || s >= S) v[k].raw = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
