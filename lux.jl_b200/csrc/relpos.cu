@@ -2,7 +2,7 @@
 // scaled_dot_product_attention (lib/LuxLib/src/api/attention.jl, impl/attention.jl:76-118) adds to its logits, and its gradient
 // dtable[h, j] = sum of dbias over the pairs (and samples) of bucket j.
 #include "common.cuh"
-#include "window.cuh"
+#include "window_tc.cuh"
 
 namespace lb2 {
 
@@ -29,9 +29,12 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
   __shared__ __align__(16) T lut[V][N];
   const int h = blockIdx.z, s0 = blockIdx.x * kRelKeys, l0 = blockIdx.y * kRelRows, keys = min(kRelKeys, S - s0), rows = min(kRelRows, L - l0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int32_t first_of[kWinMaxBuckets];
+  if (threadIdx.x < kWinMaxBuckets) first_of[threadIdx.x] = t.first[threadIdx.x];
+  __syncthreads();
   // diagonal i: s - l = s0 - l0 - (kRelRows - 1) + i
   for (int i = threadIdx.x; i < keys + kRelRows - 1; i += 256) {
-    const T v = table[h + (int64_t)H * win_bucket(t, s0 - l0 - (kRelRows - 1) + i - offset)];
+    const T v = table[h + (int64_t)H * win_bucket(t, first_of, s0 - l0 - (kRelRows - 1) + i - offset)];
 #pragma unroll
     for (int r = 0; r < V; ++r)
       if (i >= r) lut[r][i - r] = v;
@@ -53,16 +56,18 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
 // a shuffle, and out of lane 31 to the warp's sums in shared memory. The block joins its warps, then diagonals by bucket;
 // all in a fixed order. Bounded by the loads: LB2_RELPOS_BWD.
 constexpr int kRelWarps = 4;
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __restrict__ partial, const T* __restrict__ dbias,
                                                                     const __grid_constant__ lb2_rel_buckets t, int S, int L, int H, int B, int offset,
                                                                     int columns) {
   constexpr int KEYS = 32 * V, N = KEYS + kRelRows;                       // diagonal i: s - l = s0 - l0 - (kRelRows - 1) + i
   __shared__ __align__(16) float sums[kRelWarps][N];
-  __shared__ uint8_t of[N];
+  __shared__ uint4 ring[kRelWarps][2][V == 1 ? 1 : V][32];                // each lane's next loads, two blocks of rows ahead
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.z, s0 = blockIdx.x * KEYS, l0 = blockIdx.y * kRelRows;
   for (int i = threadIdx.x; i < N; i += 32 * kRelWarps) {
-    of[i] = (uint8_t)win_bucket(t, s0 - l0 - (kRelRows - 1) + i - offset);
 #pragma unroll
     for (int w = 0; w < kRelWarps; ++w) sums[w][i] = 0.f;
   }
@@ -77,7 +82,18 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
     float a[2 * V - 1];                                                   // diagonal s - row + x - (V - 1) of the block of V rows
 #pragma unroll
     for (int x = 0; x < 2 * V - 1; ++x) a[x] = 0.f;
-    int row = lo;
+    auto fetch = [&](int r0, int stage) {
+      if constexpr (V > 1) {
+        if (r0 < hi) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) copy_async16(smem_u32(&ring[warp][stage][k][lane]), in + (int64_t)min(r0 + k, hi - 1) * S);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    };
+    fetch(lo, 0);
+    fetch(lo + V, 1);
+    int row = lo, stage = 0;
     for (; row < hi; row += V) {
       if (row > lo) {
 #pragma unroll
@@ -94,19 +110,17 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
         const float v = to_f32(in[(int64_t)row * S]);
         a[0] += s < S ? v : 0.f;
       } else {
-        Vec16<T> v[V];
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
-        for (int k = 0; k < V; ++k) {                                     // volatile: all in flight before the first is used
-          const T* at = in + (int64_t)min(row + k, hi - 1) * S;
-          asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[k].w[0]), "=r"(v[k].w[1]), "=r"(v[k].w[2]), "=r"(v[k].w[3]) : "l"(at));
+        for (int k = 0; k < V; ++k) {
+          Vec16<T> v;
+          v.raw = ring[warp][stage][k][lane];
+          if (row + k >= hi || s >= S) v.raw = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < V; ++e) a[e - k + V - 1] += v.get(e);
         }
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (row + k >= hi || s >= S) v[k].raw = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-#pragma unroll
-          for (int e = 0; e < V; ++e) a[e - k + V - 1] += v[k].get(e);
+        fetch(row + 2 * V, stage);
+        stage ^= 1;
       }
     }
     row -= V;                                                             // the last block's first row; empty where lo >= hi
@@ -131,11 +145,23 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
     sums[0][i] = v;
   }
   __syncthreads();
-  if (threadIdx.x < columns) {
+  // a bucket's diagonals lie side by side: a warp per bucket
+  const int base = s0 - l0 - (kRelRows - 1) - offset;
+  for (int j = warp; j < columns; j += kRelWarps) {
+    const int k = j < t.count ? j : j - t.count, near = t.first[k], past = k + 1 < t.count ? t.first[k + 1] : 0x7FFFFFFF;
+    int lo, hi;                                                           // relative positions of the bucket
+    if (j < t.count) {
+      lo = -(past - 1);
+      hi = t.bidirectional || near > 0 ? -near : 0x7FFFFFFF;
+      if (!t.bidirectional && near == 0 && past == 0) hi = lo - 1;
+    } else {
+      lo = max(near, 1); hi = past - 1;
+    }
     float v = 0.f;
-    for (int i = 0; i < N; ++i)
-      if (of[i] == threadIdx.x) v += sums[0][i];
-    partial[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * H + h) * columns + threadIdx.x] = v;
+    const int64_t end = min((int64_t)hi - base, (int64_t)N - 1);
+    for (int64_t i = max((int64_t)lo - base, (int64_t)0) + lane; i <= end; i += 32) v += sums[0][i];
+    v = warp_sum(v);
+    if (lane == 0) partial[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * H + h) * columns + j] = v;
   }
 }
 // dtable[h, bucket]: the blocks' sums, 64 bits, a warp per entry

@@ -53,18 +53,23 @@ __device__ __forceinline__ bool win_any(const WinParams& p, int l, int keys) {
   return sinks > 0 || lo < hi;
 }
 
-// bucket of the relative position rel = s - l: the last one that starts at or below the distance
-__device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, int rel) {
+// bucket of the relative position rel = s - l: the last one that starts at or below the distance. `first` is t.first, or a copy of it
+// in shared memory: lanes that look in different places of the parameters are served one by one.
+__device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, const int32_t* first, int rel) {
   const int dist = t.bidirectional ? abs(rel) : max(-rel, 0);
   int lo = 0, n = t.count;                  // invariant: first[lo] <= dist, the answer lies in [lo, lo + n)
   while (n > 1) {
     const int half = n >> 1;
-    if (t.first[lo + half] <= dist) { lo += half; n -= half; } else { n = half; }
+    if (first[lo + half] <= dist) { lo += half; n -= half; } else { n = half; }
   }
   return lo + (t.bidirectional && rel > 0 ? t.count : 0);
 }
+__device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, int rel) { return win_bucket(t, t.first, rel); }
 template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, int h, int rel) {
   return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, rel)]));
+}
+template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, const int32_t* first, int h, int rel) {
+  return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, first, rel)]));
 }
 
 // ---- rows once more ---------------------------------------------------------------------------

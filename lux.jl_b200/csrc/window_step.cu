@@ -173,6 +173,8 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
   static_assert(R == 8 || R == 16, "rows of an m16 tile");
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ float head_bias[R][2 * kWinMaxBuckets];
+  __shared__ int32_t first_of[kWinMaxBuckets];
+  if (threadIdx.x < kWinMaxBuckets) first_of[threadIdx.x] = p.buckets.first[threadIdx.x];
   const StepPlace w = step_place<R>(p);
   step_edges<T, R>(p, w, head_bias);
   if (w.n < 0) return;                             // the whole cluster
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + (k >> 1) * 8 + 2 * t + (k & 1);
-      const int bk = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, -keys.distance(i, w.n)) : 0;
+      const int bk = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, first_of, -keys.distance(i, w.n)) : 0;
 #pragma unroll
       for (int a = 0; a < R / 8; ++a) {
         float v = s[k >> 1][2 * a + (k & 1)] * p.scale2;
@@ -341,6 +343,8 @@ __global__ void __launch_bounds__(kStepThreads) win_step_f32_kernel(const __grid
   extern __shared__ __align__(16) uint8_t raw[];
   auto& j = *reinterpret_cast<StepJoin<R, DC, PARTS>*>(raw);
   __shared__ float head_bias[R][2 * kWinMaxBuckets];
+  __shared__ int32_t first_of[kWinMaxBuckets];
+  if (threadIdx.x < kWinMaxBuckets) first_of[threadIdx.x] = p.buckets.first[threadIdx.x];
   const StepPlace w = step_place<R>(p);
   step_edges<float, R>(p, w, head_bias);
   if (w.n < 0) return;
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_f32_kernel(const __grid
 #pragma unroll
     for (int x = 0; x < U; ++x) {
       const int i = i0 + x * PARTS + part;
-      bk[x] = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, -keys.distance(i, w.n)) : 0;
+      bk[x] = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, first_of, -keys.distance(i, w.n)) : 0;
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {

@@ -23,7 +23,7 @@ constexpr int kWtFwdThreads = 384, kWtFwdFew = 56, kWtFwdMany = 224;
 template <int NB> struct WtFwd {
   static constexpr int TILE = NB * kWtBox;
   static constexpr int STAGES = NB == 1 ? 6 : 4;
-  static constexpr int SMEM = 2 * TILE + STAGES * TILE + 2 * 2 * 256 * 4 + 256 + 1024;
+  static constexpr int SMEM = 2 * TILE + STAGES * TILE + 2 * 2 * 256 * 4 + kWinMaxBuckets * 4 + 256 + 1024;
 };
 
 struct WtFwdParams {
@@ -65,7 +65,8 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);      // [group][parity][256]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(lut + 2 * 2 * 256);
+  int32_t* first = reinterpret_cast<int32_t*>(lut + 2 * 2 * 256);              // where the buckets start
+  uint64_t* bars = reinterpret_cast<uint64_t*>(first + kWinMaxBuckets);
   // [group]: S is there, P is there, its product is in O, O has been read
   uint64_t *q_full = bars, *q_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *p_ready = s_full + 2,
            *pv_done = p_ready + 2, *o_empty = pv_done + 2;
@@ -81,6 +82,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1); mbar_init(&o_empty[i], 4); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + kWinMaxBuckets) first[threadIdx.x - 64] = w.buckets.first[threadIdx.x - 64];
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -202,7 +204,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           } else {                               // index j - row + 127: rel = low + index
             float* at = lut + (grp * 2 + turn) * 256;
             turn ^= 1;
-            for (int x = gt; x < 2 * kWtTile - 1; x += 128) at[x] = win_bias<__nv_bfloat16>(w, h, low + x);
+            for (int x = gt; x < 2 * kWtTile - 1; x += 128) at[x] = win_bias<__nv_bfloat16>(w, first, h, low + x);
             bar_group(1 + grp, 128);
             bias = at + (kWtTile - 1 - row);
           }

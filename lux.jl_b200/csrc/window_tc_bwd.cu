@@ -38,7 +38,7 @@ template <int NB> struct WtBwd {
   static constexpr int TILE = NB * kWtBox;
   static constexpr int STAGES = NB == 1 ? 6 : 4;
   // dq: bias and bucket of the diagonals (two tiles), diagonal sums of 8 warps, bucket sums of 8 warps; dk, dv: bias, columns' stats
-  static constexpr int EXTRA = 2 * 256 * 4 + 2 * 256 + 8 * 4 * 48 * 4 + 8 * 2 * kWinMaxBuckets * 4 + 128 * 4;
+  static constexpr int EXTRA = 2 * 256 * 4 + 2 * 256 + 8 * 4 * 48 * 4 + 8 * 2 * kWinMaxBuckets * 4 + 128 * 4 + kWinMaxBuckets * 4;
   static constexpr int SMEM = (2 + STAGES) * TILE + EXTRA + 256 + 1024;
 };
 
@@ -110,7 +110,8 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   float* bsum = diag + 8 * 4 * 48;                                                 // [warp][buckets]
   int* bad = reinterpret_cast<int*>(bsum + 8 * 2 * kWinMaxBuckets);
   uint8_t* of = reinterpret_cast<uint8_t*>(bad + 128);                             // [parity][256]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(of + 2 * 256);
+  int32_t* first_of = reinterpret_cast<int32_t*>(of + 2 * 256);                    // where the buckets start
+  uint64_t* bars = reinterpret_cast<uint64_t*>(first_of + kWinMaxBuckets);
   uint64_t *q_full = bars, *q_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 2,
            *ds_ready = dp_full + 1, *o_full = ds_ready + 1, *o_empty = o_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
@@ -125,6 +126,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(&s_full[0], 1); mbar_init(&s_full[1], 1); mbar_init(dp_full, 1); mbar_init(ds_ready, 8); mbar_init(o_full, 1); mbar_init(o_empty, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + kWinMaxBuckets) first_of[threadIdx.x - 64] = w.buckets.first[threadIdx.x - 64];
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -257,7 +259,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           } else {
             float* to = lut + table * 256;
             if (st < 255) {
-              const int bk = win_bucket(w.buckets, low + st);
+              const int bk = win_bucket(w.buckets, first_of, low + st);
               to[st] = win_bias2(to_f32(static_cast<const __nv_bfloat16*>(w.table)[h + (int64_t)w.H * bk]));
               of[table * 256 + st] = (uint8_t)bk;
             }
@@ -418,7 +420,8 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
   float* cols = lut + 2 * 256;                                                     // [parity][-m2, -log2 sum, -delta][128]
   int* bad = reinterpret_cast<int*>(cols + 2 * 3 * 128);                           // [128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(bad + 128);
+  int32_t* first_of = reinterpret_cast<int32_t*>(bad + 128);                       // where the buckets start
+  uint64_t* bars = reinterpret_cast<uint64_t*>(first_of + kWinMaxBuckets);
   uint64_t *k_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 1, *p_ready = dp_full + 1,
            *ds_ready = p_ready + 1, *o_full = ds_ready + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
@@ -449,6 +452,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(o_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + kWinMaxBuckets) first_of[threadIdx.x - 64] = w.buckets.first[threadIdx.x - 64];
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -559,7 +563,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           flat = tail.right;
         } else {                                   // index (column - row) + 127: rel = low + 254 - index
           float* to = lut + (i & 1) * 256;
-          if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, h, low + 254 - st);
+          if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, first_of, h, low + 254 - st);
           bias = to + (kWtTile - 1 - row) + half * 64;
         }
       }
