@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
 // diagonals; V of them, complete for this lane, are the next lane's upper ones in the next V queries: they move there with
 // a shuffle, and out of lane 31 to the warp's sums in shared memory. The block joins its warps, then diagonals by bucket;
 // all in a fixed order. Bounded by the loads: LB2_RELPOS_BWD.
-constexpr int kRelWarps = 4;
+constexpr int kRelWarps = 4, kRelBwdRows = 32;    // 32 rows: blocks enough to even out over the SMs
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -63,10 +63,10 @@ template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __restrict__ partial, const T* __restrict__ dbias,
                                                                     const __grid_constant__ lb2_rel_buckets t, int S, int L, int H, int B, int offset,
                                                                     int columns) {
-  constexpr int KEYS = 32 * V, N = KEYS + kRelRows;                       // diagonal i: s - l = s0 - l0 - (kRelRows - 1) + i
+  constexpr int KEYS = 32 * V, N = KEYS + kRelBwdRows;                       // diagonal i: s - l = s0 - l0 - (kRelBwdRows - 1) + i
   __shared__ __align__(16) float sums[kRelWarps][N];
   __shared__ uint4 ring[kRelWarps][2][V == 1 ? 1 : V][32];                // each lane's next loads, two blocks of rows ahead
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.z, s0 = blockIdx.x * KEYS, l0 = blockIdx.y * kRelRows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.z, s0 = blockIdx.x * KEYS, l0 = blockIdx.y * kRelBwdRows;
   for (int i = threadIdx.x; i < N; i += 32 * kRelWarps) {
 #pragma unroll
     for (int w = 0; w < kRelWarps; ++w) sums[w][i] = 0.f;
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
   __syncthreads();
   // the warps share the samples, or the rows where samples are few
   const bool by_sample = B >= kRelWarps;
-  const int lo = by_sample ? 0 : warp * (kRelRows / kRelWarps), hi = min(L - l0, by_sample ? kRelRows : lo + kRelRows / kRelWarps);
+  const int lo = by_sample ? 0 : warp * (kRelBwdRows / kRelWarps), hi = min(L - l0, by_sample ? kRelBwdRows : lo + kRelBwdRows / kRelWarps);
   const int s = s0 + lane * V;
   float* my = sums[warp];
   for (int b = by_sample ? warp : 0; b < B; b += by_sample ? kRelWarps : 1) {
@@ -91,6 +91,17 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
         asm volatile("cp.async.commit_group;" ::: "memory");
       }
     };
+    float next[8];                                                        // V = 1: eight rows at a time
+    auto load8 = [&](int r0) {
+      if constexpr (V == 1) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float v = to_f32(in[(int64_t)min(r0 + k, max(hi - 1, 0)) * S]);
+          next[k] = r0 + k < hi && s < S ? v : 0.f;
+        }
+      }
+    };
+    if (lo < hi) load8(lo);
     fetch(lo, 0);
     fetch(lo + V, 1);
     int row = lo, stage = 0;
@@ -99,16 +110,15 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
 #pragma unroll
         for (int x = 0; x < V; ++x) {
           const float up = __shfl_up_sync(0xffffffffu, a[V - 1 + x], 1);
-          if (lane == 31) my[31 * V + x + kRelRows - 1 - (row - V)] += a[V - 1 + x];
+          if (lane == 31) my[31 * V + x + kRelBwdRows - 1 - (row - V)] += a[V - 1 + x];
           a[V - 1 + x] = (lane == 0 ? 0.f : up) + (x > 0 ? a[x - 1] : 0.f);
         }
 #pragma unroll
         for (int x = 0; x < V - 1; ++x) a[x] = 0.f;
-        __syncwarp();
       }
       if constexpr (V == 1) {
-        const float v = to_f32(in[(int64_t)row * S]);
-        a[0] += s < S ? v : 0.f;
+        a[0] += next[(row - lo) & 7];
+        if (((row - lo) & 7) == 7) load8(row + 1);
       } else {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
@@ -124,14 +134,15 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
       }
     }
     row -= V;                                                             // the last block's first row; empty where lo >= hi
+    __syncwarp();
     if (lo < hi) {
       // neighbouring lanes share diagonals: the upper ones first, then the lower ones
 #pragma unroll
-      for (int x = 0; x < V; ++x) my[lane * V + x + kRelRows - 1 - row] += a[V - 1 + x];
+      for (int x = 0; x < V; ++x) my[lane * V + x + kRelBwdRows - 1 - row] += a[V - 1 + x];
       __syncwarp();
 #pragma unroll
       for (int x = 0; x < V - 1; ++x) {
-        const int i = lane * V + x - (V - 1) + kRelRows - 1 - row;
+        const int i = lane * V + x - (V - 1) + kRelBwdRows - 1 - row;
         if (i >= 0) my[i] += a[x];                                        // rows past the last held zeros
       }
       __syncwarp();
@@ -146,7 +157,7 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
   }
   __syncthreads();
   // a bucket's diagonals lie side by side: a warp per bucket
-  const int base = s0 - l0 - (kRelRows - 1) - offset;
+  const int base = s0 - l0 - (kRelBwdRows - 1) - offset;
   for (int j = warp; j < columns; j += kRelWarps) {
     const int k = j < t.count ? j : j - t.count, near = t.first[k], past = k + 1 < t.count ? t.first[k + 1] : 0x7FFFFFFF;
     int lo, hi;                                                           // relative positions of the bucket
@@ -183,7 +194,7 @@ int64_t rel_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
 int32_t relpos_check(const lb2_rel_buckets* t, int64_t S, int64_t L, int64_t H, int64_t offset, int32_t dtype) {
   LB2_REQUIRE(valid_dtype(dtype), LB2_UNSUPPORTED_DTYPE, "dtype %d not supported", (int)dtype);
   LB2_REQUIRE(S >= 0 && L >= 0 && H >= 0, LB2_BAD_SHAPE, "negative extent");
-  const int64_t big = 65535 * kRelRows;                 // blocks along a grid's second axis
+  const int64_t big = 65535 * kRelBwdRows;                 // blocks along a grid's second axis
   LB2_REQUIRE(S <= big && L <= big && H <= 65535, LB2_BAD_SHAPE, "extent too large");
   LB2_REQUIRE(offset >= -(1 << 29) && offset <= (1 << 29), LB2_BAD_ARG, "offset too large");
   return check_rel_buckets(t);
@@ -215,7 +226,7 @@ int32_t lb2_relpos_bias_fwd(void* bias, const void* table, const lb2_rel_buckets
 
 size_t lb2_relpos_bias_bwd_workspace_bytes(const lb2_rel_buckets* buckets, int64_t S, int64_t L, int64_t H, int64_t B) {
   if (buckets == nullptr || S <= 0 || L <= 0 || H <= 0 || B <= 0) return 0;
-  return align_up((size_t)(rel_blocks(S, 32) * rel_blocks(L, kRelRows) * H * rel_columns(buckets)) * sizeof(float), 256);
+  return align_up((size_t)(rel_blocks(S, 32) * rel_blocks(L, kRelBwdRows) * H * rel_columns(buckets)) * sizeof(float), 256);
 }
 
 int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_buckets* buckets, int64_t S, int64_t L, int64_t H, int64_t B,
@@ -240,7 +251,7 @@ int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_bucke
     if (!none) {
       constexpr int V = Vec16<T>::N;
       auto launch = [&](auto kernel, int keys) {       // whole vectors only where every row starts on one
-        const dim3 grid((unsigned)rel_blocks(S, keys), (unsigned)rel_blocks(L, kRelRows), (unsigned)H);
+        const dim3 grid((unsigned)rel_blocks(S, keys), (unsigned)rel_blocks(L, kRelBwdRows), (unsigned)H);
         blocks = (int64_t)grid.x * grid.y;
         kernel<<<grid, 32 * kRelWarps, 0, st>>>(partial, (const T*)dbias, *buckets, (int)S, (int)L, (int)H, (int)B, (int)offset, columns);
       };
