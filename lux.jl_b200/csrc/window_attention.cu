@@ -565,7 +565,7 @@ size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* d, const 
   if (d == nullptr || !valid_dtype(dtype) || d->queries <= 0 || d->heads <= 0 || d->batch <= 0) return 0;
   if (d->kv_heads <= 0 || d->heads % d->kv_heads != 0) return 0;
   const size_t rows = (size_t)(d->queries * d->heads * d->batch);
-  return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + (win_tc_serves(d, dtype) ? align_up(win_tc_sink_bytes(d), 256) : 0);
+  return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + (win_tc_serves(d, dtype) ? align_up(win_tc_sink_bytes(d), 256) + win_tc_row_bytes(d) : 0);
 }
 
 int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const float* stats, const void* q,
@@ -600,10 +600,11 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   const int64_t qt = win_tiles(d->queries, tile), kt = win_tiles(d->keys, tile);
   LB2_REQUIRE(qt * d->heads * d->batch <= 0x7FFFFFFF && kt * d->kv_heads * d->batch <= 0x7FFFFFFF && (rows + 7) / 8 <= 0x7FFFFFFF, LB2_BAD_SHAPE,
               "too many rows");
-  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(q, 16) &&
+  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(q, 16) &&
       aligned_to(k, 16) && aligned_to(v, 16)) {
-    if ((rc = win_delta(delta, (const __nv_bfloat16*)dx, (const __nv_bfloat16*)x, p, rows, st)) != LB2_OK) return rc;
-    if ((rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, dx, reinterpret_cast<const float2*>(stats), delta, st)) != LB2_OK || columns == 0) return rc;
+    float* constants = sink_sums + align_up(win_tc_sink_bytes(d), 256) / sizeof(float);
+    rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, constants, dx, x, reinterpret_cast<const float2*>(stats), delta, st);
+    if (rc != LB2_OK || columns == 0) return rc;
     win_dtable_kernel<<<(unsigned)((p.H * columns + 7) / 8), 256, 0, st>>>((__nv_bfloat16*)dtable, partial, p.H, columns, win_tc_partials(d) * d->batch);
     LB2_CHECK_LAUNCH("windowed attention dtable");
     return LB2_OK;

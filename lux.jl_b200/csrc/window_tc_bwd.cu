@@ -20,6 +20,7 @@ namespace {
 
 // warp 0: TMA, warp 1: MMA, warps 4-11: softmax; registers 88 + 2 x 208 = 3 x 168 per thread at launch
 constexpr int kWtBwdThreads = 384, kWtBwdFew = 88, kWtBwdMany = 208, kWtSoft = 256;
+constexpr uint32_t kWtRowBytes = 3 * kWtTile * 4;
 
 struct WtBwdParams {
   WinParams w;
@@ -27,9 +28,10 @@ struct WtBwdParams {
   const void* dx;
   const float2* stats;
   const float* delta;
+  float* rows;                               // [batch][head][tile][-m2 | -log2 sum | -delta][128]
   float* partial;
   float* sink_sums;                          // [split][tile][batch][kv head][128][D + E], fp32
-  int tiles, items, columns, boxes_d, boxes_e, wide_d;
+  int tiles, query_tiles, items, columns, boxes_d, boxes_e, wide_d;
   int sink_tiles, splits;                    // dk, dv: the first tiles, whose keys all later queries see, are shared by `splits` blocks
   unsigned int* status;
 };
@@ -239,10 +241,9 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int l0 = t.l0, l = l0 + row, n = t.own.count(), h = t.h;
       const WtView<kWtTile> view(w, l0, t.queries, t.keys);
       const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
-      const int64_t at = ((int64_t)t.b * w.H + h) * w.L + l;
-      const float2 stat = l < t.queries ? p.stats[at] : make_float2(0.f, INFINITY);
-      const float delta = l < t.queries ? p.delta[at] : 0.f;
-      const uint64_t nm = pack2(-stat.x, -stat.x), nl = pack2(-stat.y, -stat.y), nd = pack2(-delta, -delta);
+      const float* of_row = p.rows + (((int64_t)t.b * w.H + h) * p.query_tiles + l0 / kWtTile) * 3 * kWtTile + row;
+      const float neg_m = of_row[0], neg_l = of_row[kWtTile], neg_d = of_row[2 * kWtTile];
+      const uint64_t nm = pack2(neg_m, neg_m), nl = pack2(neg_l, neg_l), nd = pack2(neg_d, neg_d);
       float left_sum = 0.f, right_sum = 0.f;
       for (int i = 0; i < n; ++i) {
         const int s0 = t.own.at(i) * kWtTile, low = s0 - l0 - (kWtTile - 1);
@@ -276,7 +277,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_row64<0>(tS, d);
         const uint64_t mul2_ = pack2(c2, c2);
         if (bias == nullptr && wt_apart(c2, flat)) {
-          const float off = (flat - stat.x) - stat.y;
+          const float off = (flat + neg_m) + neg_l;
           const uint64_t off2_ = pack2(off, off);
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
@@ -418,8 +419,8 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
-  float* cols = lut + 2 * 256;                                                     // [parity][-m2, -log2 sum, -delta][128]
-  int* bad = reinterpret_cast<int*>(cols + 2 * 3 * 128);                           // [128]
+  float* cols = lut + 2 * 256;                                                     // per query tile of the ring: -m2 | -log2 sum | -delta
+  int* bad = reinterpret_cast<int*>(cols + C::STAGES / 2 * 3 * 128);               // [128]
   int32_t* first_of = reinterpret_cast<int32_t*>(bad + 128);                       // where the buckets start
   uint64_t* bars = reinterpret_cast<uint64_t*>(first_of + kWinMaxBuckets);
   uint64_t *k_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 1, *p_ready = dp_full + 1,
@@ -473,14 +474,19 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       __syncwarp();
       uint32_t stage = 0, phase = 0;
+      int h = g * w.rep + begin / per_head, qt = first + begin % per_head;
       for (int i = 0; i < 2 * n; ++i) {
         if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) break;
         if (elect_one()) {
           const bool is_q = (i & 1) == 0;
-          const int boxes = is_q ? p.boxes_d : p.boxes_e, it = begin + (i >> 1), h = g * w.rep + it / per_head, l0 = (first + it % per_head) * kWtTile;
-          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
-          for (int x = 0; x < boxes; ++x) tma_load_4d(sQG + stage * C::TILE + x * kWtBox, is_q ? &tmQ : &tmG, x * 64, h, l0, b, &full[stage]);
+          const int boxes = is_q ? p.boxes_d : p.boxes_e;
+          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox + (is_q ? kWtRowBytes : 0)));
+          for (int x = 0; x < boxes; ++x) tma_load_4d(sQG + stage * C::TILE + x * kWtBox, is_q ? &tmQ : &tmG, x * 64, h, qt * kWtTile, b, &full[stage]);
+          if (is_q)
+            bulk_load_1d(smem_u32(cols) + (stage >> 1) * kWtRowBytes, p.rows + (((int64_t)b * w.H + h) * p.query_tiles + qt) * 3 * kWtTile, kWtRowBytes,
+                         &full[stage]);
         }
+        if ((i & 1) == 1 && ++qt == first + per_head) { qt = first; ++h; }
         __syncwarp();
         if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -536,44 +542,36 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tD = tDP + lanes + half * 64;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
-    // the stats of a tile's queries: threads 0-127 bring the softmax's two, the others delta
-    auto fetch = [&](int i) {
-      float2 f = make_float2(0.f, INFINITY);
-      const int h = g * w.rep + (begin + i) / per_head, l = (first + (begin + i) % per_head) * kWtTile + (st & 127);
-      const int64_t at = ((int64_t)b * w.H + h) * w.L + l;
-      if (st < 128) { if (l < queries) f = p.stats[at]; }
-      else f.x = l < queries ? p.delta[at] : 0.f;
-      return f;
-    };
-    float2 coming = n > 0 ? fetch(0) : make_float2(0.f, 0.f);
     bool ok = true;
+    int h = 0, qt = 0, table = 0;
+    uint32_t qst = 0, ph_q = 0;
+    if (n > 0) { h = g * w.rep + begin / per_head; qt = first + begin % per_head; }
+    WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
     for (int i = 0; i < n; ++i) {
-      const int h = g * w.rep + (begin + i) / per_head, l0 = (first + (begin + i) % per_head) * kWtTile;
-      float* col = cols + (i & 1) * 3 * 128;
-      if (st < 128) { col[st] = -coming.x; col[128 + st] = -coming.y; }
-      else col[256 + st - 128] = -coming.x;
+      const int l0 = qt * kWtTile;
+      const float* col = cols + qst * 3 * kWtTile;
       float flat = 0.f;
       const float* bias = nullptr;
       if (biased) {
         const int low = s0 - l0 - (kWtTile - 1);
-        const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
         if (tail.is_left(low + 2 * (kWtTile - 1))) {
           flat = tail.left;
         } else if (tail.is_right(w, low)) {
           flat = tail.right;
         } else {                                   // index (column - row) + 127: rel = low + 254 - index
-          float* to = lut + (i & 1) * 256;
+          float* to = lut + table * 256;
+          table ^= 1;                              // each use has a barrier: two tables are enough
           if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, first_of, h, low + 254 - st);
+          bar_group(1, kWtSoft);
           bias = to + (kWtTile - 1 - row) + half * 64;
         }
       }
-      bar_group(1, kWtSoft);
-      if (i + 1 < n) coming = fetch(i + 1);
       // the queries that see key s: columns from..to
       int from = w.causal ? s - l0 : (s < w.sinks ? 0 : s - w.window + 1 - l0);
       int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
       if (s >= keys) to = -1;
-      const bool whole = wt_all_seen(w, l0, queries, s0, keys);
+      const bool whole = wt_all_seen(w, l0, queries, s0, keys, kWtTile);
+      ok = ok && mbar_wait_warp(&full[2 * qst], ph_q, p.status, 0x8u);       // the columns' stats
       ok = ok && mbar_wait_warp(s_full, (uint32_t)i & 1u, p.status, 0x1000u);
       tc_fence_after();
       float d[64];
@@ -648,6 +646,11 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
+      if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
+      if (++qt == first + per_head) {
+        qt = first; ++h;
+        if (biased && i + 1 < n) tail = WtFlat(w, static_cast<const __nv_bfloat16*>(w.table), h);
+      }
     }
     if (n > 0) ok = ok && mbar_wait_warp(o_full, 0, p.status, 0x4000u);
     if (splits > 1) {
@@ -720,6 +723,34 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
+// delta[batch][head][query] = dx . x and the rows' constants, LR lanes of a row taking eight features each
+template <int LR>
+__global__ void __launch_bounds__(256) win_tc_rows_kernel(const __grid_constant__ WtBwdParams p, float* __restrict__ delta, const __nv_bfloat16* __restrict__ x) {
+  const WinParams& w = p.w;
+  const int lane = threadIdx.x % LR, padded = p.query_tiles * kWtTile;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;         // (batch, query up to whole tiles, head)
+  const int h = (int)(row % w.H);
+  const int64_t bl = row / w.H;
+  const int b = (int)(bl / padded), l = (int)(bl - (int64_t)b * padded);
+  const bool in = b < w.B && l < w.L;
+  float s = 0.f;
+  if (in && lane * 8 < w.E) {
+    const int64_t at = (((int64_t)b * w.L + l) * w.H + h) * w.E + lane * 8;
+    const Vec16<__nv_bfloat16> u = load16(static_cast<const __nv_bfloat16*>(p.dx) + at), v = load16(x + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(u.get(i), v.get(i), s);
+  }
+#pragma unroll
+  for (int o = LR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane != 0 || b >= w.B) return;
+  const int64_t hb = (int64_t)b * w.H + h;
+  const bool counts = l < win_tokens(w, b, w.L);
+  const float2 stat = counts ? p.stats[hb * w.L + l] : make_float2(0.f, INFINITY);
+  float* to = p.rows + (hb * p.query_tiles + l / kWtTile) * 3 * kWtTile + l % kWtTile;
+  to[0] = -stat.x; to[kWtTile] = -stat.y; to[2 * kWtTile] = counts ? -s : 0.f;
+  if (in) delta[hb * w.L + l] = s;
+}
+
 // dk, dv of the shared tiles: the sums of their blocks in order, a warp per key and head
 __global__ void __launch_bounds__(256) win_tc_sinks_kernel(const __grid_constant__ WtBwdParams p) {
   const WinParams& w = p.w;
@@ -758,6 +789,10 @@ void wt_sink_plan(int64_t queries, int64_t keys, int64_t window, int64_t sinks, 
 
 }  // namespace
 
+size_t win_tc_row_bytes(const lb2_window_dims* d) {
+  return (size_t)((d->queries + kWtTile - 1) / kWtTile * d->heads * d->batch) * kWtRowBytes;
+}
+
 size_t win_tc_sink_bytes(const lb2_window_dims* d) {
   int tiles, splits;
   wt_sink_plan(d->queries, d->keys, std::min(d->window, d->queries + d->keys + 1), d->sinks, d->heads / d->kv_heads, d->kv_heads * d->batch, &tiles, &splits);
@@ -766,10 +801,10 @@ size_t win_tc_sink_bytes(const lb2_window_dims* d) {
 
 int64_t win_tc_partials(const lb2_window_dims* d) { return (d->queries + kWtTile - 1) / kWtTile; }
 
-int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* partial, float* sink_sums, const void* dx, const float2* stats, const float* delta,
-                   cudaStream_t st) {
+int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* partial, float* sink_sums, float* rows, const void* dx, const void* x,
+                   const float2* stats, float* delta, cudaStream_t st) {
   WtBwdParams p{};
-  p.w = w; p.dq = dq; p.dk = dk; p.dv = dv; p.dx = dx; p.stats = stats; p.delta = delta; p.partial = partial; p.sink_sums = sink_sums;
+  p.w = w; p.dq = dq; p.dk = dk; p.dv = dv; p.dx = dx; p.stats = stats; p.delta = delta; p.partial = partial; p.sink_sums = sink_sums; p.rows = rows;
   wt_sink_plan(w.L, w.S, w.window, w.sinks, w.rep, (int64_t)w.Hkv * w.B, &p.sink_tiles, &p.splits);
   p.columns = w.buckets.count * (w.buckets.bidirectional ? 2 : 1);
   p.boxes_d = (w.D + 63) / 64; p.boxes_e = (w.E + 63) / 64;
@@ -781,6 +816,13 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
     return fail(LB2_LAUNCH_FAIL, "windowed attention: cuTensorMapEncodeTiled failed");
   const int64_t qt = (w.L + kWtTile - 1) / kWtTile, kt = (w.S + kWtTile - 1) / kWtTile;
   LB2_REQUIRE(qt * w.H * w.B <= 0x7FFFFFFF && kt * w.Hkv * w.B <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
+  p.query_tiles = (int)qt;
+  const int lanes = w.E <= 64 ? 8 : 16;
+  const int64_t row_blocks = (qt * kWtTile * w.H * w.B * lanes + 255) / 256;
+  LB2_REQUIRE(row_blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
+  if (lanes == 8) win_tc_rows_kernel<8><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x));
+  else win_tc_rows_kernel<16><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x));
+  LB2_CHECK_LAUNCH("windowed attention rows");
   auto launch = [&](auto kernel, int smem, int64_t tiles, int64_t blocks) -> int32_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
