@@ -372,15 +372,18 @@ LB2_API int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_r
  * do not reach it, infinities and NaN among them. head_dim and value_dim up to 256.
  * stats (2, queries, heads, batch), fp32, 8-byte aligned, for the backward call: a reference value of each softmax and the log2 of its
  * sum relative to that (0 and +inf for a query that sees nothing); NULL: not kept.
+ * x_rest (as x; NULL: not kept): what rounding took from x, so that the backward call's dx . x is that of the unrounded result; worth
+ * keeping for LB2_BF16, all zero for LB2_F32.
  * Backward: dq, dk, dv, and dtable (NULL without a table), zero for tokens past lengths[b]; every sum has a fixed order. */
 typedef struct lb2_window_dims {
   int64_t head_dim, value_dim, heads, kv_heads, queries, keys, batch, window, sinks, causal;
 } lb2_window_dims;
-LB2_API int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const void* k, const void* v, const void* table,
+LB2_API int32_t lb2_window_attention_fwd(void* x, void* x_rest, float* stats, const void* q, const void* k, const void* v, const void* table,
                                          const lb2_rel_buckets* buckets, const int32_t* lengths, double scale,
                                          const lb2_window_dims* dims, int32_t dtype, void* stream);
+/* Its pullback, the rule of scaled_dot_product_attention (lib/LuxLib/src/impl/attention.jl:76-118) differentiated. */
 LB2_API size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* dims, const lb2_rel_buckets* buckets, int32_t dtype);
-LB2_API int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const float* stats,
+LB2_API int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const void* x_rest, const float* stats,
                                          const void* q, const void* k, const void* v, const void* table, const lb2_rel_buckets* buckets,
                                          const int32_t* lengths, double scale, const lb2_window_dims* dims, int32_t dtype,
                                          void* workspace, size_t workspace_bytes, void* stream);

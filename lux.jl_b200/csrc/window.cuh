@@ -53,6 +53,14 @@ __device__ __forceinline__ bool win_any(const WinParams& p, int l, int keys) {
   return sinks > 0 || lo < hi;
 }
 
+// Query l sees one key alone: its weight is 1 whatever its logit, so the logit's gradient p (dp - delta) is dp - dp, not the difference
+// of two sums in different orders.
+__device__ __forceinline__ bool win_single(const WinParams& p, int l, int keys) {
+  int sinks, lo, hi;
+  win_key_range(p, l, l + 1, keys, &sinks, &lo, &hi);
+  return sinks + max(0, hi - lo) == 1;
+}
+
 // bucket of the relative position rel = s - l: the last one that starts at or below the distance. `first` is t.first, or a copy of it
 // in shared memory: lanes that look in different places of the parameters are served one by one.
 __device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, const int32_t* first, int rel) {
@@ -65,6 +73,8 @@ __device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, const int32_
   return lo + (t.bidirectional && rel > 0 ? t.count : 0);
 }
 __device__ __forceinline__ int win_bucket(const lb2_rel_buckets& t, int rel) { return win_bucket(t, t.first, rel); }
+// what rounding took from a value; nothing where it is infinite
+__device__ __forceinline__ float win_rest(float a, float rounded) { return isinf(rounded) ? 0.f : a - rounded; }
 template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, int h, int rel) {
   return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, rel)]));
 }
@@ -104,7 +114,8 @@ template <typename T> __device__ __forceinline__ const T* win_kv_row(const WinPa
 
 // stats of a row: the reference m2 that its logits were compared with (their maximum, or a little less) and log2(sum of 2^(z2 - m2)),
 // apart: their sum would lose the second beside an m2 as large as the type's lowest value. A row that sees nothing has (0, inf).
-template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, float2* stats, int l, int h, int b, int keys) {
+// rest: x less its rounding, or null
+template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, T* rest, float2* stats, int l, int h, int b, int keys) {
   const int lane = threadIdx.x & 31, g = h / p.rep;
   float q[kWinLaneDims], t[kWinLaneDims], o[kWinLaneDims] = {};
   win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, q);
@@ -127,7 +138,13 @@ template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& 
   }
 #pragma unroll
   for (int i = 0; i < kWinLaneDims; ++i) o[i] /= sum;
-  win_store_lane(x + (((int64_t)b * p.L + l) * p.H + h) * p.E, p.E, lane, o);
+  const int64_t at = (((int64_t)b * p.L + l) * p.H + h) * p.E;
+  win_store_lane(x + at, p.E, lane, o);
+  if (rest != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kWinLaneDims; ++i) o[i] = win_rest(o[i], to_f32(from_f32<T>(o[i])));
+    win_store_lane(rest + at, p.E, lane, o);
+  }
   if (stats != nullptr && lane == 0) *stats = make_float2(m, log2f(sum));
 }
 
@@ -140,13 +157,14 @@ __device__ __noinline__ void win_row_dq(const WinParams& p, T* dq, const void* d
   win_load_lane(win_q_row<T>(p, dx, p.E, l, h, b), p.E, lane, go);
   int sinks, lo, hi;
   win_key_range(p, l, l + 1, keys, &sinks, &lo, &hi);
+  const bool single = win_single(p, l, keys);
   for (int i0 = 0, n = sinks + max(0, hi - lo); i0 < n; ++i0) {
     const int s = i0 < sinks ? i0 : lo + (i0 - sinks);
     win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
     win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, u);
     float z = win_dot_lane(q, t, p.D) * p.scale2;
     if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
-    const float ds = exp2f((z - stats.x) - stats.y) * (win_dot_lane(go, u, p.E) - delta) * p.scale;
+    const float dp = win_dot_lane(go, u, p.E), ds = exp2f((z - stats.x) - stats.y) * (single ? dp - dp : dp - delta) * p.scale;
 #pragma unroll
     for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(ds, t[i], o[i]);
   }
@@ -156,7 +174,7 @@ __device__ __noinline__ void win_row_dq(const WinParams& p, T* dq, const void* d
 // stats, delta: [batch][head][query]
 template <typename T>
 __device__ __noinline__ void win_row_dkv(const WinParams& p, T* dk, T* dv, const void* dx, const float2* stats, const float* delta, int s, int g,
-                                         int b, int queries) {
+                                         int b, int queries, int keys) {
   const int lane = threadIdx.x & 31;
   float k[kWinLaneDims], v[kWinLaneDims], t[kWinLaneDims], u[kWinLaneDims], ok[kWinLaneDims] = {}, ov[kWinLaneDims] = {};
   win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, k);
@@ -171,7 +189,8 @@ __device__ __noinline__ void win_row_dkv(const WinParams& p, T* dk, T* dv, const
       float z = win_dot_lane(t, k, p.D) * p.scale2;
       if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
       const int64_t at = ((int64_t)b * p.H + h) * p.L + l;
-      const float w = exp2f((z - stats[at].x) - stats[at].y), ds = w * (win_dot_lane(u, v, p.E) - delta[at]) * p.scale;
+      const float w = exp2f((z - stats[at].x) - stats[at].y), dp = win_dot_lane(u, v, p.E);
+      const float ds = w * (win_single(p, l, keys) ? dp - dp : dp - delta[at]) * p.scale;
 #pragma unroll
       for (int i = 0; i < kWinLaneDims; ++i) { ov[i] = fmaf(w, u[i], ov[i]); ok[i] = fmaf(ds, t[i], ok[i]); }
     }

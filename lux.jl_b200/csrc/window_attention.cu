@@ -99,8 +99,13 @@ __device__ __forceinline__ void win_cols(float4 (&o)[TN][NC], const float* P, co
 #pragma unroll 4
   for (int m = 0; m < M; ++m) {
     float w[TN];
+    if constexpr (TN == 4) {
+      const float4 f = ld4(P + m * LDP + 4 * ty);
+      w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < TN; ++i) w[i] = P[m * LDP + TN * ty + i];
+      for (int i = 0; i < TN; ++i) w[i] = P[m * LDP + TN * ty + i];
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const float4 f = ld4(G + m * LD + 4 * tx + 64 * c);
@@ -110,11 +115,14 @@ __device__ __forceinline__ void win_cols(float4 (&o)[TN][NC], const float* P, co
   }
 }
 __device__ __forceinline__ bool finite4(const float4& v) { return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w); }
-template <typename T> __device__ __forceinline__ void win_put4(T* row, int c, int n, const float4& v, float f) {
+template <typename T> __device__ __forceinline__ void win_put4(T* row, int c, int n, const float4& v, float f, T* rest = nullptr) {
   const float a[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (c + i < n) row[c + i] = from_f32<T>(a[i]);
+    if (c + i < n) {
+      row[c + i] = from_f32<T>(a[i]);
+      if (rest != nullptr) rest[c + i] = from_f32<T>(win_rest(a[i], to_f32(from_f32<T>(a[i]))));
+    }
 }
 // the maximum / sum over the 16 threads that share rows
 __device__ __forceinline__ float half_max(float v) {
@@ -147,7 +155,7 @@ template <typename T, int BM> __device__ __forceinline__ void win_fill_diag(floa
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x, float2* __restrict__ stats, const __grid_constant__ WinParams p,
+__global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x, T* __restrict__ rest, float2* __restrict__ stats, const __grid_constant__ WinParams p,
                                                               int tiles, int vecq, int vecv) {
   using C = WinTile<DP>;
   constexpr int BM = C::BM, TM = C::TM, LD = C::LD, LDP = C::LDP, NC = C::NC;
@@ -228,20 +236,21 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       ok = ok && finite4(o[i][c]);
-      win_put4(xb + (int64_t)l * p.H * p.E, 4 * tx + 64 * c, p.E, any ? o[i][c] : make_float4(0.f, 0.f, 0.f, 0.f), inv);
+      win_put4(xb + (int64_t)l * p.H * p.E, 4 * tx + 64 * c, p.E, any ? o[i][c] : make_float4(0.f, 0.f, 0.f, 0.f), inv,
+               rest != nullptr ? rest + (xb - x) + (int64_t)l * p.H * p.E : nullptr);
     }
     if (lb != nullptr && tx == 0) lb[l] = any ? make_float2(m[i], log2f(sum[i])) : make_float2(0.f, INFINITY);
     if (any && !ok) bad[ty + 16 * i] = 1;
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < BM; r += kWinThreads / 32)
-    if (bad[r]) win_row_fwd<T>(p, x, lb != nullptr ? lb + l0 + r : nullptr, l0 + r, h, b, keys);
+    if (bad[r]) win_row_fwd<T>(p, x, rest, lb != nullptr ? lb + l0 + r : nullptr, l0 + r, h, b, keys);
 }
 
 // delta[batch][head][query] = dx . x; LR lanes share a row and take a 16-byte vector each, or (LR = 0) a warp walks it
 template <typename T, int LR>
-__global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delta, const T* __restrict__ dx, const T* __restrict__ x, int E, int H,
-                                                        int L, int64_t rows) {
+__global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delta, const T* __restrict__ dx, const T* __restrict__ x,
+                                                        const T* __restrict__ rest, int E, int H, int L, int64_t rows) {
   constexpr int LANES = LR == 0 ? 32 : LR, V = Vec16<T>::N;
   const int lane = threadIdx.x % LANES;
   const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;      // (batch, query, head)
@@ -249,11 +258,14 @@ __global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delt
   if (row < rows) {
     const T *a = dx + row * E, *c = x + row * E;
     if constexpr (LR == 0) {
-      for (int e = lane; e < E; e += 32) s = fmaf(to_f32(a[e]), to_f32(c[e]), s);
+      for (int e = lane; e < E; e += 32) s = fmaf(to_f32(a[e]), to_f32(c[e]) + (rest != nullptr ? to_f32(rest[row * E + e]) : 0.f), s);
     } else if (lane * V < E) {
       const Vec16<T> u = load16(a + lane * V), v = load16(c + lane * V);
+      Vec16<T> r;
+      r.raw = make_uint4(0, 0, 0, 0);
+      if (rest != nullptr) r = load16(rest + row * E + lane * V);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s = fmaf(u.get(i), v.get(i), s);
+      for (int i = 0; i < V; ++i) s = fmaf(u.get(i), v.get(i) + r.get(i), s);
     }
   }
 #pragma unroll
@@ -289,11 +301,13 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq,
   float4 o[TM][NC];
   float2 ls[TM];
   float de[TM], of_bucket = 0.f;
+  bool single[TM];
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int l = l0 + ty + 16 * i;
     ls[i] = l < queries ? lb[l] : make_float2(0.f, INFINITY);
     de[i] = l < queries ? db[l] : 0.f;
+    single[i] = win_single(p, l, keys);
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
@@ -318,7 +332,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq,
         const int r = ty + 16 * i, c = tx + 16 * j, l = l0 + r, s = s0 + c;
         float u = z[i][j] * p.scale2;
         if (p.buckets.count > 0) u += sD[r - c + BM - 1];
-        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? exp2f((u - ls[i].x) - ls[i].y) * (dp[i][j] - de[i]) : 0.f;
+        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? exp2f((u - ls[i].x) - ls[i].y) * (dp[i][j] - (single[i] ? dp[i][j] : de[i])) : 0.f;
       }
     if (p.buckets.count > 0) {          // sums along the diagonals, then those of a bucket, each in order
       __syncthreads();
@@ -414,6 +428,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
         const int r = ty + 16 * i, l = l0 + r;
         const float2 ls = l < queries ? lb[l] : make_float2(0.f, INFINITY);
         const float de = l < queries ? db[l] : 0.f;
+        const bool single = win_single(p, l, keys);
 #pragma unroll
         for (int jj = 0; jj < TM; ++jj) {
           const int c = tx + 16 * jj, s = s0 + c;
@@ -422,7 +437,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
           const bool in = l < queries && s < keys && win_sees(p, l, s);
           const float w = in ? exp2f((u - ls.x) - ls.y) : 0.f;
           sP[r * LDP + c] = w;
-          sS[r * LDP + c] = in ? w * (dp[i][jj] - de) : 0.f;
+          sS[r * LDP + c] = in ? w * (dp[i][jj] - (single ? dp[i][jj] : de)) : 0.f;
         }
       }
       __syncthreads();
@@ -451,7 +466,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
   }
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < BM; r += kWinThreads / 32)
-    if (bad[r]) win_row_dkv<T>(p, dk, dv, dx, stats, delta, s0 + r, g, b, queries);
+    if (bad[r]) win_row_dkv<T>(p, dk, dv, dx, stats, delta, s0 + r, g, b, queries, keys);
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -511,11 +526,11 @@ template <typename K> int32_t win_smem(K kernel, int bytes) {
   return LB2_OK;
 }
 
-template <typename T> int32_t win_delta(float* delta, const T* dx, const T* x, const WinParams& p, int64_t rows, cudaStream_t st) {
+template <typename T> int32_t win_delta(float* delta, const T* dx, const T* x, const T* rest, const WinParams& p, int64_t rows, cudaStream_t st) {
   const int lanes = p.E / Vec16<T>::N;
-  const bool vec = p.E > 0 && p.E % Vec16<T>::N == 0 && lanes <= 32 && aligned_to(dx, 16) && aligned_to(x, 16);
+  const bool vec = p.E > 0 && p.E % Vec16<T>::N == 0 && lanes <= 32 && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(rest, 16);
   auto launch = [&](auto kernel, int per_row) {
-    kernel<<<(unsigned)((rows * per_row + 255) / 256), 256, 0, st>>>(delta, dx, x, p.E, p.H, p.L, rows);
+    kernel<<<(unsigned)((rows * per_row + 255) / 256), 256, 0, st>>>(delta, dx, x, rest, p.E, p.H, p.L, rows);
   };
   if (!vec) launch(win_delta_kernel<T, 0>, 32);
   else if (lanes <= 8) launch(win_delta_kernel<T, 8>, 8);
@@ -533,7 +548,7 @@ using namespace lb2;
 
 extern "C" {
 
-int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const void* k, const void* v, const void* table,
+int32_t lb2_window_attention_fwd(void* x, void* x_rest, float* stats, const void* q, const void* k, const void* v, const void* table,
                                  const lb2_rel_buckets* buckets, const int32_t* lengths, double scale, const lb2_window_dims* d,
                                  int32_t dtype, void* stream) {
   int32_t rc = win_check(d, buckets, table, lengths, dtype);
@@ -542,19 +557,20 @@ int32_t lb2_window_attention_fwd(void* x, float* stats, const void* q, const voi
   const size_t es = dtype_size(dtype);
   LB2_REQUIRE((x || d->value_dim == 0) && (q || d->head_dim == 0) && (d->keys == 0 || ((k || d->head_dim == 0) && (v || d->value_dim == 0))), LB2_BAD_ARG,
               "null tensor pointer");
-  LB2_REQUIRE(aligned_to(x, es) && aligned_to(q, es) && aligned_to(k, es) && aligned_to(v, es) && aligned_to(table, es) && aligned_to(stats, 8),
+  LB2_REQUIRE(aligned_to(x, es) && aligned_to(x_rest, es) && aligned_to(q, es) && aligned_to(k, es) && aligned_to(v, es) && aligned_to(table, es) &&
+                  aligned_to(stats, 8),
               LB2_BAD_ALIGN, "pointer not aligned to the element size");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const WinParams p = win_params(d, q, k, v, table, buckets, lengths, scale);
-  if (win_tc_serves(d, dtype) && aligned_to(x, 16) && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16))
-    return win_tc_fwd(p, x, reinterpret_cast<float2*>(stats), st);
+  if (win_tc_serves(d, dtype) && aligned_to(x, 16) && aligned_to(x_rest, 16) && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16))
+    return win_tc_fwd(p, x, x_rest, reinterpret_cast<float2*>(stats), st);
   const int tile = win_simt_tile(d);
   const int64_t tiles = win_tiles(d->queries, tile), blocks = tiles * d->heads * d->batch;
   LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
   LB2_DISPATCH_DTYPE(dtype, LB2_WIN_DISPATCH(d, {
     auto kernel = win_fwd_kernel<T, DP>;
     if ((rc = win_smem(kernel, WinTile<DP>::FWD_BYTES)) != LB2_OK) return rc;
-    kernel<<<(unsigned)blocks, kWinThreads, WinTile<DP>::FWD_BYTES, st>>>((T*)x, (float2*)stats, p, (int)tiles, win_vec(d->head_dim, q, k, es),
+    kernel<<<(unsigned)blocks, kWinThreads, WinTile<DP>::FWD_BYTES, st>>>((T*)x, (T*)x_rest, (float2*)stats, p, (int)tiles, win_vec(d->head_dim, q, k, es),
                                                                           win_vec(d->value_dim, v, nullptr, es));
   }));
   LB2_CHECK_LAUNCH("windowed attention");
@@ -568,7 +584,7 @@ size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* d, const 
   return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + (win_tc_serves(d, dtype) ? align_up(win_tc_sink_bytes(d), 256) + win_tc_row_bytes(d) : 0);
 }
 
-int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const float* stats, const void* q,
+int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const void* x_rest, const float* stats, const void* q,
                                  const void* k, const void* v, const void* table, const lb2_rel_buckets* buckets, const int32_t* lengths,
                                  double scale, const lb2_window_dims* d, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int32_t rc = win_check(d, buckets, table, lengths, dtype);
@@ -583,7 +599,7 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   LB2_REQUIRE((dq || !nq || !nd) && (dk || !nk || !nd) && (dv || !nk || !ne) && (dx || !nq || !ne) && (x || !nq || !ne) && (stats || !nq) &&
                   (q || !nq || !nd) && (k || !nk || !nd) && (v || !nk || !ne) && (dtable || buckets == nullptr),
               LB2_BAD_ARG, "null tensor pointer");
-  LB2_REQUIRE(aligned_to(dq, es) && aligned_to(dk, es) && aligned_to(dv, es) && aligned_to(dtable, es) && aligned_to(dx, es) && aligned_to(x, es) &&
+  LB2_REQUIRE(aligned_to(dq, es) && aligned_to(dk, es) && aligned_to(dv, es) && aligned_to(dtable, es) && aligned_to(dx, es) && aligned_to(x, es) && aligned_to(x_rest, es) &&
                   aligned_to(stats, 8) && aligned_to(q, es) && aligned_to(k, es) && aligned_to(v, es) && aligned_to(table, es),
               LB2_BAD_ALIGN, "pointer not aligned to the element size");
   const size_t need = lb2_window_attention_bwd_workspace_bytes(d, buckets, dtype);
@@ -600,10 +616,11 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   const int64_t qt = win_tiles(d->queries, tile), kt = win_tiles(d->keys, tile);
   LB2_REQUIRE(qt * d->heads * d->batch <= 0x7FFFFFFF && kt * d->kv_heads * d->batch <= 0x7FFFFFFF && (rows + 7) / 8 <= 0x7FFFFFFF, LB2_BAD_SHAPE,
               "too many rows");
-  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(q, 16) &&
+  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(x_rest, 16) &&
+      aligned_to(q, 16) &&
       aligned_to(k, 16) && aligned_to(v, 16)) {
     float* constants = sink_sums + align_up(win_tc_sink_bytes(d), 256) / sizeof(float);
-    rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, constants, dx, x, reinterpret_cast<const float2*>(stats), delta, st);
+    rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, constants, dx, x, x_rest, reinterpret_cast<const float2*>(stats), delta, st);
     if (rc != LB2_OK || columns == 0) return rc;
     win_dtable_kernel<<<(unsigned)((p.H * columns + 7) / 8), 256, 0, st>>>((__nv_bfloat16*)dtable, partial, p.H, columns, win_tc_partials(d) * d->batch);
     LB2_CHECK_LAUNCH("windowed attention dtable");
@@ -612,7 +629,7 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   LB2_DISPATCH_DTYPE(dtype, LB2_WIN_DISPATCH(d, {
     using C = WinTile<DP>;
     if (nq) {
-      if ((rc = win_delta(delta, (const T*)dx, (const T*)x, p, rows, st)) != LB2_OK) return rc;
+      if ((rc = win_delta(delta, (const T*)dx, (const T*)x, (const T*)x_rest, p, rows, st)) != LB2_OK) return rc;
       if ((rc = win_smem(win_dq_kernel<T, DP>, C::DQ_BYTES)) != LB2_OK) return rc;
       win_dq_kernel<T, DP><<<(unsigned)(qt * d->heads * d->batch), kWinThreads, C::DQ_BYTES, st>>>((T*)dq, partial, (const T*)dx, (const float2*)stats, delta, p, (int)qt,
                                                                                                    vecq, vecv);

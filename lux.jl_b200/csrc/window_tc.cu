@@ -28,7 +28,7 @@ template <int NB> struct WtFwd {
 
 struct WtFwdParams {
   WinParams w;
-  void* x;
+  void *x, *rest;                            // rest: x less its rounding, or null
   float2* stats;
   int items, pairs, by_head;                        // by_head: a pair is two heads of a group, else two neighbouring tiles
   int boxes_d, boxes_e, wide;
@@ -180,6 +180,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + grp * 128, tO = tmem + lanes + 256 + grp * 128;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
+    __nv_bfloat16* rest = static_cast<__nv_bfloat16*>(p.rest);
     bool ok = true, redo = false;                // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
     uint32_t made = 0;                           // steps so far
     int turn = 0;                                // of the bias tables: each use has a barrier of the group, two are enough
@@ -302,14 +303,18 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
 #pragma unroll
       for (int q = 0; q < 4 * NB; ++q) {
-        uint32_t v[8];
+        uint32_t v[8], r[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const float a = o[q * 16 + 2 * x] * inv, c = o[q * 16 + 2 * x + 1] * inv;
           if (q * 16 + 2 * x < w.E) fine = fine && isfinite(a) && isfinite(c);
           v[x] = any ? pack_bf16(a, c) : 0u;
+          r[x] = any ? pack_bf16(win_rest(a, __uint_as_float(v[x] << 16)), win_rest(c, __uint_as_float(v[x] & 0xFFFF0000u))) : 0u;
         }
-        if (in) wt_store16(xr + q * 16, v, w.E - q * 16, p.wide != 0);
+        if (in) {
+          wt_store16(xr + q * 16, v, w.E - q * 16, p.wide != 0);
+          if (rest != nullptr) wt_store16(rest + (xr - static_cast<__nv_bfloat16*>(p.x)) + q * 16, r, w.E - q * 16, p.wide != 0);
+        }
       }
       float2* st = p.stats != nullptr ? p.stats + ((int64_t)t.b * w.H + h) * w.L : nullptr;
       if (st != nullptr && in) st[l] = any ? make_float2(m2, log2f(sum)) : make_float2(0.f, INFINITY);
@@ -327,7 +332,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int e = 0; e < w.E; ++e) bad = bad || !isfinite(__bfloat162float(xr[e]));
         for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
           const int r = l - lane + __ffs(again) - 1;
-          win_row_fwd<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.x), p.stats != nullptr ? p.stats + ((int64_t)t.b * w.H + h) * w.L + r : nullptr, r, h,
+          win_row_fwd<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.x), rest, p.stats != nullptr ? p.stats + ((int64_t)t.b * w.H + h) * w.L + r : nullptr, r, h,
                                      t.b, t.keys);
         }
       }
@@ -350,14 +355,14 @@ bool win_tc_serves(const lb2_window_dims* d, int32_t dtype) {
          d->value_dim % 8 == 0 && d->keys > 0 && d->queries > 0 && tensor_map_encoder() != nullptr;
 }
 
-int32_t win_tc_fwd(const WinParams& w, void* x, float2* stats, cudaStream_t st) {
+int32_t win_tc_fwd(const WinParams& w, void* x, void* rest, float2* stats, cudaStream_t st) {
   WtFwdParams p{};
-  p.w = w; p.x = x; p.stats = stats;
+  p.w = w; p.x = x; p.rest = rest; p.stats = stats;
   const int tiles = (w.L + kWtTile - 1) / kWtTile;
   p.by_head = w.rep % 2 == 0;
   p.pairs = p.by_head ? tiles : (tiles + 1) / 2;
   p.boxes_d = (w.D + 63) / 64; p.boxes_e = (w.E + 63) / 64;
-  p.wide = aligned_to(x, 32) && w.E % 16 == 0;
+  p.wide = aligned_to(x, 32) && aligned_to(rest, 32) && w.E % 16 == 0;
   p.status = device_status_word();
   LB2_REQUIRE(p.status != nullptr, LB2_LAUNCH_FAIL, "windowed attention: device status word unavailable");
   CUtensorMap mq, mk, mv;

@@ -13,8 +13,8 @@ int64_t win_tc_partials(const lb2_window_dims* d);      // blocks that leave a p
 size_t win_tc_sink_bytes(const lb2_window_dims* d);    // scratch for the keys that all later queries see
 size_t win_tc_row_bytes(const lb2_window_dims* d);     // scratch for the rows' constants
 int32_t win_tc_bwd(const WinParams& p, void* dq, void* dk, void* dv, float* partial, float* sink_sums, float* rows, const void* dx, const void* x,
-                   const float2* stats, float* delta, cudaStream_t st);
-int32_t win_tc_fwd(const WinParams& p, void* x, float2* stats, cudaStream_t st);
+                   const void* rest, const float2* stats, float* delta, cudaStream_t st);
+int32_t win_tc_fwd(const WinParams& p, void* x, void* rest, float2* stats, cudaStream_t st);
 
 // token arrays (features, heads, tokens, batch) in boxes of 64 features x 128 tokens of one head
 inline bool wt_encode(CUtensorMap* map, const void* ptr, int64_t features, int64_t heads, int64_t tokens, int64_t batch) {

@@ -244,6 +244,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const float* of_row = p.rows + (((int64_t)t.b * w.H + h) * p.query_tiles + l0 / kWtTile) * 3 * kWtTile + row;
       const float neg_m = of_row[0], neg_l = of_row[kWtTile], neg_d = of_row[2 * kWtTile];
       const uint64_t nm = pack2(neg_m, neg_m), nl = pack2(neg_l, neg_l), nd = pack2(neg_d, neg_d);
+      const bool single = win_single(w, l, t.keys);
       float left_sum = 0.f, right_sum = 0.f;
       for (int i = 0; i < n; ++i) {
         const int s0 = t.own.at(i) * kWtTile, low = s0 - l0 - (kWtTile - 1);
@@ -251,7 +252,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         float flat = 0.f;
         const float* bias = nullptr;
         const uint8_t* bucket = nullptr;
-        const bool in_left = biased && tail.is_left(low + 2 * (kWtTile - 1));
+        const bool whole = view.whole(s0), in_left = biased && tail.is_left(low + 2 * (kWtTile - 1));
         if (biased) {
           if (in_left) {
             flat = tail.left;
@@ -300,13 +301,17 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         {
           float e[64];
           tmem_row64<0>(tDP + lanes + half * 64, e);
+          if (!whole && __any_sync(0xffffffffu, single)) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) e[j] = single ? (e[j] - e[j]) - neg_d : e[j];     // plus neg_d: nothing, unless dp is not finite
+          }
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
             const uint64_t y = mul2(add2(pack2(e[j], e[j + 1]), nd), pack2(d[j], d[j + 1]));
             unpack2(y, d[j], d[j + 1]);
           }
         }
-        if (!view.whole(s0)) {
+        if (!whole) {
           const WtSeen seen(w, l, t.queries, s0, t.keys);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
@@ -624,6 +629,17 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       {
         float e[64];
         tmem_row64<0>(tD, e);
+        if (!whole) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t single = __ballot_sync(0xffffffffu, win_single(w, l0 + half * 64 + q * 32 + lane, keys));
+            if (single != 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                e[q * 32 + j] = single >> j & 1u ? (e[q * 32 + j] - e[q * 32 + j]) - col[256 + half * 64 + q * 32 + j] : e[q * 32 + j];
+            }
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
           const float4 nd = lds4(col + 256 + half * 64 + j);
@@ -710,7 +726,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       bar_group(1, kWtSoft);
       for (int r = sw; r < kWtTile; r += 8)
         if (bad[r])
-          win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s0 + r, g, b, queries);
+          win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s0 + r, g, b, queries, keys);
     }
   }
 
@@ -725,7 +741,8 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
 // delta[batch][head][query] = dx . x and the rows' constants, LR lanes of a row taking eight features each
 template <int LR>
-__global__ void __launch_bounds__(256) win_tc_rows_kernel(const __grid_constant__ WtBwdParams p, float* __restrict__ delta, const __nv_bfloat16* __restrict__ x) {
+__global__ void __launch_bounds__(256) win_tc_rows_kernel(const __grid_constant__ WtBwdParams p, float* __restrict__ delta, const __nv_bfloat16* __restrict__ x,
+                                                          const __nv_bfloat16* __restrict__ rest) {
   const WinParams& w = p.w;
   const int lane = threadIdx.x % LR, padded = p.query_tiles * kWtTile;
   const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LR;         // (batch, query up to whole tiles, head)
@@ -737,8 +754,11 @@ __global__ void __launch_bounds__(256) win_tc_rows_kernel(const __grid_constant_
   if (in && lane * 8 < w.E) {
     const int64_t at = (((int64_t)b * w.L + l) * w.H + h) * w.E + lane * 8;
     const Vec16<__nv_bfloat16> u = load16(static_cast<const __nv_bfloat16*>(p.dx) + at), v = load16(x + at);
+    Vec16<__nv_bfloat16> r;
+    r.raw = make_uint4(0, 0, 0, 0);
+    if (rest != nullptr) r = load16(rest + at);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(u.get(i), v.get(i), s);
+    for (int i = 0; i < 8; ++i) s = fmaf(u.get(i), v.get(i) + r.get(i), s);
   }
 #pragma unroll
   for (int o = LR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -772,7 +792,7 @@ __global__ void __launch_bounds__(256) win_tc_sinks_kernel(const __grid_constant
   }
   if (s < keys && !__all_sync(0xffffffffu, fine))
     win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s, g, b,
-                               win_tokens(w, b, w.L));
+                               win_tokens(w, b, w.L), keys);
 }
 
 // The tiles of keys that hold sinks, and by how many blocks each is shared: a block walks no more tiles of queries than an ordinary one
@@ -802,7 +822,7 @@ size_t win_tc_sink_bytes(const lb2_window_dims* d) {
 int64_t win_tc_partials(const lb2_window_dims* d) { return (d->queries + kWtTile - 1) / kWtTile; }
 
 int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* partial, float* sink_sums, float* rows, const void* dx, const void* x,
-                   const float2* stats, float* delta, cudaStream_t st) {
+                   const void* rest, const float2* stats, float* delta, cudaStream_t st) {
   WtBwdParams p{};
   p.w = w; p.dq = dq; p.dk = dk; p.dv = dv; p.dx = dx; p.stats = stats; p.delta = delta; p.partial = partial; p.sink_sums = sink_sums; p.rows = rows;
   wt_sink_plan(w.L, w.S, w.window, w.sinks, w.rep, (int64_t)w.Hkv * w.B, &p.sink_tiles, &p.splits);
@@ -820,8 +840,8 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
   const int lanes = w.E <= 64 ? 8 : 16;
   const int64_t row_blocks = (qt * kWtTile * w.H * w.B * lanes + 255) / 256;
   LB2_REQUIRE(row_blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
-  if (lanes == 8) win_tc_rows_kernel<8><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x));
-  else win_tc_rows_kernel<16><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x));
+  if (lanes == 8) win_tc_rows_kernel<8><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(rest));
+  else win_tc_rows_kernel<16><<<(unsigned)row_blocks, 256, 0, st>>>(p, delta, static_cast<const __nv_bfloat16*>(x), static_cast<const __nv_bfloat16*>(rest));
   LB2_CHECK_LAUNCH("windowed attention rows");
   auto launch = [&](auto kernel, int smem, int64_t tiles, int64_t blocks) -> int32_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);

@@ -122,9 +122,9 @@ PROTOTYPES = {
     "lb2_relpos_bias_fwd": (_i32, [_p, _p, C.POINTER(RelBuckets), _i64, _i64, _i64, _i64, _i32, _p]),
     "lb2_relpos_bias_bwd_workspace_bytes": (_sz, [C.POINTER(RelBuckets), _i64, _i64, _i64, _i64]),
     "lb2_relpos_bias_bwd": (_i32, [_p, _p, C.POINTER(RelBuckets), _i64, _i64, _i64, _i64, _i64, _i32, _p, _sz, _p]),
-    "lb2_window_attention_fwd": (_i32, [_p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32, _p]),
+    "lb2_window_attention_fwd": (_i32, [_p, _p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32, _p]),
     "lb2_window_attention_bwd_workspace_bytes": (_sz, [C.POINTER(WindowDims), C.POINTER(RelBuckets), _i32]),
-    "lb2_window_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32,
+    "lb2_window_attention_bwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _fp, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32,
                                         _p, _sz, _p]),
     "lb2_window_attention_step": (_i32, [_p, _p, _p, _p, _p, _p, _p, C.POINTER(RelBuckets), _p, _dbl, C.POINTER(WindowDims), _i32, _p]),
     "lb2_window_cache_fill": (_i32, [_p, _p, _p, _p, _p, _i64, C.POINTER(WindowDims), _i32, _p]),

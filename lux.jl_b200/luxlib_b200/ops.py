@@ -998,8 +998,9 @@ def _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets
     Tb, plan = _table_of(table, buckets)
     out = jl_empty(xshape, Q.dtype, device)
     stats = torch.empty(2 * dims.queries * dims.heads * dims.batch, dtype=torch.float32, device=device) if want_stats else None
-    _launch(device, "lb2_window_attention_fwd", ptr(out), ptr(stats), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lengths), sc, C.byref(dims), dt)
-    return out, (stats, Q, Kx, V, Tb, plan, lengths, sc, dims, dt, device)
+    rest = jl_empty(xshape, Q.dtype, device) if want_stats and Q.dtype == torch.bfloat16 else None     # what rounding takes from x
+    _launch(device, "lb2_window_attention_fwd", ptr(out), ptr(rest), ptr(stats), ptr(Q), ptr(Kx), ptr(V), ptr(Tb), plan, ptr(lengths), sc, C.byref(dims), dt)
+    return out, (rest, stats, Q, Kx, V, Tb, plan, lengths, sc, dims, dt, device)
 
 
 def windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal: bool = True, scale=None, table=None, buckets=None, lengths=None):
@@ -1012,7 +1013,7 @@ def windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal: bool 
 
 def rrule_windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal: bool = True, scale=None, table=None, buckets=None, lengths=None):
     """Forward + pullback Δ -> (∂q, ∂k, ∂v, ∂table); ∂table is None without a table."""
-    x, (stats, Q, Kx, V, Tb, plan, lens, sc, dims, dt, device) = _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets,
+    x, (rest, stats, Q, Kx, V, Tb, plan, lens, sc, dims, dt, device) = _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets,
                                                                                    lengths, True)
 
     def pullback(dx):
@@ -1023,7 +1024,7 @@ def rrule_windowed_attention(q, k, v, *, window: int, sinks: int = 0, is_causal:
         dq, dk, dv = (jl_empty(tuple(t.shape), Q.dtype, device) for t in (Q, Kx, V))
         dtable = jl_empty(tuple(Tb.shape), Q.dtype, device) if Tb is not None else None
         _, wsp, wsn = _ws(_cabi.load().lb2_window_attention_bwd_workspace_bytes(C.byref(dims), plan, dt), device)
-        _launch(device, "lb2_window_attention_bwd", ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(G), ptr(x), ptr(stats), ptr(Q), ptr(Kx), ptr(V),
+        _launch(device, "lb2_window_attention_bwd", ptr(dq), ptr(dk), ptr(dv), ptr(dtable), ptr(G), ptr(x), ptr(rest), ptr(stats), ptr(Q), ptr(Kx), ptr(V),
                 ptr(Tb), plan, ptr(lens), sc, C.byref(dims), dt, wsp, wsn)
         return dq, dk, dv, dtable
 

@@ -5,7 +5,8 @@ Tolerances, per element and relative to the same sum over absolute values (its m
   logit, of the row's log-sum and of the exponential: 2 (D + 4) u Z + 16 u; a sum over n terms adds n u, the products dx . v and dx . x
   E u each. Together u (2 (D + 4) (Z + 1) + 2 E + n + 32).
   BFloat16: those of Float32 arithmetic (the exponential to 2^-20 instead), and 2^-8 for each rounding to bf16 on the way: the weights
-  and the result (x, dv); the weights of the logits' gradient, x in dx . x and the result (dq, dk, dtable)."""
+  and the result (x, dv); the logits' gradient and the result (dq, dk); the result alone (dtable). The x of dx . x comes in two
+  parts, which leave 2^-16 of it."""
 import ctypes as C
 import math
 
@@ -37,7 +38,7 @@ def host(t):
 def bound(dt, name, mag, zmax, D, E, n):
     rel = U32 * (2 * (D + 4) * (zmax + 1) + 2 * E + n + 32)
     if dt == "bf16":
-        rel += 2.0 ** -20 + U16 * (2 if name in ("x", "dv") else 3)
+        rel += 2.0 ** -20 + 2.0 ** -16 + U16 * (1 if name == "dtable" else 2)
     return rel * mag + 1e-35
 
 
@@ -141,6 +142,22 @@ def test_what_a_query_does_not_see_does_not_reach_it(dt, D, value):
     a["v"][2, 1, 90, 0] = value
     a["dx"][0, 1, 100, 0] = value
     run_case(dt, D, D, 2, 2, 200, 200, 2, 9, 0, True, lengths=[200, 150], a=a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128, 33])
+def test_queries_that_see_one_key_alone_have_no_gradient_in_their_logits(dt, D):
+    """Their weight is 1 whatever the logit: exactly zero, not the difference of two sums."""
+    a = make(18, dt, D, D, 4, 2, 150, 150, 2, len(B6))
+    t = {n: dev(x, dt) for n, x in a.items()}
+    x, pb = L.rrule_windowed_attention(t["q"], t["k"], t["v"], window=1, table=t["table"], buckets=B6)
+    dq, dk, dv, dtable = pb(t["dx"])
+    assert np.array_equal(host(x), np.repeat(a["v"], 2, 1))
+    assert not host(dq).any() and not host(dk).any() and not host(dtable).any()
+    x, pb = L.rrule_windowed_attention(t["q"], t["k"][:, :, :1], t["v"][:, :, :1], window=5, sinks=1, table=t["table"], buckets=B6)
+    dq, dk, dv, dtable = pb(t["dx"])
+    assert not host(dq).any() and not host(dk).any() and not host(dtable).any()
 
 
 @pytest.mark.gpu
@@ -528,7 +545,7 @@ def test_status_codes_of_the_windowed_entry_points():
     lib = _cabi.load()
     one = 256
     fwd = lambda dims, dt=0, x=one, table=None, buckets=None, lens=None, q=one: lib.lb2_window_attention_fwd(
-        x, None, q, one, one, table, buckets, lens, 0.125, dims, dt, None)
+        x, None, None, q, one, one, table, buckets, lens, 0.125, dims, dt, None)
     assert fwd(None) == _cabi.BAD_ARG
     assert fwd(_dims(), dt=5) == _cabi.UNSUPPORTED_DTYPE
     assert fwd(_dims(window=0)) == _cabi.BAD_ARG and fwd(_dims(sinks=-1)) == _cabi.BAD_ARG
@@ -541,7 +558,7 @@ def test_status_codes_of_the_windowed_entry_points():
     assert fwd(_dims(batch=0)) == _cabi.OK and fwd(_dims(queries=0)) == _cabi.OK and fwd(_dims(heads=0, kv_heads=0)) == _cabi.OK
 
     bwd = lambda dims, ws=one, n=1 << 20, dq=one, dtable=None, table=None, buckets=None: lib.lb2_window_attention_bwd(
-        dq, one, one, dtable, one, one, one, one, one, one, table, buckets, None, 0.125, dims, 0, ws, n, None)
+        dq, one, one, dtable, one, one, None, one, one, one, one, table, buckets, None, 0.125, dims, 0, ws, n, None)
     need = lib.lb2_window_attention_bwd_workspace_bytes(_dims(), None, 0)
     assert need >= 40 * 4
     assert bwd(_dims(), n=need - 1) == _cabi.WORKSPACE_TOO_SMALL and bwd(_dims(), ws=None, n=0) == _cabi.WORKSPACE_TOO_SMALL
