@@ -5,6 +5,8 @@
 //   l < n, s < n,  s <= l if causal,  |l - s| < window or s < sinks.
 // z[s, l] = scale * k_s . q_l + table[h, bucket(s - l)],  p = softmax of z over the visible s (nothing visible: all zero).
 #pragma once
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace lb2 {
@@ -81,6 +83,35 @@ template <typename T> __device__ __forceinline__ float win_bias(const WinParams&
 template <typename T> __device__ __forceinline__ float win_bias(const WinParams& p, const int32_t* first, int h, int rel) {
   return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, first, rel)]));
 }
+
+// The tiles of keys that hold sinks, and by how many blocks each is shared in dk, dv: a block walks no more tiles of queries than an
+// ordinary one or, if that is more, half an SM's share of the whole.
+struct WinSinkPlan { int tiles, splits; };
+inline WinSinkPlan win_sink_plan(int tile, int64_t queries, int64_t keys, int64_t window, int64_t sinks, int64_t rep, int64_t groups) {
+  auto tiles = [&](int64_t n) { return (n + tile - 1) / tile; };
+  const int64_t nsink = tiles(std::min(sinks, keys)), usual = std::min(tiles(queries), tiles(window) + 1) * rep;
+  const int64_t all = groups * ((tiles(keys) - nsink) * usual + nsink * tiles(queries) * rep), share = std::max(usual, all / (2 * sm_count()) + 1);
+  const int64_t n = nsink > 0 ? std::min<int64_t>(8, (tiles(queries) * rep + share - 1) / share) : 1;
+  return {n > 1 ? (int)nsink : 0, (int)n};
+}
+// What the blocks of dk, dv share: block -> tile of keys, key head and sample, and its part of a shared tile. Shared tiles, the longest, first.
+struct WinKeyTile {
+  int tile, gb, split, splits;
+  __device__ __forceinline__ WinKeyTile(int block, int tiles, int groups, const WinSinkPlan& plan) {
+    const int shared = plan.tiles * plan.splits * groups;
+    split = 0; splits = 1;
+    if (block < shared) {
+      gb = block % groups;
+      split = block / groups % plan.splits; splits = plan.splits;
+      tile = block / groups / plan.splits;
+    } else {
+      tile = plan.tiles + (block - shared) / groups; gb = (block - shared) % groups;
+    }
+  }
+};
+// dk, dv of the shared tiles from their blocks' sums [split][tile][group][rows of a tile][D + E]
+int32_t win_sinks_join(const WinParams& p, const WinSinkPlan& plan, int tile, void* dk, void* dv, const float* sums, const void* dx, const float2* stats,
+                       const float* delta, int32_t dtype, cudaStream_t st);
 
 // ---- rows once more ---------------------------------------------------------------------------
 // A tile's products multiply the weights that the mask made zero with whatever the array holds there: an infinity or NaN in a

@@ -18,11 +18,23 @@ namespace {
 
 constexpr int kWinThreads = 256;      // 16 x 16, each TM x TN of a tile of logits
 
-// rows [row0, row0 + ROWS) of n features, `stride` elements apart, as fp32 into rows of LD floats; zeros past `rows` and past n
+// rows [row0, row0 + ROWS) of n features, `stride` elements apart, as fp32 into rows of LD floats; zeros past `rows` and past n.
+// Whole Float32 vectors are copied asynchronously: win_loaded() before the barrier that hands them on.
+__device__ __forceinline__ void win_loaded() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <typename T, int ROWS, int LD>
 __device__ __forceinline__ void win_load_tile(float* dst, const T* src, int64_t stride, int row0, int rows, int n, int n4, bool vec) {
   if (vec) {                          // rows are whole vectors of four
     const int quads = n4 >> 2;
+    if constexpr (sizeof(T) == 4) {
+      for (int i = threadIdx.x; i < ROWS * quads; i += kWinThreads) {
+        const int r = i / quads, c = (i - r * quads) * 4;
+        const bool in = row0 + r < rows;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * LD + c)),
+                     "l"(src + (int64_t)(in ? row0 + r : 0) * stride + c), "r"(in ? 16 : 0)
+                     : "memory");
+      }
+      return;
+    }
     for (int i = threadIdx.x; i < ROWS * quads; i += kWinThreads) {
       const int r = i / quads, c = (i - r * quads) * 4;
       float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -188,6 +200,7 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
     win_load_tile<T, BM, LD>(sK, kb, (int64_t)p.Hkv * p.D, s0, keys, p.D, D4, vecq);
     win_load_tile<T, BM, LD>(sV, vb, (int64_t)p.Hkv * p.E, s0, keys, p.E, E4, vecv);
     if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, nullptr, p, h, l0, s0);
+    win_loaded();
     __syncthreads();
     float z[TM][TM] = {};
     win_dots<LD>(z, sQ, sK, D4, ty, tx);
@@ -321,6 +334,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq,
     win_load_tile<T, BM, LD>(sK, kb, (int64_t)p.Hkv * p.D, s0, keys, p.D, D4, vecq);
     win_load_tile<T, BM, LD>(sV, vb, (int64_t)p.Hkv * p.E, s0, keys, p.E, E4, vecv);
     if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, sB, p, h, l0, s0);
+    win_loaded();
     __syncthreads();
     float z[TM][TM] = {}, dp[TM][TM] = {};
     win_dots<LD>(z, sQ, sK, D4, ty, tx);
@@ -389,13 +403,16 @@ __global__ void __launch_bounds__(256) win_dtable_kernel(T* __restrict__ dtable,
 template <typename T, int DP>
 __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk, T* __restrict__ dv, const T* __restrict__ dx,
                                                               const float2* __restrict__ stats, const float* __restrict__ delta,
-                                                              const __grid_constant__ WinParams p, int tiles, int vecq, int vecv) {
+                                                              float* __restrict__ sums, const __grid_constant__ WinParams p, WinSinkPlan plan,
+                                                              int tiles, int vecq, int vecv) {
   using C = WinTile<DP>;
   constexpr int BM = C::BM, TM = C::TM, LD = C::LD, LDP = C::LDP, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
   float *sQ = sm, *sG = sQ + C::TILE, *sK = sG + C::TILE, *sV = sK + C::TILE, *sP = sV + C::TILE, *sS = sP + C::PTILE, *sD = sS + C::PTILE;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int tile = blockIdx.x % tiles, gb = blockIdx.x / tiles, g = gb % p.Hkv, b = gb / p.Hkv;
+  const int groups = p.Hkv * p.B;
+  const WinKeyTile mine(blockIdx.x, tiles, groups, plan);
+  const int tile = mine.tile, gb = mine.gb, g = gb % p.Hkv, b = gb / p.Hkv;
   const int s0 = tile * BM, queries = win_tokens(p, b, p.L), keys = win_tokens(p, b, p.S);
   const int D4 = (p.D + 3) & ~3, E4 = (p.E + 3) & ~3;
   win_load_tile<T, BM, LD>(sK, win_kv_row<T>(p, p.k, p.D, 0, g, b), (int64_t)p.Hkv * p.D, s0, keys, p.D, D4, vecq);
@@ -410,40 +427,51 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
   int lo, hi;
   win_query_range(p, s0, min(s0 + BM, keys), queries, &lo, &hi);
   if (s0 >= keys) hi = 0;
-  for (int j = 0; j < p.rep; ++j) {
-    const int h = g * p.rep + j;
+  const int per_head = lo < hi ? (hi + BM - 1) / BM - lo / BM : 0, count = per_head * p.rep;
+  for (int it = (int)((int64_t)count * mine.split / mine.splits), end = (int)((int64_t)count * (mine.split + 1) / mine.splits); it < end; ++it) {
+    const int h = g * p.rep + it / per_head, l0 = (lo / BM + it % per_head) * BM;
     const float2* lb = stats + ((int64_t)b * p.H + h) * p.L;
     const float* db = delta + ((int64_t)b * p.H + h) * p.L;
-    for (int l0 = lo / BM * BM; l0 < hi; l0 += BM) {
-      __syncthreads();
-      win_load_tile<T, BM, LD>(sQ, win_q_row<T>(p, p.q, p.D, 0, h, b), (int64_t)p.H * p.D, l0, queries, p.D, D4, vecq);
-      win_load_tile<T, BM, LD>(sG, win_q_row<T>(p, dx, p.E, 0, h, b), (int64_t)p.H * p.E, l0, queries, p.E, E4, vecv);
-      if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, nullptr, p, h, l0, s0);
-      __syncthreads();
-      float z[TM][TM] = {}, dp[TM][TM] = {};
-      win_dots<LD>(z, sQ, sK, D4, ty, tx);
-      win_dots<LD>(dp, sG, sV, E4, ty, tx);
+    __syncthreads();
+    win_load_tile<T, BM, LD>(sQ, win_q_row<T>(p, p.q, p.D, 0, h, b), (int64_t)p.H * p.D, l0, queries, p.D, D4, vecq);
+    win_load_tile<T, BM, LD>(sG, win_q_row<T>(p, dx, p.E, 0, h, b), (int64_t)p.H * p.E, l0, queries, p.E, E4, vecv);
+    if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, nullptr, p, h, l0, s0);
+    win_loaded();
+    __syncthreads();
+    float z[TM][TM] = {}, dp[TM][TM] = {};
+    win_dots<LD>(z, sQ, sK, D4, ty, tx);
+    win_dots<LD>(dp, sG, sV, E4, ty, tx);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int r = ty + 16 * i, l = l0 + r;
-        const float2 ls = l < queries ? lb[l] : make_float2(0.f, INFINITY);
-        const float de = l < queries ? db[l] : 0.f;
-        const bool single = win_single(p, l, keys);
+    for (int i = 0; i < TM; ++i) {
+      const int r = ty + 16 * i, l = l0 + r;
+      const float2 ls = l < queries ? lb[l] : make_float2(0.f, INFINITY);
+      const float de = l < queries ? db[l] : 0.f;
+      const bool single = win_single(p, l, keys);
 #pragma unroll
-        for (int jj = 0; jj < TM; ++jj) {
-          const int c = tx + 16 * jj, s = s0 + c;
-          float u = z[i][jj] * p.scale2;
-          if (p.buckets.count > 0) u += sD[r - c + BM - 1];
-          const bool in = l < queries && s < keys && win_sees(p, l, s);
-          const float w = in ? exp2f((u - ls.x) - ls.y) : 0.f;
-          sP[r * LDP + c] = w;
-          sS[r * LDP + c] = in ? w * (dp[i][jj] - (single ? dp[i][jj] : de)) : 0.f;
-        }
+      for (int jj = 0; jj < TM; ++jj) {
+        const int c = tx + 16 * jj, s = s0 + c;
+        float u = z[i][jj] * p.scale2;
+        if (p.buckets.count > 0) u += sD[r - c + BM - 1];
+        const bool in = l < queries && s < keys && win_sees(p, l, s);
+        const float w = in ? exp2f((u - ls.x) - ls.y) : 0.f;
+        sP[r * LDP + c] = w;
+        sS[r * LDP + c] = in ? w * (dp[i][jj] - (single ? dp[i][jj] : de)) : 0.f;
       }
-      __syncthreads();
-      win_cols<LDP, LD, BM>(ov4, sP, sG, ty, tx);
-      win_cols<LDP, LD, BM>(ok4, sS, sQ, ty, tx);
     }
+    __syncthreads();
+    win_cols<LDP, LD, BM>(ov4, sP, sG, ty, tx);
+    win_cols<LDP, LD, BM>(ok4, sS, sQ, ty, tx);
+  }
+  if (mine.splits > 1) {
+    float* out = sums + (((int64_t)mine.split * plan.tiles + tile) * groups + gb) * BM * (p.D + p.E);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        win_put4(out + (TM * ty + i) * (p.D + p.E), 4 * tx + 64 * c, p.D, ok4[i][c], p.scale);
+        win_put4(out + (TM * ty + i) * (p.D + p.E) + p.D, 4 * tx + 64 * c, p.E, ov4[i][c], 1.f);
+      }
+    return;
   }
   T* dkb = dk + ((int64_t)b * p.S * p.Hkv + g) * p.D;
   T* dvb = dv + ((int64_t)b * p.S * p.Hkv + g) * p.E;
@@ -467,6 +495,29 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < BM; r += kWinThreads / 32)
     if (bad[r]) win_row_dkv<T>(p, dk, dv, dx, stats, delta, s0 + r, g, b, queries, keys);
+}
+
+// the sums of a shared tile's blocks in order, a warp per key and head
+template <typename T>
+__global__ void __launch_bounds__(256) win_sinks_kernel(T* __restrict__ dk, T* __restrict__ dv, const float* __restrict__ sums, const T* __restrict__ dx,
+                                                        const float2* __restrict__ stats, const float* __restrict__ delta,
+                                                        const __grid_constant__ WinParams p, WinSinkPlan plan, int tile) {
+  const int lane = threadIdx.x & 31, groups = p.Hkv * p.B, width = p.D + p.E;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), all = (int64_t)plan.tiles * groups * tile;
+  if (row >= all) return;
+  const int r = (int)(row % tile), gb = (int)(row / tile % groups), g = gb % p.Hkv, b = gb / p.Hkv, s = (int)(row / tile / groups) * tile + r;
+  if (s >= p.S) return;
+  const int keys = win_tokens(p, b, p.S);
+  T* dkr = dk + (((int64_t)b * p.S + s) * p.Hkv + g) * p.D;
+  T* dvr = dv + (((int64_t)b * p.S + s) * p.Hkv + g) * p.E;
+  bool fine = true;
+  for (int c = lane; c < width; c += 32) {
+    float t = 0.f;
+    for (int i = 0; i < plan.splits; ++i) t += sums[(i * all + row) * width + c];
+    fine = fine && isfinite(t);
+    (c < p.D ? dkr[c] : dvr[c - p.D]) = from_f32<T>(s < keys ? t : 0.f);
+  }
+  if (s < keys && !__all_sync(0xffffffffu, fine)) win_row_dkv<T>(p, dk, dv, dx, stats, delta, s, g, b, win_tokens(p, b, p.L), keys);
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -540,7 +591,29 @@ template <typename T> int32_t win_delta(float* delta, const T* dx, const T* x, c
   return LB2_OK;
 }
 
+WinSinkPlan win_plan(const lb2_window_dims* d, int tile) {
+  return win_sink_plan(tile, d->queries, d->keys, std::min(d->window, d->queries + d->keys + 1), d->sinks, d->heads / d->kv_heads, d->kv_heads * d->batch);
+}
+// scratch of the tiles whose keys all later queries see
+size_t win_sink_bytes(const lb2_window_dims* d, int32_t dtype) {
+  auto bytes = [&](int tile) {
+    const WinSinkPlan n = win_plan(d, tile);
+    return (size_t)n.tiles * n.splits * (size_t)(d->batch * d->kv_heads * tile * (d->head_dim + d->value_dim)) * sizeof(float);
+  };
+  return align_up(std::max(bytes(win_simt_tile(d)), win_tc_serves(d, dtype) ? bytes(kWtTile) : 0), 256);
+}
+
 }  // namespace
+
+int32_t win_sinks_join(const WinParams& p, const WinSinkPlan& plan, int tile, void* dk, void* dv, const float* sums, const void* dx, const float2* stats,
+                       const float* delta, int32_t dtype, cudaStream_t st) {
+  const int64_t rows = (int64_t)plan.tiles * p.Hkv * p.B * tile;
+  LB2_DISPATCH_DTYPE(dtype, {
+    win_sinks_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>((T*)dk, (T*)dv, sums, (const T*)dx, stats, delta, p, plan, tile);
+  });
+  LB2_CHECK_LAUNCH("windowed attention dk, dv of the sinks");
+  return LB2_OK;
+}
 
 }  // namespace lb2
 
@@ -581,7 +654,7 @@ size_t lb2_window_attention_bwd_workspace_bytes(const lb2_window_dims* d, const 
   if (d == nullptr || !valid_dtype(dtype) || d->queries <= 0 || d->heads <= 0 || d->batch <= 0) return 0;
   if (d->kv_heads <= 0 || d->heads % d->kv_heads != 0) return 0;
   const size_t rows = (size_t)(d->queries * d->heads * d->batch);
-  return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + (win_tc_serves(d, dtype) ? align_up(win_tc_sink_bytes(d), 256) + win_tc_row_bytes(d) : 0);
+  return align_up(rows * sizeof(float), 256) + win_partial_bytes(d, buckets) + win_sink_bytes(d, dtype) + (win_tc_serves(d, dtype) ? win_tc_row_bytes(d) : 0);
 }
 
 int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, const void* dx, const void* x, const void* x_rest, const float* stats, const void* q,
@@ -619,7 +692,7 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(x_rest, 16) &&
       aligned_to(q, 16) &&
       aligned_to(k, 16) && aligned_to(v, 16)) {
-    float* constants = sink_sums + align_up(win_tc_sink_bytes(d), 256) / sizeof(float);
+    float* constants = sink_sums + win_sink_bytes(d, dtype) / sizeof(float);
     rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, constants, dx, x, x_rest, reinterpret_cast<const float2*>(stats), delta, st);
     if (rc != LB2_OK || columns == 0) return rc;
     win_dtable_kernel<<<(unsigned)((p.H * columns + 7) / 8), 256, 0, st>>>((__nv_bfloat16*)dtable, partial, p.H, columns, win_tc_partials(d) * d->batch);
@@ -641,9 +714,13 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
     }
     if (nk) {
       if ((rc = win_smem(win_dkv_kernel<T, DP>, C::DKV_BYTES)) != LB2_OK) return rc;
-      win_dkv_kernel<T, DP><<<(unsigned)(kt * d->kv_heads * d->batch), kWinThreads, C::DKV_BYTES, st>>>((T*)dk, (T*)dv, (const T*)dx, (const float2*)stats, delta, p, (int)kt,
-                                                                                                        vecq, vecv);
+      const WinSinkPlan plan = win_plan(d, tile);
+      const int64_t blocks = (kt - plan.tiles + (int64_t)plan.tiles * plan.splits) * d->kv_heads * d->batch;
+      LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
+      win_dkv_kernel<T, DP><<<(unsigned)blocks, kWinThreads, C::DKV_BYTES, st>>>((T*)dk, (T*)dv, (const T*)dx, (const float2*)stats, delta, sink_sums, p, plan,
+                                                                                (int)kt, vecq, vecv);
       LB2_CHECK_LAUNCH("windowed attention dk, dv");
+      if (plan.tiles > 0 && (rc = win_sinks_join(p, plan, tile, dk, dv, sink_sums, dx, (const float2*)stats, delta, dtype, st)) != LB2_OK) return rc;
     }
   }));
   return LB2_OK;

@@ -10,7 +10,6 @@ constexpr int kWtBox = kWtTile * 128;        // bytes of a TMA box: 128 tokens x
 // what the tensor-core kernels serve: rows of whole 16-byte vectors for TMA, at most two boxes of features
 bool win_tc_serves(const lb2_window_dims* d, int32_t dtype);
 int64_t win_tc_partials(const lb2_window_dims* d);      // blocks that leave a partial sum of dtable per head and sample
-size_t win_tc_sink_bytes(const lb2_window_dims* d);    // scratch for the keys that all later queries see
 size_t win_tc_row_bytes(const lb2_window_dims* d);     // scratch for the rows' constants
 int32_t win_tc_bwd(const WinParams& p, void* dq, void* dk, void* dv, float* partial, float* sink_sums, float* rows, const void* dx, const void* x,
                    const void* rest, const float2* stats, float* delta, cudaStream_t st);

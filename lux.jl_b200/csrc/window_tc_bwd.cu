@@ -32,7 +32,7 @@ struct WtBwdParams {
   float* partial;
   float* sink_sums;                          // [split][tile][batch][kv head][128][D + E], fp32
   int tiles, query_tiles, items, columns, boxes_d, boxes_e, wide_d;
-  int sink_tiles, splits;                    // dk, dv: the first tiles, whose keys all later queries see, are shared by `splits` blocks
+  WinSinkPlan sinks;
   unsigned int* status;
 };
 
@@ -434,17 +434,9 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t sK = base, sV = base + C::TILE, sQG = base + 2 * C::TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinParams& w = p.w;
-  // the shared tiles' blocks come first: they are the longest
-  const int shared = p.sink_tiles * p.splits, per = p.tiles - p.sink_tiles, groups = w.Hkv * w.B;
-  int tile, gb, split = 0, splits = 1;
-  if ((int)blockIdx.x < shared * groups) {
-    gb = blockIdx.x % groups;
-    split = blockIdx.x / groups % p.splits; splits = p.splits;
-    tile = blockIdx.x / groups / p.splits;
-  } else {
-    const int r = blockIdx.x - shared * groups;
-    tile = p.sink_tiles + r % per; gb = r / per;
-  }
+  const int groups = w.Hkv * w.B;
+  const WinKeyTile mine(blockIdx.x, p.tiles, groups, p.sinks);
+  const int tile = mine.tile, gb = mine.gb, split = mine.split, splits = mine.splits;
   const int g = gb % w.Hkv, b = gb / w.Hkv, s0 = tile * kWtTile;
   const int queries = warp_uniform(win_tokens(w, b, w.L)), keys = warp_uniform(win_tokens(w, b, w.S));
   int lo, hi;
@@ -671,7 +663,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (n > 0) ok = ok && mbar_wait_warp(o_full, 0, p.status, 0x4000u);
     if (splits > 1) {
       tc_fence_after();
-      float* out = p.sink_sums + ((((int64_t)split * p.sink_tiles + tile) * groups + gb) * kWtTile + row) * (w.D + w.E);
+      float* out = p.sink_sums + ((((int64_t)split * p.sinks.tiles + tile) * groups + gb) * kWtTile + row) * (w.D + w.E);
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const int width = which == 0 ? w.D : w.E;
@@ -771,52 +763,10 @@ __global__ void __launch_bounds__(256) win_tc_rows_kernel(const __grid_constant_
   if (in) delta[hb * w.L + l] = s;
 }
 
-// dk, dv of the shared tiles: the sums of their blocks in order, a warp per key and head
-__global__ void __launch_bounds__(256) win_tc_sinks_kernel(const __grid_constant__ WtBwdParams p) {
-  const WinParams& w = p.w;
-  const int lane = threadIdx.x & 31, groups = w.Hkv * w.B, width = w.D + w.E;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), stride = (int64_t)p.sink_tiles * groups * kWtTile * width;
-  if (row >= (int64_t)p.sink_tiles * groups * kWtTile) return;
-  const int r = (int)(row % kWtTile), gb = (int)(row / kWtTile % groups), g = gb % w.Hkv, b = gb / w.Hkv, s = (int)(row / kWtTile / groups) * kWtTile + r;
-  if (s >= w.S) return;
-  const int keys = win_tokens(w, b, w.S);
-  const float* in = p.sink_sums + row * width;
-  __nv_bfloat16* dk = static_cast<__nv_bfloat16*>(p.dk) + (((int64_t)b * w.S + s) * w.Hkv + g) * w.D;
-  __nv_bfloat16* dv = static_cast<__nv_bfloat16*>(p.dv) + (((int64_t)b * w.S + s) * w.Hkv + g) * w.E;
-  bool fine = true;
-  for (int c = lane; c < width; c += 32) {
-    float t = 0.f;
-    for (int i = 0; i < p.splits; ++i) t += in[i * stride + c];
-    fine = fine && isfinite(t);
-    (c < w.D ? dk[c] : dv[c - w.D]) = __float2bfloat16_rn(s < keys ? t : 0.f);
-  }
-  if (s < keys && !__all_sync(0xffffffffu, fine))
-    win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s, g, b,
-                               win_tokens(w, b, w.L), keys);
-}
-
-// The tiles of keys that hold sinks, and by how many blocks each is shared: a block walks no more tiles of queries than an ordinary one
-// or, if that is more, half an SM's share of the whole; 8192 tokens, 32 heads on 8, window 1024, 4 sinks: 4 blocks,
-// 995 us without them, 450 with.
-void wt_sink_plan(int64_t queries, int64_t keys, int64_t window, int64_t sinks, int64_t rep, int64_t groups, int* sink_tiles, int* splits) {
-  const int64_t qt = (queries + kWtTile - 1) / kWtTile, kt = (keys + kWtTile - 1) / kWtTile;
-  const int64_t nsink = (std::min(sinks, keys) + kWtTile - 1) / kWtTile, usual = std::min(qt, (window + kWtTile - 1) / kWtTile + 1) * rep;
-  const int64_t all = groups * ((kt - nsink) * usual + nsink * qt * rep), share = std::max(usual, all / (2 * sm_count()) + 1);
-  const int64_t n = nsink > 0 ? std::min<int64_t>(8, (qt * rep + share - 1) / share) : 1;
-  *sink_tiles = n > 1 ? (int)nsink : 0;
-  *splits = (int)n;
-}
-
 }  // namespace
 
 size_t win_tc_row_bytes(const lb2_window_dims* d) {
   return (size_t)((d->queries + kWtTile - 1) / kWtTile * d->heads * d->batch) * kWtRowBytes;
-}
-
-size_t win_tc_sink_bytes(const lb2_window_dims* d) {
-  int tiles, splits;
-  wt_sink_plan(d->queries, d->keys, std::min(d->window, d->queries + d->keys + 1), d->sinks, d->heads / d->kv_heads, d->kv_heads * d->batch, &tiles, &splits);
-  return (size_t)tiles * splits * (size_t)(d->batch * d->kv_heads * kWtTile * (d->head_dim + d->value_dim)) * sizeof(float);
 }
 
 int64_t win_tc_partials(const lb2_window_dims* d) { return (d->queries + kWtTile - 1) / kWtTile; }
@@ -825,7 +775,7 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
                    const void* rest, const float2* stats, float* delta, cudaStream_t st) {
   WtBwdParams p{};
   p.w = w; p.dq = dq; p.dk = dk; p.dv = dv; p.dx = dx; p.stats = stats; p.delta = delta; p.partial = partial; p.sink_sums = sink_sums; p.rows = rows;
-  wt_sink_plan(w.L, w.S, w.window, w.sinks, w.rep, (int64_t)w.Hkv * w.B, &p.sink_tiles, &p.splits);
+  p.sinks = win_sink_plan(kWtTile, w.L, w.S, w.window, w.sinks, w.rep, (int64_t)w.Hkv * w.B);
   p.columns = w.buckets.count * (w.buckets.bidirectional ? 2 : 1);
   p.boxes_d = (w.D + 63) / 64; p.boxes_e = (w.E + 63) / 64;
   p.status = device_status_word();
@@ -858,13 +808,11 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
   const int64_t resident = std::min(p.items, sm_count());
   int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, resident);
   if (rc != LB2_OK) return rc;
-  const int64_t groups = (int64_t)w.Hkv * w.B, blocks = (kt - p.sink_tiles + (int64_t)p.sink_tiles * p.splits) * groups;
+  const int64_t groups = (int64_t)w.Hkv * w.B, blocks = (kt - p.sinks.tiles + (int64_t)p.sinks.tiles * p.sinks.splits) * groups;
   LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
   rc = one ? launch(win_tc_dkv_kernel<1>, WtBwd<1>::SMEM, kt, blocks) : launch(win_tc_dkv_kernel<2>, WtBwd<2>::SMEM, kt, blocks);
-  if (rc != LB2_OK || p.sink_tiles == 0) return rc;
-  win_tc_sinks_kernel<<<(unsigned)(p.sink_tiles * groups * (kWtTile / 8)), 256, 0, st>>>(p);
-  LB2_CHECK_LAUNCH("windowed attention dk, dv of the sinks");
-  return LB2_OK;
+  if (rc != LB2_OK || p.sinks.tiles == 0) return rc;
+  return win_sinks_join(w, p.sinks, kWtTile, dk, dv, sink_sums, dx, stats, delta, LB2_BF16, st);
 }
 
 }  // namespace lb2
