@@ -58,29 +58,36 @@ __device__ __forceinline__ void win_load_tile(float* dst, const T* src, int64_t 
   }
 }
 
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-
-// acc[i][j] += A[ty + 16 i] . B[tx + 16 j] over n4 features
+// acc[i][j] = A[ty + 16 i] . B[tx + 16 j] over n4 features: even and odd ones side by side in one instruction, added at the end
 template <int LD, int TM, int TN>
 __device__ __forceinline__ void win_dots(float (&acc)[TM][TN], const float* A, const float* B, int n4, int ty, int tx) {
+  uint64_t two[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) two[i][j] = 0;
 #pragma unroll 2
   for (int d = 0; d < n4; d += 4) {
-    float4 a[TM], b[TN];
+    ulonglong2 a[TM], b[TN];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) a[i] = ld4(A + (ty + 16 * i) * LD + d);
+    for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(A + (ty + 16 * i) * LD + d);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) b[j] = ld4(B + (tx + 16 * j) * LD + d);
+    for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(B + (tx + 16 * j) * LD + d);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        acc[i][j] = fmaf(a[i].x, b[j].x, acc[i][j]);
-        acc[i][j] = fmaf(a[i].y, b[j].y, acc[i][j]);
-        acc[i][j] = fmaf(a[i].z, b[j].z, acc[i][j]);
-        acc[i][j] = fmaf(a[i].w, b[j].w, acc[i][j]);
-      }
+      for (int j = 0; j < TN; ++j) two[i][j] = fma2(a[i].y, b[j].y, fma2(a[i].x, b[j].x, two[i][j]));
   }
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      float even, odd;
+      unpack2(two[i][j], even, odd);
+      acc[i][j] = even + odd;
+    }
 }
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ void axpy4(float4& o, float w, const float4& v) {
   o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
 }
@@ -202,7 +209,7 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(T* __restrict__ x,
     if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, nullptr, p, h, l0, s0);
     win_loaded();
     __syncthreads();
-    float z[TM][TM] = {};
+    float z[TM][TM];
     win_dots<LD>(z, sQ, sK, D4, ty, tx);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -291,7 +298,7 @@ __global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delt
 
 // dq, and partial[tile][batch][head][bucket] of dtable
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq, float* __restrict__ partial, const T* __restrict__ dx,
+__global__ void __launch_bounds__(kWinThreads, DP == 64 ? 2 : 1) win_dq_kernel(T* __restrict__ dq, float* __restrict__ partial, const T* __restrict__ dx,
                                                              const float2* __restrict__ stats, const float* __restrict__ delta,
                                                              const __grid_constant__ WinParams p, int tiles, int vecq, int vecv) {
   using C = WinTile<DP>;
@@ -336,7 +343,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(T* __restrict__ dq,
     if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, sB, p, h, l0, s0);
     win_loaded();
     __syncthreads();
-    float z[TM][TM] = {}, dp[TM][TM] = {};
+    float z[TM][TM], dp[TM][TM];
     win_dots<LD>(z, sQ, sK, D4, ty, tx);
     win_dots<LD>(dp, sG, sV, E4, ty, tx);
 #pragma unroll
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(256) win_dtable_kernel(T* __restrict__ dtable,
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk, T* __restrict__ dv, const T* __restrict__ dx,
+__global__ void __launch_bounds__(kWinThreads, DP == 64 ? 2 : 1) win_dkv_kernel(T* __restrict__ dk, T* __restrict__ dv, const T* __restrict__ dx,
                                                               const float2* __restrict__ stats, const float* __restrict__ delta,
                                                               float* __restrict__ sums, const __grid_constant__ WinParams p, WinSinkPlan plan,
                                                               int tiles, int vecq, int vecv) {
@@ -438,7 +445,7 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(T* __restrict__ dk
     if (p.buckets.count > 0) win_fill_diag<T, BM>(sD, nullptr, p, h, l0, s0);
     win_loaded();
     __syncthreads();
-    float z[TM][TM] = {}, dp[TM][TM] = {};
+    float z[TM][TM], dp[TM][TM];
     win_dots<LD>(z, sQ, sK, D4, ty, tx);
     win_dots<LD>(dp, sG, sV, E4, ty, tx);
 #pragma unroll
