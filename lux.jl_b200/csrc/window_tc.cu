@@ -1,7 +1,7 @@
 // Windowed attention on the tensor cores, forward: BFloat16, up to 128 features.
 //
 // A block owns two tiles of 128 queries that read the same keys: the tiles of two heads that share a key head, or two
-// neighbouring tiles of one head; each has its softmax group of four warps, a thread per row, and a warp that issues its products.
+// neighbouring tiles of one head; each has its softmax group of four warps, a thread per row.
 // Per tile of 128 keys: S = Q K' into TMEM, the group turns S into weights 2^(z2 - m2), which go back to TMEM as bf16 over S,
 // O += P V with P taken from TMEM. While one group is in its softmax the tensor cores work for the other. O is rescaled only when a row's maximum has grown by more than 2^8 (the reference m2 may lag behind
 // the maximum by that: weights up to 256 are as exact in bf16 as weights up to 1).
@@ -17,7 +17,7 @@ namespace lb2 {
 
 namespace {
 
-// warp 0: TMA, warps 1 and 2: MMA, warps 4-7 and 8-11: one softmax group each; registers 56 + 2 x 224 = 3 x 168 per thread at launch
+// warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: one softmax group each; registers 56 + 2 x 224 = 3 x 168 per thread at launch
 constexpr int kWtFwdThreads = 384, kWtFwdFew = 56, kWtFwdMany = 224;
 
 template <int NB> struct WtFwd {
@@ -77,8 +77,8 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
-    mbar_init(q_full, 1); mbar_init(q_empty, 2);
-    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 2); }
+    mbar_init(q_full, 1); mbar_init(q_empty, 1);
+    for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&pv_done[i], 1); mbar_init(&o_empty[i], 4); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -121,54 +121,62 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
-    } else if (warp < 3) {
-      // a warp per group: while one waits for its weights the other's products run
-      const int grp = warp - 1;
+    } else if (warp == 1) {
+      // one warp for both groups keeps them half a tile apart: their products do not run into one another
       uint32_t turn = 0, kst = 0, kph = 0, vst = 0, vph = 0;               // pairs; the ring's next key and value tile
-      uint32_t used = 0, outs = 0;                                         // P consumed, O begun
-      const uint32_t tS = tmem + grp * 128, tO = tmem + 256 + grp * 128, q = sQ + grp * C::TILE;
+      uint32_t used[2] = {0, 0}, outs[2] = {0, 0};                         // P consumed, O begun
       bool ok = true;
       for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
         const WtPair t(p, item);
         const int n = t.all.count();
         if (n == 0) continue;
-        const WtView<128> view(w, grp == 0 ? t.l0[0] : t.l0[1], t.queries, t.keys);
+        const WtView<128> view[2] = {WtView<128>(w, t.l0[0], t.queries, t.keys), WtView<128>(w, t.l0[1], t.queries, t.keys)};
         if (!mbar_wait_uniform(q_full, turn & 1u, p.status, 0x200u)) break;
         ++turn;
-        bool begun = false;
+        bool begun[2] = {false, false};
         // the next tile's logits after this one's product, whose weights they overwrite
-        for (int j = -1; j < n; ++j) {
-          const bool next = j + 1 < n, use = j >= 0 && view.some(t.all.at(j) * kWtTile), make = next && view.some(t.all.at(j + 1) * kWtTile);
-          if (next && !mbar_wait_uniform(&full[2 * kst], kph, p.status, 0x400u)) ok = false;
-          if (j >= 0 && !mbar_wait_uniform(&full[2 * vst + 1], vph, p.status, 0x400u)) ok = false;
-          if (use) {
-            if (!begun && !mbar_wait_uniform(&o_empty[grp], (outs & 1u) ^ 1u, p.status, 0x4000u)) ok = false;
-            if (!mbar_wait_uniform(&p_ready[grp], used & 1u, p.status, 0x800u)) ok = false;
+        for (int j = -1; j < n && ok; ++j) {
+          const bool next = j + 1 < n;
+          const int s0 = j >= 0 ? t.all.at(j) * kWtTile : 0, s1 = next ? t.all.at(j + 1) * kWtTile : 0;
+          if (next && !mbar_wait_uniform(&full[2 * kst], kph, p.status, 0x400u)) { ok = false; break; }
+          if (j >= 0 && !mbar_wait_uniform(&full[2 * vst + 1], vph, p.status, 0x400u)) { ok = false; break; }
+          const uint32_t k = sKV + 2 * kst * C::TILE, v = sKV + (2 * vst + 1) * C::TILE;
+#pragma unroll
+          for (int grp = 0; grp < 2; ++grp) {
+            const bool use = j >= 0 && view[grp].some(s0), make = next && view[grp].some(s1);
+            if (use) {
+              if (!begun[grp] && !mbar_wait_uniform(&o_empty[grp], (outs[grp] & 1u) ^ 1u, p.status, 0x4000u)) ok = false;
+              if (!mbar_wait_uniform(&p_ready[grp], used[grp] & 1u, p.status, 0x800u)) ok = false;
+              if (!ok) break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t tS = tmem + grp * 128, tO = tmem + 256 + grp * 128;
+              if (use) {
+                if (NB == 2 && p.boxes_e == 2) wt_mma_tokens<NB>(tO, tS, v, begun[grp]);
+                else wt_mma_tokens<1>(tO, tS, v, begun[grp]);
+                umma_commit(&pv_done[grp]);
+              }
+              if (make) {
+                if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tS, sQ + grp * C::TILE, k);
+                else wt_mma_features<1>(tS, sQ + grp * C::TILE, k);
+                umma_commit(&s_full[grp]);
+              }
+            }
+            __syncwarp();
+            if (use) {
+              if (!begun[grp]) ++outs[grp];
+              ++used[grp];
+              begun[grp] = true;
+            }
           }
           if (!ok) break;
-          tc_fence_after();
-          const uint32_t k = sKV + 2 * kst * C::TILE, v = sKV + (2 * vst + 1) * C::TILE;
           if (elect_one()) {
-            if (use) {
-              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens<NB>(tO, tS, v, begun);
-              else wt_mma_tokens<1>(tO, tS, v, begun);
-              umma_commit(&pv_done[grp]);
-            }
-            if (make) {
-              if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tS, q, k);
-              else wt_mma_features<1>(tS, q, k);
-              umma_commit(&s_full[grp]);
-            }
             if (j >= 0) umma_commit(&empty[2 * vst + 1]);
             if (next) umma_commit(&empty[2 * kst]);
             if (j + 1 == n - 1) umma_commit(q_empty);
           }
           __syncwarp();
-          if (use) {
-            if (!begun) ++outs;
-            ++used;
-            begun = true;
-          }
           if (j >= 0 && ++vst == C::STAGES / 2) { vst = 0; vph ^= 1u; }
           if (next && ++kst == C::STAGES / 2) { kst = 0; kph ^= 1u; }
         }
@@ -372,10 +380,11 @@ int32_t win_tc_fwd(const WinParams& w, void* x, void* rest, float2* stats, cudaS
   LB2_REQUIRE(items <= 0x7FFF0000, LB2_BAD_SHAPE, "too many rows");        // and a grid more
   p.items = (int)items;
   const int sms = sm_count();
+  const int64_t steps = std::min<int64_t>(w.S, (int64_t)w.window + kWtTile) / kWtTile + 1;
   auto launch = [&](auto kernel, int smem) -> int32_t {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
-    kernel<<<(unsigned)(p.items < sms ? p.items : sms), kWtFwdThreads, smem, st>>>(mq, mk, mv, p);
+    kernel<<<wt_blocks(p.items, sms, steps), kWtFwdThreads, smem, st>>>(mq, mk, mv, p);
     LB2_CHECK_LAUNCH("windowed attention");
     return LB2_OK;
   };

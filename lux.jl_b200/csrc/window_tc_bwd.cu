@@ -31,7 +31,7 @@ struct WtBwdParams {
   float* rows;                               // [batch][head][tile][-m2 | -log2 sum | -delta][128]
   float* partial;
   float* sink_sums;                          // [split][tile][batch][kv head][128][D + E], fp32
-  int tiles, query_tiles, items, columns, boxes_d, boxes_e, wide_d;
+  int tiles, query_tiles, items, columns, boxes_d, boxes_e, wide_d, wide_kv;
   WinSinkPlan sinks;
   unsigned int* status;
 };
@@ -56,6 +56,42 @@ struct WtQueries {
     own = wt_key_tiles(p.w, l0, queries, keys);
   }
 };
+// a tile of keys, or its part of the queries: tiles of queries first .. first + per_head of each head, n of them from `begin` on
+struct WtKeys {
+  WinKeyTile mine;
+  int s0, g, b, queries, keys, first, per_head, begin, n;
+  __device__ __forceinline__ WtKeys(const WtBwdParams& p, int item) : mine(item, p.tiles, p.w.Hkv * p.w.B, p.sinks) {
+    const WinParams& w = p.w;
+    g = mine.gb % w.Hkv; b = mine.gb / w.Hkv; s0 = mine.tile * kWtTile;
+    queries = warp_uniform(win_tokens(w, b, w.L)); keys = warp_uniform(win_tokens(w, b, w.S));
+    int lo, hi;
+    win_query_range(w, s0, min(s0 + kWtTile, keys), queries, &lo, &hi);
+    first = lo / kWtTile;
+    per_head = s0 < keys && lo < hi ? (hi + kWtTile - 1) / kWtTile - first : 0;
+    const int64_t all = (int64_t)per_head * w.rep;
+    begin = (int)(all * mine.split / mine.splits);
+    n = (int)(all * (mine.split + 1) / mine.splits) - begin;
+  }
+  __device__ __forceinline__ int head(const WinParams& w) const { return g * w.rep + (per_head > 0 ? begin / per_head : 0); }
+  __device__ __forceinline__ int query_tile() const { return first + (per_head > 0 ? begin % per_head : 0); }
+};
+// 32 NB columns of a row from column c0 on, times f: whether all are finite. `in`: the row exists; `real`: it counts, else zeros
+template <int NB>
+__device__ __forceinline__ bool wt_store_row(__nv_bfloat16* to, const float (&v)[32 * NB], float f, int c0, int width, bool in, bool real, bool wide) {
+  bool fine = true;
+#pragma unroll
+  for (int q = 0; q < 2 * NB; ++q) {
+    uint32_t o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float a = v[q * 16 + 2 * x] * f, c = v[q * 16 + 2 * x + 1] * f;
+      if (c0 + q * 16 + 2 * x < width) fine = fine && isfinite(a) && isfinite(c);
+      o[x] = real ? pack_bf16(a, c) : 0u;
+    }
+    if (in) wt_store16(to + c0 + q * 16, o, width - c0 - q * 16, wide);
+  }
+  return fine;
+}
 // Adds 32 rows x 64 columns of d to the warp's sums by bucket. 16 columns at a time a lane hands the sum of its diagonal r - j on to the
 // next lane's column; lane 31's is complete. Then neighbouring diagonals of one bucket join.
 __device__ __forceinline__ void wt_diagonals(const float (&d)[64], float* my_diag, float* my_bsum, const uint8_t* bucket, int half, int quarter, int lane) {
@@ -374,19 +410,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int j = 0; j < 32 * NB; ++j) o[j] = 0.f;
       }
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.dq) + (((int64_t)t.b * w.L + l) * w.H + h) * w.D;
-      bool fine = true;
-#pragma unroll
-      for (int q = 0; q < 2 * NB; ++q) {
-        const int c0 = half * NB * 32 + q * 16;
-        uint32_t v[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float a = o[q * 16 + 2 * x] * w.scale, c = o[q * 16 + 2 * x + 1] * w.scale;
-          if (c0 + 2 * x < w.D) fine = fine && isfinite(a) && isfinite(c);
-          v[x] = l < t.queries ? pack_bf16(a, c) : 0u;
-        }
-        if (l < w.L) wt_store16(out + c0, v, w.D - c0, p.wide_d != 0);
-      }
+      const bool fine = wt_store_row<NB>(out, o, w.scale, half * NB * 32, w.D, l < w.L, l < t.queries, p.wide_d != 0);
       if (l < t.queries && !fine) *bad = 1;
     }
     // rows that an infinity or NaN reached, once the pipeline no longer waits for these warps
@@ -425,29 +449,21 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   float* lut = reinterpret_cast<float*>(gen + (2 + C::STAGES) * C::TILE);          // [parity][256]
   float* cols = lut + 2 * 256;                                                     // per query tile of the ring: -m2 | -log2 sum | -delta
-  int* bad = reinterpret_cast<int*>(cols + C::STAGES / 2 * 3 * 128);               // [128]
+  int* bad = reinterpret_cast<int*>(cols + C::STAGES / 2 * 3 * 128);
   int32_t* first_of = reinterpret_cast<int32_t*>(bad + 128);                       // where the buckets start
   uint64_t* bars = reinterpret_cast<uint64_t*>(first_of + kWinMaxBuckets);
-  uint64_t *k_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 1, *p_ready = dp_full + 1,
-           *ds_ready = p_ready + 1, *o_full = ds_ready + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 1);
+  uint64_t *k_full = bars, *k_empty = bars + 1, *full = bars + 2, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *dp_full = s_full + 1,
+           *p_ready = dp_full + 1, *ds_ready = p_ready + 1, *o_full = ds_ready + 1, *o_empty = o_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_empty + 1);
   const uint32_t sK = base, sV = base + C::TILE, sQG = base + 2 * C::TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const WinParams& w = p.w;
-  const int groups = w.Hkv * w.B;
-  const WinKeyTile mine(blockIdx.x, p.tiles, groups, p.sinks);
-  const int tile = mine.tile, gb = mine.gb, split = mine.split, splits = mine.splits;
-  const int g = gb % w.Hkv, b = gb / w.Hkv, s0 = tile * kWtTile;
-  const int queries = warp_uniform(win_tokens(w, b, w.L)), keys = warp_uniform(win_tokens(w, b, w.S));
-  int lo, hi;
-  win_query_range(w, s0, min(s0 + kWtTile, keys), queries, &lo, &hi);
-  const int first = lo / kWtTile, per_head = s0 < keys && lo < hi ? (hi + kWtTile - 1) / kWtTile - first : 0;
-  const int begin = (int)((int64_t)per_head * w.rep * split / splits), n = (int)((int64_t)per_head * w.rep * (split + 1) / splits) - begin;
 
   if (threadIdx.x == 0) {
-    mbar_init(k_full, 1);
+    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmG); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+    mbar_init(k_full, 1); mbar_init(k_empty, 1);
     for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(o_full, 1);
+    mbar_init(s_full, 1); mbar_init(dp_full, 1); mbar_init(p_ready, 8); mbar_init(ds_ready, 8); mbar_init(o_full, 1); mbar_init(o_empty, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x >= 64 && threadIdx.x < 64 + kWinMaxBuckets) first_of[threadIdx.x - 64] = w.buckets.first[threadIdx.x - 64];
@@ -455,7 +471,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (threadIdx.x < 128) bad[threadIdx.x] = 0;
+  if (threadIdx.x == 0) *bad = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -463,262 +479,278 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   if (warp < 4) {
     regs_less<kWtBwdFew>();
-    if (warp == 0 && n > 0) {
-      if (elect_one()) {
-        mbar_expect_tx(k_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
-        for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sK + x * kWtBox, &tmK, x * 64, g, s0, b, k_full);
-        for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sV + x * kWtBox, &tmV, x * 64, g, s0, b, k_full);
+    if (warp == 0) {
+      uint32_t stage = 0, phase = 0, turn = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        const WtKeys t(p, item);
+        if (t.n == 0) continue;
+        if (!mbar_wait_uniform(k_empty, (turn & 1u) ^ 1u, p.status, 0x80u)) break;
+        ++turn;
+        if (elect_one()) {
+          mbar_expect_tx(k_full, (uint32_t)((p.boxes_d + p.boxes_e) * kWtBox));
+          for (int x = 0; x < p.boxes_d; ++x) tma_load_4d(sK + x * kWtBox, &tmK, x * 64, t.g, t.s0, t.b, k_full);
+          for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sV + x * kWtBox, &tmV, x * 64, t.g, t.s0, t.b, k_full);
+        }
+        __syncwarp();
+        int h = t.head(w), qt = t.query_tile();
+        for (int i = 0; i < 2 * t.n; ++i) {
+          if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) { ok = false; break; }
+          if (elect_one()) {
+            const bool is_q = (i & 1) == 0;
+            const int boxes = is_q ? p.boxes_d : p.boxes_e;
+            mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox + (is_q ? kWtRowBytes : 0)));
+            for (int x = 0; x < boxes; ++x) tma_load_4d(sQG + stage * C::TILE + x * kWtBox, is_q ? &tmQ : &tmG, x * 64, h, qt * kWtTile, t.b, &full[stage]);
+            if (is_q)
+              bulk_load_1d(smem_u32(cols) + (stage >> 1) * kWtRowBytes, p.rows + (((int64_t)t.b * w.H + h) * p.query_tiles + qt) * 3 * kWtTile, kWtRowBytes,
+                           &full[stage]);
+          }
+          __syncwarp();
+          if ((i & 1) == 1 && ++qt == t.first + t.per_head) { qt = t.first; ++h; }
+          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        }
       }
-      __syncwarp();
-      uint32_t stage = 0, phase = 0;
-      int h = g * w.rep + begin / per_head, qt = first + begin % per_head;
-      for (int i = 0; i < 2 * n; ++i) {
-        if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) break;
-        if (elect_one()) {
-          const bool is_q = (i & 1) == 0;
-          const int boxes = is_q ? p.boxes_d : p.boxes_e;
-          mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox + (is_q ? kWtRowBytes : 0)));
-          for (int x = 0; x < boxes; ++x) tma_load_4d(sQG + stage * C::TILE + x * kWtBox, is_q ? &tmQ : &tmG, x * 64, h, qt * kWtTile, b, &full[stage]);
-          if (is_q)
-            bulk_load_1d(smem_u32(cols) + (stage >> 1) * kWtRowBytes, p.rows + (((int64_t)b * w.H + h) * p.query_tiles + qt) * 3 * kWtTile, kWtRowBytes,
-                         &full[stage]);
-        }
-        if ((i & 1) == 1 && ++qt == first + per_head) { qt = first; ++h; }
-        __syncwarp();
-        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-      }
-    } else if (warp == 1 && n > 0) {
-      bool ok = mbar_wait_uniform(k_full, 0, p.status, 0x200u);
-      uint32_t qst = 0, gst = 0, ph_q = 0, ph_g = 0, qprev = 0, gprev = 0;
-      for (int i = -1; i < n && ok; ++i) {
-        const bool next = i + 1 < n;
-        const uint32_t qn = sQG + 2 * qst * C::TILE, gn = sQG + (2 * gst + 1) * C::TILE, qc = sQG + 2 * qprev * C::TILE, gc = sQG + (2 * gprev + 1) * C::TILE;
-        if (i >= 0 && !mbar_wait_uniform(p_ready, (uint32_t)i & 1u, p.status, 0x800u)) { ok = false; break; }
-        if (next && !mbar_wait_uniform(&full[2 * qst], ph_q, p.status, 0x400u)) { ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          if (i >= 0) {
-            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, gc, i > 0);
-            else wt_mma_tokens_halves<1>(tDV, tmem, gc, i > 0);
-            umma_commit(&empty[2 * gprev + 1]);
+    } else if (warp == 1) {
+      uint32_t turn = 0, done = 0, qst = 0, gst = 0, ph_q = 0, ph_g = 0;   // items, tiles of queries so far; the ring's next tiles
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
+        const WtKeys t(p, item);
+        const int n = t.n;
+        if (n == 0) continue;
+        if (!mbar_wait_uniform(k_full, turn & 1u, p.status, 0x200u)) break;
+        uint32_t qprev = 0, gprev = 0;
+        for (int i = -1; i < n; ++i) {
+          const bool next = i + 1 < n;
+          const uint32_t par = (done + (uint32_t)i) & 1u;
+          const uint32_t qn = sQG + 2 * qst * C::TILE, gn = sQG + (2 * gst + 1) * C::TILE, qc = sQG + 2 * qprev * C::TILE, gc = sQG + (2 * gprev + 1) * C::TILE;
+          if (i >= 0 && !mbar_wait_uniform(p_ready, par, p.status, 0x800u)) { ok = false; break; }
+          if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
+          if (next && !mbar_wait_uniform(&full[2 * qst], ph_q, p.status, 0x400u)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (i >= 0) {
+              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, gc, i > 0);
+              else wt_mma_tokens_halves<1>(tDV, tmem, gc, i > 0);
+              umma_commit(&empty[2 * gprev + 1]);
+            }
+            if (next) {
+              if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, qn);
+              else wt_mma_features<1>(tmem, sK, qn);
+              umma_commit(s_full);
+            }
           }
+          __syncwarp();
+          if (i >= 0 && !mbar_wait_uniform(ds_ready, par, p.status, 0x8000u)) { ok = false; break; }
+          if (next && !mbar_wait_uniform(&full[2 * gst + 1], ph_g, p.status, 0x400u)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            if (i >= 0) {
+              if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, qc, i > 0);
+              else wt_mma_tokens_halves<1>(tDK, tDP, qc, i > 0);
+              umma_commit(&empty[2 * qprev]);
+              if (!next) umma_commit(o_full);
+            }
+            if (next) {
+              if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, gn);
+              else wt_mma_features<1>(tDP, sV, gn);
+              umma_commit(dp_full);
+              if (i + 2 == n) umma_commit(k_empty);
+            }
+          }
+          __syncwarp();
+          qprev = qst; gprev = gst;
           if (next) {
-            if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, qn);
-            else wt_mma_features<1>(tmem, sK, qn);
-            umma_commit(s_full);
+            if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
+            if (++gst == C::STAGES / 2) { gst = 0; ph_g ^= 1u; }
           }
         }
-        __syncwarp();
-        if (i >= 0 && !mbar_wait_uniform(ds_ready, (uint32_t)i & 1u, p.status, 0x8000u)) { ok = false; break; }
-        if (next && !mbar_wait_uniform(&full[2 * gst + 1], ph_g, p.status, 0x400u)) { ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          if (i >= 0) {
-            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, qc, i > 0);
-            else wt_mma_tokens_halves<1>(tDK, tDP, qc, i > 0);
-            umma_commit(&empty[2 * qprev]);
-            if (!next) umma_commit(o_full);
-          }
-          if (next) {
-            if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, gn);
-            else wt_mma_features<1>(tDP, sV, gn);
-            umma_commit(dp_full);
-          }
-        }
-        __syncwarp();
-        qprev = qst; gprev = gst;
-        if (next) {
-          if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
-          if (++gst == C::STAGES / 2) { gst = 0; ph_g ^= 1u; }
-        }
+        ++turn;
+        done += (uint32_t)n;
       }
     }
   } else {
     regs_more<kWtBwdMany>();
-    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, s = s0 + row, st = threadIdx.x - 128;
+    const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, st = threadIdx.x - 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + half * 64, tD = tDP + lanes + half * 64;
     const float c2 = w.scale2;
     const bool biased = w.buckets.count > 0;
-    bool ok = true;
-    int h = 0, qt = 0, table = 0;
-    uint32_t qst = 0, ph_q = 0;
-    if (n > 0) { h = g * w.rep + begin / per_head; qt = first + begin % per_head; }
-    WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
-    for (int i = 0; i < n; ++i) {
-      const int l0 = qt * kWtTile;
-      const float* col = cols + qst * 3 * kWtTile;
-      float flat = 0.f;
-      const float* bias = nullptr;
-      if (biased) {
-        const int low = s0 - l0 - (kWtTile - 1);
-        if (tail.is_left(low + 2 * (kWtTile - 1))) {
-          flat = tail.left;
-        } else if (tail.is_right(w, low)) {
-          flat = tail.right;
-        } else {                                   // index (column - row) + 127: rel = low + 254 - index
-          float* to = lut + table * 256;
-          table ^= 1;                              // each use has a barrier: two tables are enough
-          if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, first_of, h, low + 254 - st);
-          bar_group(1, kWtSoft);
-          bias = to + (kWtTile - 1 - row) + half * 64;
+    bool ok = true;                     // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
+    int table = 0;
+    uint32_t qst = 0, ph_q = 0, done = 0, turn = 0;
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+      const WtKeys t(p, item);
+      const int n = t.n, s0 = t.s0, s = s0 + row, b = t.b, g = t.g, queries = t.queries, keys = t.keys;
+      int h = t.head(w), qt = t.query_tile();
+      WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
+      for (int i = 0; i < n; ++i) {
+        const int l0 = qt * kWtTile;
+        const uint32_t par = (done + (uint32_t)i) & 1u;
+        const float* col = cols + qst * 3 * kWtTile;
+        float flat = 0.f;
+        const float* bias = nullptr;
+        if (biased) {
+          const int low = s0 - l0 - (kWtTile - 1);
+          if (tail.is_left(low + 2 * (kWtTile - 1))) {
+            flat = tail.left;
+          } else if (tail.is_right(w, low)) {
+            flat = tail.right;
+          } else {                                   // index (column - row) + 127: rel = low + 254 - index
+            float* to = lut + table * 256;
+            table ^= 1;                              // each use has a barrier: two tables are enough
+            if (st < 255) to[st] = win_bias<__nv_bfloat16>(w, first_of, h, low + 254 - st);
+            bar_group(1, kWtSoft);
+            bias = to + (kWtTile - 1 - row) + half * 64;
+          }
         }
-      }
-      // the queries that see key s: columns from..to
-      int from = w.causal ? s - l0 : (s < w.sinks ? 0 : s - w.window + 1 - l0);
-      int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
-      if (s >= keys) to = -1;
-      const bool whole = wt_all_seen(w, l0, queries, s0, keys, kWtTile);
-      ok = ok && mbar_wait_warp(&full[2 * qst], ph_q, p.status, 0x8u);       // the columns' stats
-      ok = ok && mbar_wait_warp(s_full, (uint32_t)i & 1u, p.status, 0x1000u);
-      tc_fence_after();
-      float d[64];
-      const bool apart = bias == nullptr && wt_apart(c2, flat);
-      const uint64_t mul2_ = pack2(c2, c2), flat2_ = pack2(flat, flat);
-      tmem_row64<0>(tS, d);
-      if (apart) {
+        // the queries that see key s: columns from..to
+        int from = w.causal ? s - l0 : (s < w.sinks ? 0 : s - w.window + 1 - l0);
+        int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
+        if (s >= keys) to = -1;
+        const bool whole = wt_all_seen(w, l0, queries, s0, keys, kWtTile);
+        ok = ok && mbar_wait_warp(&full[2 * qst], ph_q, p.status, 0x8u);       // the columns' stats
+        ok = ok && mbar_wait_warp(s_full, par, p.status, 0x1000u);
+        tc_fence_after();
+        float d[64];
+        const bool apart = bias == nullptr && wt_apart(c2, flat);
+        const uint64_t mul2_ = pack2(c2, c2), flat2_ = pack2(flat, flat);
+        tmem_row64<0>(tS, d);
+        if (apart) {
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
-          const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
-          float y[4];
-          unpack2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add2(flat2_, pack2(m.x, m.y))), pack2(e.x, e.y)), y[0], y[1]);
-          unpack2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add2(flat2_, pack2(m.z, m.w))), pack2(e.z, e.w)), y[2], y[3]);
+          for (int j = 0; j < 64; j += 4) {
+            const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
+            float y[4];
+            unpack2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add2(flat2_, pack2(m.x, m.y))), pack2(e.x, e.y)), y[0], y[1]);
+            unpack2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add2(flat2_, pack2(m.z, m.w))), pack2(e.z, e.w)), y[2], y[3]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
+            for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
+            const uint64_t add0 = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_, add1 = bias != nullptr ? pack2(bias[j + 2], bias[j + 3]) : flat2_;
+            float y[4];
+            unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add0), pack2(m.x, m.y)), pack2(e.x, e.y)), y[0], y[1]);
+            unpack2(add2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add1), pack2(m.z, m.w)), pack2(e.z, e.w)), y[2], y[3]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
+          }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 64; j += 4) {
-          const float4 m = lds4(col + half * 64 + j), e = lds4(col + 128 + half * 64 + j);
-          const uint64_t add0 = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_, add1 = bias != nullptr ? pack2(bias[j + 2], bias[j + 3]) : flat2_;
-          float y[4];
-          unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add0), pack2(m.x, m.y)), pack2(e.x, e.y)), y[0], y[1]);
-          unpack2(add2(add2(fma2(pack2(d[j + 2], d[j + 3]), mul2_, add1), pack2(m.z, m.w)), pack2(e.z, e.w)), y[2], y[3]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) d[j + k] = ex2(y[k]);
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
-        }
-      }
-      {
-        uint32_t v[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
-        tmem_st32(tS, v);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_ready);
-      ok = ok && mbar_wait_warp(dp_full, (uint32_t)i & 1u, p.status, 0x2000u);
-      tc_fence_after();
-      uint32_t o[32];
-      {
-        float e[64];
-        tmem_row64<0>(tD, e);
         if (!whole) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const uint32_t single = __ballot_sync(0xffffffffu, win_single(w, l0 + half * 64 + q * 32 + lane, keys));
-            if (single != 0) {
+            const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                e[q * 32 + j] = single >> j & 1u ? (e[q * 32 + j] - e[q * 32 + j]) - col[256 + half * 64 + q * 32 + j] : e[q * 32 + j];
+            for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
+          }
+        }
+        {
+          uint32_t v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+          tmem_st32(tS, v);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+        ok = ok && mbar_wait_warp(dp_full, par, p.status, 0x2000u);
+        tc_fence_after();
+        uint32_t o[32];
+        {
+          float e[64];
+          tmem_row64<0>(tD, e);
+          if (!whole) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const uint32_t single = __ballot_sync(0xffffffffu, win_single(w, l0 + half * 64 + q * 32 + lane, keys));
+              if (single != 0) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  e[q * 32 + j] = single >> j & 1u ? (e[q * 32 + j] - e[q * 32 + j]) - col[256 + half * 64 + q * 32 + j] : e[q * 32 + j];
+              }
             }
+          }
+#pragma unroll
+          for (int j = 0; j < 64; j += 4) {
+            const float4 nd = lds4(col + 256 + half * 64 + j);
+            unpack2(mul2(add2(pack2(e[j], e[j + 1]), pack2(nd.x, nd.y)), pack2(d[j], d[j + 1])), d[j], d[j + 1]);
+            unpack2(mul2(add2(pack2(e[j + 2], e[j + 3]), pack2(nd.z, nd.w)), pack2(d[j + 2], d[j + 3])), d[j + 2], d[j + 3]);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
           }
         }
 #pragma unroll
-        for (int j = 0; j < 64; j += 4) {
-          const float4 nd = lds4(col + 256 + half * 64 + j);
-          unpack2(mul2(add2(pack2(e[j], e[j + 1]), pack2(nd.x, nd.y)), pack2(d[j], d[j + 1])), d[j], d[j + 1]);
-          unpack2(mul2(add2(pack2(e[j + 2], e[j + 3]), pack2(nd.z, nd.w)), pack2(d[j + 2], d[j + 3])), d[j + 2], d[j + 3]);
+        for (int j = 0; j < 32; ++j) o[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+        tmem_st32(tD, o);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready);
+        if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
+        if (++qt == t.first + t.per_head) {
+          qt = t.first; ++h;
+          if (biased && i + 1 < n) tail = WtFlat(w, static_cast<const __nv_bfloat16*>(w.table), h);
         }
       }
-      if (!whole) {
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t bits = wt_below(to + 1 - half * 64 - q * 32) & ~wt_below(from - half * 64 - q * 32);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
+      done += (uint32_t)n;
+      float ak[32 * NB], av[32 * NB];
+      if (n > 0) {
+        ok = ok && mbar_wait_warp(o_full, turn & 1u, p.status, 0x4000u);
+        ++turn;
+        tc_fence_after();
+        if constexpr (NB == 2) {
+          tmem_row64<0>(tDK + lanes + half * 64, ak);
+          tmem_row64<0>(tDV + lanes + half * 64, av);
+        } else {
+          tmem_row32<0>(tDK + lanes + half * 32, ak);
+          tmem_row32<0>(tDV + lanes + half * 32, av);
         }
-      }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_empty);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) o[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
-      tmem_st32(tD, o);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(ds_ready);
-      if (++qst == C::STAGES / 2) { qst = 0; ph_q ^= 1u; }
-      if (++qt == first + per_head) {
-        qt = first; ++h;
-        if (biased && i + 1 < n) tail = WtFlat(w, static_cast<const __nv_bfloat16*>(w.table), h);
+        for (int x = 0; x < 32 * NB; ++x) ak[x] = av[x] = 0.f;
+      }
+      const int c0 = half * NB * 32;
+      if (t.mine.splits > 1) {
+        float* out = p.sink_sums + ((((int64_t)t.mine.split * p.sinks.tiles + t.mine.tile) * (w.Hkv * w.B) + t.mine.gb) * kWtTile + row) * (w.D + w.E);
+#pragma unroll
+        for (int x = 0; x < 32 * NB; x += 4) {
+          if (c0 + x < w.D) *reinterpret_cast<float4*>(out + c0 + x) = make_float4(ak[x] * w.scale, ak[x + 1] * w.scale, ak[x + 2] * w.scale, ak[x + 3] * w.scale);
+          if (c0 + x < w.E) *reinterpret_cast<float4*>(out + w.D + c0 + x) = make_float4(av[x], av[x + 1], av[x + 2], av[x + 3]);
+        }
+      } else {
+        bool fine = wt_store_row<NB>(static_cast<__nv_bfloat16*>(p.dk) + (((int64_t)b * w.S + s) * w.Hkv + g) * w.D, ak, w.scale, c0, w.D, s < w.S, s < keys,
+                                     p.wide_kv != 0);
+        fine = wt_store_row<NB>(static_cast<__nv_bfloat16*>(p.dv) + (((int64_t)b * w.S + s) * w.Hkv + g) * w.E, av, 1.f, c0, w.E, s < w.S, s < keys,
+                                p.wide_kv != 0) && fine;
+        if (s < keys && !fine) *bad = 1;
       }
     }
-    if (n > 0) ok = ok && mbar_wait_warp(o_full, 0, p.status, 0x4000u);
-    if (splits > 1) {
-      tc_fence_after();
-      float* out = p.sink_sums + ((((int64_t)split * p.sinks.tiles + tile) * groups + gb) * kWtTile + row) * (w.D + w.E);
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const int width = which == 0 ? w.D : w.E;
-        const float f = which == 0 ? w.scale : 1.f;
-#pragma unroll
-        for (int q = 0; q < NB; ++q) {
-          const int c0 = half * NB * 32 + q * 32;
-          if (c0 >= width) break;
-          uint32_t v[32] = {};
-          if (n > 0) {
-            tmem_ld32((which == 0 ? tDK : tDV) + lanes + c0, v);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            if (c0 + j < width)
-              *reinterpret_cast<float4*>(out + which * w.D + c0 + j) = make_float4(__uint_as_float(v[j]) * f, __uint_as_float(v[j + 1]) * f,
-                                                                                   __uint_as_float(v[j + 2]) * f, __uint_as_float(v[j + 3]) * f);
+    // rows that an infinity or NaN reached, once the pipeline no longer waits for these warps
+    bar_group(1, kWtSoft);
+    if (*bad != 0) {
+      for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+        const WtKeys t(p, item);
+        if (t.mine.splits > 1) continue;
+        for (int r = sw; r < kWtTile && t.s0 + r < t.keys; r += 8) {
+          const int64_t at = ((int64_t)t.b * w.S + t.s0 + r) * w.Hkv + t.g;
+          bool fine = true;
+          for (int e = lane; e < w.D; e += 32) fine = fine && isfinite(__bfloat162float(static_cast<const __nv_bfloat16*>(p.dk)[at * w.D + e]));
+          for (int e = lane; e < w.E; e += 32) fine = fine && isfinite(__bfloat162float(static_cast<const __nv_bfloat16*>(p.dv)[at * w.E + e]));
+          if (!__all_sync(0xffffffffu, fine))
+            win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, t.s0 + r, t.g, t.b,
+                                       t.queries, t.keys);
         }
       }
-    } else {
-      tc_fence_after();
-      bool fine = true;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const int width = which == 0 ? w.D : w.E;
-        const float f = which == 0 ? w.scale : 1.f;
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(which == 0 ? p.dk : p.dv) + (((int64_t)b * w.S + s) * w.Hkv + g) * width;
-#pragma unroll
-        for (int q = 0; q < NB; ++q) {
-          const int c0 = half * NB * 32 + q * 32;
-          if (c0 >= width) break;
-          uint32_t v[32] = {};
-          if (n > 0) {
-            tmem_ld32((which == 0 ? tDK : tDV) + lanes + c0, v);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint32_t x[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float a = __uint_as_float(v[j + 2 * k]) * f, c = __uint_as_float(v[j + 2 * k + 1]) * f;
-              if (c0 + j < width) fine = fine && isfinite(a) && isfinite(c);
-              x[k] = s < keys ? pack_bf16(a, c) : 0u;
-            }
-            if (s < w.S && c0 + j < width) *reinterpret_cast<uint4*>(out + c0 + j) = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        }
-      }
-      if (s < keys && !fine) bad[row] = 1;
-      bar_group(1, kWtSoft);
-      for (int r = sw; r < kWtTile; r += 8)
-        if (bad[r])
-          win_row_dkv<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.dk), static_cast<__nv_bfloat16*>(p.dv), p.dx, p.stats, p.delta, s0 + r, g, b, queries, keys);
     }
   }
 
@@ -805,12 +837,15 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
   LB2_REQUIRE(qt * w.H * w.B <= 0x7FFF0000, LB2_BAD_SHAPE, "too many rows");           // and a grid more
   p.items = (int)(qt * w.H * w.B);
   p.wide_d = aligned_to(dq, 32) && w.D % 16 == 0;
-  const int64_t resident = std::min(p.items, sm_count());
+  const int64_t steps = std::min<int64_t>(w.S, (int64_t)w.window + kWtTile) / kWtTile + 1, resident = wt_blocks(p.items, sm_count(), steps);
   int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, resident);
   if (rc != LB2_OK) return rc;
-  const int64_t groups = (int64_t)w.Hkv * w.B, blocks = (kt - p.sinks.tiles + (int64_t)p.sinks.tiles * p.sinks.splits) * groups;
-  LB2_REQUIRE(blocks <= 0x7FFFFFFF, LB2_BAD_SHAPE, "too many rows");
-  rc = one ? launch(win_tc_dkv_kernel<1>, WtBwd<1>::SMEM, kt, blocks) : launch(win_tc_dkv_kernel<2>, WtBwd<2>::SMEM, kt, blocks);
+  const int64_t blocks = (kt - p.sinks.tiles + (int64_t)p.sinks.tiles * p.sinks.splits) * w.Hkv * w.B;
+  LB2_REQUIRE(blocks <= 0x7FFF0000, LB2_BAD_SHAPE, "too many rows");
+  p.items = (int)blocks;
+  p.wide_kv = aligned_to(dk, 32) && aligned_to(dv, 32) && w.D % 16 == 0 && w.E % 16 == 0;
+  const int64_t resident_kv = wt_blocks(p.items, sm_count(), (std::min<int64_t>(w.L, (int64_t)w.window + kWtTile) / kWtTile + 1) * w.rep);
+  rc = one ? launch(win_tc_dkv_kernel<1>, WtBwd<1>::SMEM, kt, resident_kv) : launch(win_tc_dkv_kernel<2>, WtBwd<2>::SMEM, kt, resident_kv);
   if (rc != LB2_OK || p.sinks.tiles == 0) return rc;
   return win_sinks_join(w, p.sinks, kWtTile, dk, dv, sink_sums, dx, stats, delta, LB2_BF16, st);
 }
