@@ -17,8 +17,8 @@ namespace lb2 {
 
 namespace {
 
-// warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: one softmax group each; registers 56 + 2 x 224 = 3 x 168 per thread at launch
-constexpr int kWtFwdThreads = 384, kWtFwdFew = 56, kWtFwdMany = 224;
+// warp 0: TMA, warp 1: MMA, warps 4-7 and 8-11: one softmax group each; registers 104 + 2 x 200 = 3 x 168 per thread at launch
+constexpr int kWtFwdThreads = 384, kWtFwdFew = 104, kWtFwdMany = 200;
 
 template <int NB> struct WtFwd {
   static constexpr int TILE = NB * kWtBox;
