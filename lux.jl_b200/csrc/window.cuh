@@ -85,7 +85,8 @@ template <typename T> __device__ __forceinline__ float win_bias(const WinParams&
 }
 
 // The tiles of keys that hold sinks, and by how many blocks each is shared in dk, dv: a block walks no more tiles of queries than an
-// ordinary one or, if that is more, half an SM's share of the whole.
+// ordinary one or, if that is more, half an SM's share of the whole. 8192 tokens, 32 heads on 8, window 1024, 4 sinks: 4 blocks, 450 us
+// where one block for the sinks took 995.
 struct WinSinkPlan { int tiles, splits; };
 inline WinSinkPlan win_sink_plan(int tile, int64_t queries, int64_t keys, int64_t window, int64_t sinks, int64_t rep, int64_t groups) {
   auto tiles = [&](int64_t n) { return (n + tile - 1) / tile; };

