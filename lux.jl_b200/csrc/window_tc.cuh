@@ -197,7 +197,6 @@ struct WtTiles {
   int nsink, first, last;
   __device__ __forceinline__ int count() const { return nsink + max(0, last - first); }
   __device__ __forceinline__ int at(int i) const { return i < nsink ? i : first + (i - nsink); }
-  __device__ __forceinline__ bool has(int t) const { return t < nsink || (t >= first && t < last); }
 };
 __device__ __forceinline__ WtTiles wt_key_tiles(const WinParams& p, int l0, int queries, int keys) {
   WtTiles r{0, 0, 0};
@@ -242,13 +241,15 @@ template <int N> struct WtView {
 // The bias of N keys from s0 on for a tile of queries from l0 on: one value where all pairs lie in a side's last bucket.
 struct WtFlat {
   float left, right;
-  int last;                               // where the last bucket starts; no bias: out of reach
+  int last, left_bucket, right_bucket;    // where a side's last bucket starts; the table's columns
   template <typename T> __device__ __forceinline__ WtFlat(const WinParams& p, const T* table, int h) {
-    left = right = 0.f; last = 0;
+    left = right = 0.f; last = left_bucket = right_bucket = 0;
     if (p.buckets.count == 0) return;
     last = p.buckets.first[p.buckets.count - 1];
-    left = win_bias2(to_f32(table[h + (int64_t)p.H * (p.buckets.count - 1)]));
-    right = p.buckets.bidirectional ? win_bias2(to_f32(table[h + (int64_t)p.H * (2 * p.buckets.count - 1)])) : win_bias2(to_f32(table[h]));
+    left_bucket = p.buckets.count - 1;
+    right_bucket = p.buckets.bidirectional ? 2 * p.buckets.count - 1 : win_bucket(p.buckets, 1);     // one-sided: distance 0 for all of them
+    left = win_bias2(to_f32(table[h + (int64_t)p.H * left_bucket]));
+    right = win_bias2(to_f32(table[h + (int64_t)p.H * right_bucket]));
   }
   // low, high: of key - query over the pairs
   __device__ __forceinline__ bool is_left(int high) const { return high <= 0 && -high >= last; }

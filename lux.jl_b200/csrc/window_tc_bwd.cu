@@ -388,8 +388,8 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (biased) {
         const float a = warp_sum(left_sum), c = warp_sum(right_sum);
         if (lane == 0) {
-          my_bsum[w.buckets.count - 1] += a;
-          my_bsum[w.buckets.bidirectional ? 2 * w.buckets.count - 1 : 0] += c;
+          my_bsum[tail.left_bucket] += a;
+          my_bsum[tail.right_bucket] += c;
         }
         bar_group(1, kWtSoft);
         if (st < p.columns) {

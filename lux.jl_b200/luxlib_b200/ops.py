@@ -1049,6 +1049,11 @@ def _check_caches(kcache, vcache, k, v):
         raise DimensionMismatch("kcache and vcache must have the same capacity and batch")
 
 
+def _check_apart(kcache, vcache):
+    if kcache.data_ptr() == vcache.data_ptr() and kcache.numel():
+        raise ArgumentError("kcache and vcache must not be the same array")
+
+
 @functools.lru_cache(maxsize=4096)
 def _step_plan(q, k, v, kcache, vcache, lengths, window, sinks, scale, table, buckets):
     """The checks of a step, as _windowed_plan: (dims, scale, dtype code, device, output shape, whether all arrays are dense)."""
@@ -1079,6 +1084,7 @@ def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, si
     over the caches kcache (D, Hkv, capacity, B...), vcache (E, Hkv, capacity, B...), which take the token in place: position p goes to
     slot p while p < sinks, then to sinks + (p - sinks) mod (capacity - sinks); capacity >= sinks + window. `lengths` (B..., Int32 on
     the device, not changed) counts the tokens before this one; where it is negative there is no sequence: x is zero, the caches stay."""
+    _check_apart(kcache, vcache)
     dims, sc, dt, device, xshape, dense = _step_plan(_meta(q), _meta(k), _meta(v), _meta(kcache), _meta(vcache), _meta(lengths), window, sinks, scale,
                                                      _meta(table), buckets)
     if not dense:
@@ -1096,6 +1102,7 @@ def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     device = _same_device(kcache=_meta(kcache), vcache=_meta(vcache), k=_meta(k), v=_meta(v), lengths=_meta(lengths))
     if k.dim() < 4 or v.dim() != k.dim():
         raise AssertionError("N must be at least 4")
+    _check_apart(kcache, vcache)
     _check_caches(_meta(kcache), _meta(vcache), _meta(k), _meta(v))
     Kx, V = as_colmajor(k), as_colmajor(v)
     if tuple(Kx.shape[1:]) != tuple(V.shape[1:]) or tuple(Kx.shape[3:]) != tuple(kcache.shape[3:]):

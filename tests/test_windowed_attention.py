@@ -86,6 +86,8 @@ B32 = L.RelativeBuckets.make(32, 128, True)
 B32C = L.RelativeBuckets.make(32, 128, False)
 B6 = L.RelativeBuckets.make(6, 20, True)
 B128 = L.RelativeBuckets.make(128, 300, True)
+BD = L.RelativeBuckets((0, 0, 3, 3, 3, 9), False)          # starts that coincide: the earlier buckets are empty
+BDB = L.RelativeBuckets((0, 0, 3, 3, 40), True)
 
 # D, E, H, Hkv, L, S, B, window, sinks, causal, buckets, lengths
 CASES = [
@@ -113,6 +115,8 @@ CASES = [
     (1, 1, 1, 1, 40, 40, 1, 7, 0, True, None, None),
     (64, 64, 8, 1, 140, 140, 1, 60, 0, True, B32C, None),            # eight heads share a key head
     (128, 64, 2, 2, 385, 385, 1, 128, 128, True, B32C, [385]),       # tiles and window on the same boundaries
+    (64, 64, 2, 2, 300, 300, 1, 260, 0, False, BD, None),            # one-sided buckets where keys come after the query too
+    (128, 128, 2, 1, 300, 300, 1, 260, 4, False, BDB, None),
 ]
 
 
@@ -443,7 +447,7 @@ def test_a_step_does_not_read_slots_that_it_does_not_see(dt):
 
 # ---- relative position bias ---------------------------------------------------------------------
 BIAS_CASES = [(1, 1, 1, 1, 0, B6), (197, 197, 3, 2, 0, B32), (64, 130, 2, 1, 0, B32C), (130, 64, 2, 3, 17, B32), (1, 300, 4, 1, -20, B6),
-              (300, 1, 4, 1, 299, B32C), (256, 64, 1, 5, 0, B128), (513, 70, 2, 1, 0, L.RelativeBuckets((0,), False))]
+              (300, 1, 4, 1, 299, B32C), (256, 64, 1, 5, 0, B128), (513, 70, 2, 1, 0, L.RelativeBuckets((0,), False)), (90, 100, 2, 4, 3, BD), (90, 100, 2, 1, -3, BDB)]
 
 
 @pytest.mark.gpu
@@ -613,7 +617,9 @@ def test_refusals_of_the_operators():
         (L.LuxLibB200Error, lambda: L.windowed_attention_step(tq, tk, tk, kc, kc.clone(), lens, window=6, sinks=3)),
         (L.ArgumentError, lambda: L.windowed_attention_step(tq, tk, tk, kc, kc.bfloat16(), lens, window=4)),
         (L.ArgumentError, lambda: L.windowed_attention_step(tq, tk, tk, kc, kc.clone(), lens.long(), window=4)),
-        (L.ArgumentError, lambda: L.windowed_attention_step(tq, tk, tk, kc[:, :, ::2], kc[:, :, ::2], lens, window=4)),
+        (L.ArgumentError, lambda: L.windowed_attention_step(tq, tk, tk, kc[:, :, ::2], kc[:, :, 1::2], lens, window=4)),
+        (L.ArgumentError, lambda: L.windowed_attention_step(tq, tk, tk, kc, kc, lens, window=4)),
+        (L.ArgumentError, lambda: L.windowed_cache_fill(kc, kc, k, k)),
         (L.DimensionMismatch, lambda: L.windowed_attention_step(tq, tk, tk, kc, z(64, 2, 9, 1), lens, window=4)),
         (L.DimensionMismatch, lambda: L.windowed_attention_step(tq, tk, tk, z(64, 2, 8, 2), z(64, 2, 8, 2), lens, window=4)),
         (L.LuxLibB200Error, lambda: L.windowed_cache_fill(kc, kc.clone(), k, k, sinks=8)),
