@@ -225,7 +225,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             bias = at + (kWtTile - 1 - row);
           }
         }
-        ok = ok && mbar_wait_warp(&s_full[grp], made & 1u, p.status, 0x1000u);
+        ok = ok && wt_wait(&s_full[grp], made & 1u, p.status, 0x1000u);
         tc_fence_after();
         // logits = mul * z + add, mul > 0; what a row does not see is -inf
         const bool apart = bias == nullptr && wt_apart(c2, flat);
@@ -305,7 +305,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __nv_bfloat16* xr = static_cast<__nv_bfloat16*>(p.x) + (((int64_t)t.b * w.L + l) * w.H + h) * w.E;
       float o[64 * NB];
       if (begun) {
-        ok = ok && mbar_wait_warp(&pv_done[grp], (made - 1) & 1u, p.status, 0x2000u);
+        ok = ok && wt_wait(&pv_done[grp], (made - 1) & 1u, p.status, 0x2000u);
         tc_fence_after();
         tmem_row64<0>(tO, o);
         if constexpr (NB == 2) tmem_row64<64>(tO + 64, o);

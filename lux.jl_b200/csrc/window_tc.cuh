@@ -220,6 +220,10 @@ __device__ __forceinline__ WtTiles wt_union(const WtTiles& a, const WtTiles& b) 
   return r;
 }
 __device__ __forceinline__ int warp_uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }   // the same in all lanes, and known to be
+// A warp's wait that is mostly over before it begins: one look by all lanes, and lane 0 alone only where that was too early.
+__device__ __forceinline__ bool wt_wait(uint64_t* bar, uint32_t parity, unsigned int* status, unsigned int code) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || mbar_wait_warp(bar, parity, status, code);
+}
 // Where a tile of 128 queries from l0 on stands to `N` keys from s0 on: some row sees some of them; every row sees all of them.
 template <int N> struct WtView {
   int sinks, lo, hi, whole_sinks, whole_lo, whole_hi, whole_end;

@@ -314,7 +314,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             table ^= 1;
           }
         }
-        ok = ok && mbar_wait_warp(&s_full[cur], ((done + (uint32_t)i) >> 1) & 1u, p.status, 0x1000u);
+        ok = ok && wt_wait(&s_full[cur], ((done + (uint32_t)i) >> 1) & 1u, p.status, 0x1000u);
         tc_fence_after();
         const uint32_t tS = tmem + lanes + cur * 128 + half * 64;
         float d[64];
@@ -339,7 +339,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             d[j] = ex2(e0); d[j + 1] = ex2(e1);
           }
         }
-        ok = ok && mbar_wait_warp(dp_full, cur, p.status, 0x2000u);
+        ok = ok && wt_wait(dp_full, cur, p.status, 0x2000u);
         tc_fence_after();
         {
           float e[64];
@@ -404,7 +404,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       float o[32 * NB];
       if (n > 0) {
-        ok = ok && mbar_wait_warp(o_full, turn & 1u, p.status, 0x4000u);
+        ok = ok && wt_wait(o_full, turn & 1u, p.status, 0x4000u);
         ++turn;
         tc_fence_after();
         if constexpr (NB == 2) tmem_row64<0>(tDQ + lanes + half * 64, o);
@@ -614,8 +614,8 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         int to = (s < w.sinks ? queries - 1 : min(queries - 1, s + w.window - 1)) - l0;
         if (s >= keys) to = -1;
         const bool whole = wt_all_seen(w, l0, queries, s0, keys, kWtTile);
-        ok = ok && mbar_wait_warp(&full[2 * qst], ph_q, p.status, 0x8u);       // the columns' stats
-        ok = ok && mbar_wait_warp(s_full, par, p.status, 0x1000u);
+        ok = ok && wt_wait(&full[2 * qst], ph_q, p.status, 0x8u);       // the columns' stats
+        ok = ok && wt_wait(s_full, par, p.status, 0x1000u);
         tc_fence_after();
         float d[64];
         const bool apart = bias == nullptr && wt_apart(c2, flat);
@@ -661,7 +661,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
-        ok = ok && mbar_wait_warp(dp_full, par, p.status, 0x2000u);
+        ok = ok && wt_wait(dp_full, par, p.status, 0x2000u);
         tc_fence_after();
         uint32_t o[32];
         {
@@ -709,7 +709,7 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       done += (uint32_t)n;
       float ak[32 * NB], av[32 * NB];
       if (n > 0) {
-        ok = ok && mbar_wait_warp(o_full, turn & 1u, p.status, 0x4000u);
+        ok = ok && wt_wait(o_full, turn & 1u, p.status, 0x4000u);
         ++turn;
         tc_fence_after();
         if constexpr (NB == 2) {
