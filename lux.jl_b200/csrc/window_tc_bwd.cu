@@ -46,6 +46,10 @@ struct WtBwdParams {
 template <int NB> struct WtBwd {
   static constexpr int TILE = NB * kWtBox;
   static constexpr int STAGES = NB == 1 ? 6 : 4;
+  // dq: the ring's tiles of keys and how far their loads run ahead of the values'. Keys are held until the product that ends a tile,
+  // values only for the one that begins it: 3 + 1 tiles of 128 features, one ahead, 361 us at window 4096 where 2 + 2 took 384; 3 + 3 of
+  // 64 features, in turn, 264 us, one ahead 301
+  static constexpr int KS = 3, AHEAD = NB == 1 ? 0 : 1;
   // dq: bias and bucket of the diagonals (two tiles), diagonal sums of 8 warps, bucket sums of 8 warps; dk, dv: bias, columns' stats
   static constexpr int EXTRA = 2 * 256 * 4 + 2 * 256 + 8 * 4 * 48 * 4 + 8 * 2 * kWinMaxBuckets * 4 + 128 * 4 + kWinMaxBuckets * 4;
   static constexpr int SMEM = (2 + STAGES) * TILE + EXTRA + 256 + 1024;
@@ -186,7 +190,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp < 4) {
     regs_less<kWtBwdFew>();
     if (warp == 0) {
-      uint32_t stage = 0, phase = 0, turn = 0;
+      uint32_t kst = 0, vst = 0, ph_k = 0, ph_v = 0, turn = 0;
       bool ok = true;
       for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
         const WtQueries t(p, item);
@@ -200,16 +204,22 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int x = 0; x < p.boxes_e; ++x) tma_load_4d(sG + x * kWtBox, &tmG, x * 64, t.h, t.l0, t.b, q_full);
         }
         __syncwarp();
-        for (int i = 0; i < 2 * n; ++i) {
-          if (!mbar_wait_uniform(&empty[stage], phase ^ 1u, p.status, 0x100u)) { ok = false; break; }
-          if (elect_one()) {
-            const bool is_k = (i & 1) == 0;
-            const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = t.own.at(i >> 1) * kWtTile;
-            mbar_expect_tx(&full[stage], (uint32_t)(boxes * kWtBox));
-            for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + stage * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, t.h / w.rep, s0, t.b, &full[stage]);
+        for (int i = 0; i < n + C::AHEAD && ok; ++i) {
+          for (int which = 0; which < 2; ++which) {
+            const bool is_k = which == 0;
+            const int tile = is_k ? i : i - C::AHEAD;
+            if (tile < 0 || tile >= n) continue;
+            const uint32_t slot = is_k ? kst : C::KS + vst;
+            if (!mbar_wait_uniform(&empty[slot], (is_k ? ph_k : ph_v) ^ 1u, p.status, 0x100u)) { ok = false; break; }
+            if (elect_one()) {
+              const int boxes = is_k ? p.boxes_d : p.boxes_e, s0 = t.own.at(tile) * kWtTile;
+              mbar_expect_tx(&full[slot], (uint32_t)(boxes * kWtBox));
+              for (int x = 0; x < boxes; ++x) tma_load_4d(sKV + slot * C::TILE + x * kWtBox, is_k ? &tmK : &tmV, x * 64, t.h / w.rep, s0, t.b, &full[slot]);
+            }
+            __syncwarp();
+            if (is_k) { if (++kst == C::KS) { kst = 0; ph_k ^= 1u; } }
+            else if (++vst == C::STAGES - C::KS) { vst = 0; ph_v ^= 1u; }
           }
-          __syncwarp();
-          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
     } else if (warp == 1) {
@@ -223,9 +233,9 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         uint32_t kprev = 0;                                                // where tile i's keys are
         for (int i = -1; i < n; ++i) {
           const bool next = i + 1 < n;
-          const uint32_t cur = (done + (uint32_t)i) & 1u, nxt = cur ^ 1u, k = sKV + 2 * kst * C::TILE, v = sKV + (2 * vst + 1) * C::TILE;
+          const uint32_t cur = (done + (uint32_t)i) & 1u, nxt = cur ^ 1u, k = sKV + kst * C::TILE, v = sKV + (C::KS + vst) * C::TILE;
           if (next) {
-            if (!mbar_wait_uniform(&full[2 * kst], ph_k, p.status, 0x400u)) { ok = false; break; }
+            if (!mbar_wait_uniform(&full[kst], ph_k, p.status, 0x400u)) { ok = false; break; }
             tc_fence_after();
             if (elect_one()) {
               if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem + nxt * 128, sQ, k);
@@ -239,29 +249,29 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
             tc_fence_after();
           }
-          if (next && !mbar_wait_uniform(&full[2 * vst + 1], ph_v, p.status, 0x400u)) { ok = false; break; }
+          if (next && !mbar_wait_uniform(&full[C::KS + vst], ph_v, p.status, 0x400u)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
             if (next) {
               if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, v);
               else wt_mma_features<1>(tDP, sG, v);
               umma_commit(dp_full);
-              umma_commit(&empty[2 * vst + 1]);
+              umma_commit(&empty[C::KS + vst]);
               if (i + 2 == n) umma_commit(q_empty);
             }
             if (i >= 0) {
-              const uint32_t kc = sKV + 2 * kprev * C::TILE;
+              const uint32_t kc = sKV + kprev * C::TILE;
               if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDQ, tmem + cur * 128, kc, i > 0);
               else wt_mma_tokens_halves<1>(tDQ, tmem + cur * 128, kc, i > 0);
-              umma_commit(&empty[2 * kprev]);
+              umma_commit(&empty[kprev]);
               if (!next) umma_commit(o_full);
             }
           }
           __syncwarp();
           kprev = kst;
           if (next) {
-            if (++kst == C::STAGES / 2) { kst = 0; ph_k ^= 1u; }
-            if (++vst == C::STAGES / 2) { vst = 0; ph_v ^= 1u; }
+            if (++kst == C::KS) { kst = 0; ph_k ^= 1u; }
+            if (++vst == C::STAGES - C::KS) { vst = 0; ph_v ^= 1u; }
           }
         }
         ++turn;
