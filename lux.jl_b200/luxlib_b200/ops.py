@@ -969,6 +969,20 @@ def _dense(meta) -> bool:
     return all(s == x or d == 1 for s, x, d in zip(meta[1], colmajor_strides(meta[0]), meta[0])) or 0 in meta[0]
 
 
+def _lengths(lengths):
+    """Numbers of tokens as the library takes them: Int32, one past its range as its largest value."""
+    if lengths is None or lengths.dtype == torch.int32:
+        return None if lengths is None else as_colmajor(lengths)
+    if lengths.dtype not in (torch.int64, torch.int16, torch.int8, torch.uint8):
+        raise ArgumentError(f"lengths must hold whole numbers, not {lengths.dtype}")
+    return as_colmajor((lengths.clamp(-1, 2 ** 31 - 1) if lengths.dtype == torch.int64 else lengths).to(torch.int32))
+
+
+def _number(scale):
+    """A plain number: plans are kept by their arguments' values, and an array's may change."""
+    return None if scale is None else float(scale)
+
+
 @functools.lru_cache(maxsize=4096)
 def _windowed_plan(q, k, v, window, sinks, is_causal, scale, table, buckets, lengths):
     """The checks of a windowed attention call, which the arrays' shapes, types and devices decide, once per set of them:
@@ -987,8 +1001,8 @@ def _windowed_plan(q, k, v, window, sinks, is_causal, scale, table, buckets, len
     if lengths is not None and math.prod(lengths[0]) != Bn:
         raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {math.prod(lengths[0])}")
     _check_table(table, buckets, H)
-    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
-    dims = _cabi.WindowDims(D, E, H, Hkv, Lq, S, Bn, int(window), int(sinks), int(bool(is_causal)))
+    sc = 1.0 / (scale if scale is not None else float(D) ** 0.5)
+    dims = _cabi.WindowDims(D, E, H, Hkv, Lq, S, Bn, window, sinks, int(is_causal))
     return dims, sc, dtype_code(q[2]), device, (E, H, Lq) + batch_shape
 
 
@@ -996,10 +1010,10 @@ def _windowed_attention(q, k, v, window, sinks, is_causal, scale, table, buckets
     if q.dim() < 4 or k.dim() != q.dim() or v.dim() != q.dim():
         raise AssertionError("N must be at least 4")
     q, k, v, table = _promote(q, k, v, table)
-    dims, sc, dt, device, xshape = _windowed_plan(_meta(q), _meta(k), _meta(v), window, sinks, is_causal, scale, _meta(table), buckets, _meta(lengths))
+    dims, sc, dt, device, xshape = _windowed_plan(_meta(q), _meta(k), _meta(v), int(window), int(sinks), bool(is_causal), _number(scale), _meta(table), buckets,
+                                                  _meta(lengths))
     Q, Kx, V = as_colmajor(q), as_colmajor(k), as_colmajor(v)
-    if lengths is not None:
-        lengths = as_colmajor(lengths.to(torch.int32))
+    lengths = _lengths(lengths)
     Tb, plan = _table_of(table, buckets)
     out = jl_empty(xshape, Q.dtype, device)
     stats = torch.empty(2 * dims.queries * dims.heads * dims.batch, dtype=torch.float32, device=device) if want_stats else None
@@ -1050,8 +1064,9 @@ def _check_caches(kcache, vcache, k, v):
 
 
 def _check_apart(kcache, vcache):
-    if kcache.data_ptr() == vcache.data_ptr() and kcache.numel():
-        raise ArgumentError("kcache and vcache must not be the same array")
+    a, b = kcache.data_ptr(), vcache.data_ptr()
+    if a < b + vcache.nbytes and b < a + kcache.nbytes:
+        raise ArgumentError("kcache and vcache must not share memory")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1074,8 +1089,8 @@ def _step_plan(q, k, v, kcache, vcache, lengths, window, sinks, scale, table, bu
     if lengths[2] != torch.int32 or math.prod(lengths[0]) != Bn:
         raise ArgumentError(f"lengths must hold one Int32 per sample ({Bn})")
     _check_table(table, buckets, H)
-    sc = 1.0 / (float(scale) if scale is not None else float(D) ** 0.5)
-    dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache[0][2], Bn, int(window), int(sinks), 1)
+    sc = 1.0 / (scale if scale is not None else float(D) ** 0.5)
+    dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache[0][2], Bn, window, sinks, 1)
     return dims, sc, dtype_code(q[2]), device, (E, H) + batch_shape, all(_dense(m) for m in (q, k, v, lengths, table) if m is not None)
 
 
@@ -1085,8 +1100,8 @@ def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, si
     slot p while p < sinks, then to sinks + (p - sinks) mod (capacity - sinks); capacity >= sinks + window. `lengths` (B..., Int32 on
     the device, not changed) counts the tokens before this one; where it is negative there is no sequence: x is zero, the caches stay."""
     _check_apart(kcache, vcache)
-    dims, sc, dt, device, xshape, dense = _step_plan(_meta(q), _meta(k), _meta(v), _meta(kcache), _meta(vcache), _meta(lengths), window, sinks, scale,
-                                                     _meta(table), buckets)
+    dims, sc, dt, device, xshape, dense = _step_plan(_meta(q), _meta(k), _meta(v), _meta(kcache), _meta(vcache), _meta(lengths), int(window), int(sinks),
+                                                     _number(scale), _meta(table), buckets)
     if not dense:
         q, k, v, lengths = (as_colmajor(t) for t in (q, k, v, lengths))
     table, plan = _table_of(table, buckets)
@@ -1099,10 +1114,10 @@ def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, si
 def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     """Puts a prompt k (D, Hkv, S, B...), v (E, Hkv, S, B...) into the caches of windowed_attention_step, as if its tokens had come one by
     one; `lengths` (B...) as in windowed_attention. The slots that hold none of them stay as they are."""
+    _check_apart(kcache, vcache)
     device = _same_device(kcache=_meta(kcache), vcache=_meta(vcache), k=_meta(k), v=_meta(v), lengths=_meta(lengths))
     if k.dim() < 4 or v.dim() != k.dim():
         raise AssertionError("N must be at least 4")
-    _check_apart(kcache, vcache)
     _check_caches(_meta(kcache), _meta(vcache), _meta(k), _meta(v))
     Kx, V = as_colmajor(k), as_colmajor(v)
     if tuple(Kx.shape[1:]) != tuple(V.shape[1:]) or tuple(Kx.shape[3:]) != tuple(kcache.shape[3:]):
@@ -1111,7 +1126,7 @@ def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     if lengths is not None:
         if lengths.numel() != Bn:
             raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {lengths.numel()}")
-        lengths = as_colmajor(lengths.to(torch.int32))
+        lengths = _lengths(lengths)
     dims = _cabi.WindowDims(Kx.shape[0], V.shape[0], 0, Kx.shape[1], 0, Kx.shape[2], Bn, 1, int(sinks), 1)
     _launch(device, "lb2_window_cache_fill", ptr(kcache), ptr(vcache), ptr(Kx), ptr(V), ptr(lengths), kcache.shape[2], C.byref(dims),
             dtype_code(Kx.dtype))

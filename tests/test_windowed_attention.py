@@ -587,6 +587,40 @@ def test_status_codes_of_the_windowed_entry_points():
     assert lib.lb2_relpos_bias_bwd(None, one, _buckets(), 4, 4, 2, 1, 0, 0, one, 1 << 20, None) == _cabi.BAD_ARG
 
 
+def test_caches_that_overlap_are_refused():
+    z = lambda *s: L.jl_zeros(s, torch.float32, "cpu")
+    both = torch.zeros(3 * 8 * 2 * 4)
+    cache = lambda at: L.arrays.jl_reshape(both[at:at + 64], (8, 2, 4, 1))
+    for a, b in ((0, 0), (0, 32), (63, 0), (32, 16)):
+        with pytest.raises(L.ArgumentError, match="share memory"):
+            L.windowed_attention_step(z(8, 2, 1), z(8, 2, 1), z(8, 2, 1), cache(a), cache(b), torch.zeros(1, dtype=torch.int32), window=2)
+        with pytest.raises(L.ArgumentError, match="share memory"):
+            L.windowed_cache_fill(cache(a), cache(b), z(8, 2, 4, 1), z(8, 2, 4, 1))
+    with pytest.raises(L.ArgumentError, match="CUDA"):                             # side by side: refused for the device alone
+        L.windowed_attention_step(z(8, 2, 1), z(8, 2, 1), z(8, 2, 1), cache(0), cache(64), torch.zeros(1, dtype=torch.int32), window=2)
+
+
+@pytest.mark.gpu
+def test_lengths_of_every_whole_type_and_a_scale_in_an_array():
+    """Int64 lengths past 2^31 are not taken modulo 2^32, fractions are refused; a scale held in an array may change between calls."""
+    a = make(31, "f32", 32, 32, 2, 1, 40, 40, 3)
+    q, k, v = (dev(a[n], "f32") for n in "qkv")
+    run = lambda lens, scale=None: host(L.windowed_attention(q, k, v, window=9, lengths=lens, scale=scale))
+    lens = lambda n, t: torch.tensor(n, dtype=t, device="cuda")
+    for t in (torch.int64, torch.int16, torch.int8, torch.uint8):
+        assert np.array_equal(run(lens([40, 7, 0], t)), run(lens([40, 7, 0], torch.int32))), t
+    assert np.array_equal(run(lens([2 ** 32, 2 ** 31, -2 ** 40], torch.int64)), run(lens([40, 40, 0], torch.int32)))
+    for t in (torch.float32, torch.bool):
+        with pytest.raises(L.ArgumentError):
+            run(lens([1, 1, 0], t))
+        with pytest.raises(L.ArgumentError):
+            L.windowed_cache_fill(L.jl_zeros((32, 1, 9, 3), torch.float32, "cuda"), L.jl_zeros((32, 1, 9, 3), torch.float32, "cuda"), k, v, lens([1, 1, 0], t))
+    scale = torch.tensor(4.0)
+    first = run(None, scale)
+    scale.fill_(2.0)
+    assert np.array_equal(first, run(None, 4.0)) and np.array_equal(run(None, scale), run(None, 2.0))
+
+
 @pytest.mark.gpu
 def test_refusals_of_the_operators():
     z = lambda *s, t=torch.float32: L.jl_zeros(s, t, "cuda")
