@@ -249,25 +249,31 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
             tc_fence_after();
           }
-          if (next && !mbar_wait_uniform(&full[C::KS + vst], ph_v, p.status, 0x400u)) { ok = false; break; }
-          tc_fence_after();
-          if (elect_one()) {
-            if (next) {
-              if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, v);
-              else wt_mma_features<1>(tDP, sG, v);
-              umma_commit(dp_full);
-              umma_commit(&empty[C::KS + vst]);
-              if (i + 2 == n) umma_commit(q_empty);
-            }
-            if (i >= 0) {
+          const auto product_dq = [&] {
+            if (i < 0) return;
+            if (elect_one()) {
               const uint32_t kc = sKV + kprev * C::TILE;
               if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDQ, tmem + cur * 128, kc, i > 0);
               else wt_mma_tokens_halves<1>(tDQ, tmem + cur * 128, kc, i > 0);
               umma_commit(&empty[kprev]);
               if (!next) umma_commit(o_full);
             }
+            __syncwarp();
+          };
+          if (NB == 2) product_dq();
+          if (next) {
+            if (!mbar_wait_uniform(&full[C::KS + vst], ph_v, p.status, 0x400u)) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+              if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sG, v);
+              else wt_mma_features<1>(tDP, sG, v);
+              umma_commit(dp_full);
+              umma_commit(&empty[C::KS + vst]);
+              if (i + 2 == n) umma_commit(q_empty);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (NB == 1) product_dq();
           kprev = kst;
           if (next) {
             if (++kst == C::KS) { kst = 0; ph_k ^= 1u; }
