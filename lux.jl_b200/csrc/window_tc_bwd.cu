@@ -548,37 +548,37 @@ win_tc_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const uint32_t qn = sQG + 2 * qst * C::TILE, gn = sQG + (2 * gst + 1) * C::TILE, qc = sQG + 2 * qprev * C::TILE, gc = sQG + (2 * gprev + 1) * C::TILE;
           if (i >= 0 && !mbar_wait_uniform(p_ready, par, p.status, 0x800u)) { ok = false; break; }
           if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
+          tc_fence_after();
+          if (i >= 0 && elect_one()) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, gc, i > 0);
+            else wt_mma_tokens_halves<1>(tDV, tmem, gc, i > 0);
+            umma_commit(&empty[2 * gprev + 1]);
+          }
+          __syncwarp();
           if (next && !mbar_wait_uniform(&full[2 * qst], ph_q, p.status, 0x400u)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
-            if (i >= 0) {
-              if (NB == 2 && p.boxes_e == 2) wt_mma_tokens_halves<NB>(tDV, tmem, gc, i > 0);
-              else wt_mma_tokens_halves<1>(tDV, tmem, gc, i > 0);
-              umma_commit(&empty[2 * gprev + 1]);
-            }
-            if (next) {
-              if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, qn);
-              else wt_mma_features<1>(tmem, sK, qn);
-              umma_commit(s_full);
-            }
+          if (next && elect_one()) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_features<NB>(tmem, sK, qn);
+            else wt_mma_features<1>(tmem, sK, qn);
+            umma_commit(s_full);
           }
           __syncwarp();
           if (i >= 0 && !mbar_wait_uniform(ds_ready, par, p.status, 0x8000u)) { ok = false; break; }
+          tc_fence_after();
+          if (i >= 0 && elect_one()) {
+            if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, qc, i > 0);
+            else wt_mma_tokens_halves<1>(tDK, tDP, qc, i > 0);
+            umma_commit(&empty[2 * qprev]);
+            if (!next) umma_commit(o_full);
+          }
+          __syncwarp();
           if (next && !mbar_wait_uniform(&full[2 * gst + 1], ph_g, p.status, 0x400u)) { ok = false; break; }
           tc_fence_after();
-          if (elect_one()) {
-            if (i >= 0) {
-              if (NB == 2 && p.boxes_d == 2) wt_mma_tokens_halves<NB>(tDK, tDP, qc, i > 0);
-              else wt_mma_tokens_halves<1>(tDK, tDP, qc, i > 0);
-              umma_commit(&empty[2 * qprev]);
-              if (!next) umma_commit(o_full);
-            }
-            if (next) {
-              if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, gn);
-              else wt_mma_features<1>(tDP, sV, gn);
-              umma_commit(dp_full);
-              if (i + 2 == n) umma_commit(k_empty);
-            }
+          if (next && elect_one()) {
+            if (NB == 2 && p.boxes_e == 2) wt_mma_features<NB>(tDP, sV, gn);
+            else wt_mma_features<1>(tDP, sV, gn);
+            umma_commit(dp_full);
+            if (i + 2 == n) umma_commit(k_empty);
           }
           __syncwarp();
           qprev = qst; gprev = gst;
