@@ -3,18 +3,19 @@
 // A block owns two tiles of 128 queries that read the same keys: the tiles of two heads that share a key head, or two
 // neighbouring tiles of one head; each has its softmax group of four warps, a thread per row.
 // Per tile of 128 keys: S = Q K' into TMEM, the group turns S into weights 2^(z2 - m2), which go back to TMEM as bf16 over S,
-// O += P V with P taken from TMEM. While one group is in its softmax the tensor cores work for the other. O is rescaled only when a row's maximum has grown by more than 2^8 (the reference m2 may lag behind
-// the maximum by that: weights up to 256 are as exact in bf16 as weights up to 1).
+// O += P V with P taken from TMEM. While one group is in its softmax the tensor cores work for the other. O is rescaled only when
+// a row's maximum has grown by more than 2^8 (the reference m2 may lag behind the maximum by that: weights up to 256 are as exact in
+// bf16 as weights up to 1).
 //
 // Blocks stay on their SM and take pairs of tiles in turn: the next pair's Q and keys are loaded, and its first logits formed, while
 // the groups finish and store this one's.
 //
-// Measured: 32 heads on 8, 128 features, 16384 tokens, window 4096: 1.10 ms, 870 TFLOP/s of the visible pairs (0.53 of the GEMM rate);
-// 8192 tokens, window 1024, bias: 233 us. What bounds it: a group's chain per tile, 4300 cycles: its products 1300 (1024 of MMA time at
-// full rate; S from shared memory takes all of its 128 bytes per cycle), reading S 440, maximum 590, exponentials 1350 (the
-// 16 per cycle and SM), storing and signalling 700; the other group's fills the same time.
+// Measured: 32 heads on 8, 128 features, 16384 tokens, window 4096: 1.06 ms, 909 TFLOP/s of the visible pairs (0.55 of the GEMM rate);
+// 8192 tokens, window 1024, bias: 226 us. What bounds it: a group's chain per tile, 3780 cycles by the SM's clock: from its signal to
+// the next logits 1600 (1024 of MMA time at full rate; S from shared memory takes all of its 128 bytes per cycle), reading S 140,
+// maximum 560, exponentials 1370 (the 16 per cycle and SM), storing 130; the other group's fills the same time.
 // A third of the chain would go if the next S were formed during the softmax, but 512 TMEM columns hold two S and two O and no more;
-// 64 keys at a time with two S each were slower (303 against 262 us at window 4096): S at N = 64 is bound by its shared-memory reads.
+// 64 keys at a time with two S each were slower (303 against 262 us at 8192 tokens, 16 heads, window 4096; the kernel as it is takes 237): S at N = 64 is bound by its shared-memory reads.
 //
 // TMEM columns: S0 | S1 | O0 | O1, 128 each. Shared memory: both tiles of Q, a ring of key and value tiles in turn.
 #include "common.cuh"

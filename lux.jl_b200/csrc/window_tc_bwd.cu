@@ -8,11 +8,14 @@
 // already (tokens as the contraction). Two warpgroups share the exponentials of a tile.
 //
 // The weights of the logits' gradient are rounded to bf16 for dq and dk, as the weights are for dv: with the result's own rounding that leaves
-// 0.0024 of the result, where a result rounded once has 0.0017.
+// 0.0024 of the result, where a result rounded once has 0.0017. The table's gradient sums them unrounded; where one bucket holds nearly all
+// of the rows' weight its sum cancels (a row's logit gradients sum to zero) and is as good as the magnitude of its terms, not its own.
 //
-// Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 42 us (201 MB), dq 350 us, dk dv 370 us.
-// What bounds them: a tile's chain through the softmax warps, 3800 cycles each, and in dk dv the shared-memory bytes that the four
-// products and the loads take (2300 cycles a tile at 128 bytes per cycle).
+// Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 42 us (201 MB), dq 312 us, dk dv 356 us.
+// What bounds them: in dq a tile's chain through the softmax warps (weights 1140 cycles, their gradients 650, the signals and waits between
+// 700) and at 128 features the values, whose one place in shared memory is free only after the product before; in dk dv, whose four
+// accumulators leave TMEM no second S, weights and products take turns, and the products and loads take 2300 cycles a tile of
+// shared memory at 128 bytes per cycle.
 //
 // The bias table's gradient: sums of dS (fp32) by bucket. A tile of one bucket is summed in registers; in the others each warp adds
 // along its diagonals with shuffles, then joins neighbouring diagonals of a bucket; per-warp sums, fixed order.
@@ -47,7 +50,7 @@ template <int NB> struct WtBwd {
   static constexpr int TILE = NB * kWtBox;
   static constexpr int STAGES = NB == 1 ? 6 : 4;
   // dq: the ring's tiles of keys and how far their loads run ahead of the values'. Keys are held until the product that ends a tile,
-  // values only for the one that begins it: 3 + 1 tiles of 128 features, one ahead, 361 us at window 4096 where 2 + 2 took 384; 3 + 3 of
+  // values only for the one that begins it: 3 + 1 tiles of 128 features, one ahead, 361 us at window 4096 where 2 + 2 took 384 (before the product order below); 3 + 3 of
   // 64 features, in turn, 264 us, one ahead 301
   static constexpr int KS = 3, AHEAD = NB == 1 ? 0 : 1;
   // dq: bias and bucket of the diagonals (two tiles), diagonal sums of 8 warps, bucket sums of 8 warps; dk, dv: bias, columns' stats
@@ -249,6 +252,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
             tc_fence_after();
           }
+          // 128 features wait for their one tile of values here: the product with the finished tile first (361 -> 303 us at window 4096)
           const auto product_dq = [&] {
             if (i < 0) return;
             if (elect_one()) {
