@@ -27,9 +27,10 @@ inline bool wt_encode(CUtensorMap* map, const void* ptr, int64_t features, int64
 }
 
 // Blocks for `items`, each of about `steps` tiles: one per SM that takes its items in turn, or one per item, which the device hands out as
-// SMs come free. Taking them in turn saves some 8 us an item (start, first loads, last stores); the other way saves about half an
-// item (2.2 us a step) where they do not come out even. Measured at 16 heads, 8192 tokens, 128 features, dk dv on 4 key heads:
-// 3.5 items an SM: 9 steps 117 us in turn, 121 as they come, 33 steps 287 and 262; 1.7 items of 36 steps 179 and 169.
+// SMs come free. Taking them in turn saves some 3 us an item (start, first loads, last stores); the other way saves about half an
+// item (2 us a step) where they do not come out even. Measured at 16 heads on 4, 8192 tokens, 128 features, in turn and as they come:
+// forward, 3.5 items an SM of 9 steps 108 and 117 us, of 33 steps 270 and 237; dq, 6.9 items of 2 steps 50 and 71, of 33 steps 305
+// and 296 (the rule's side is the slower one by 3 %); dk dv, 1.7 items of 36 steps 168 and 171, of 132 steps 477 and 449.
 inline unsigned wt_blocks(int items, int sms, int64_t steps) { return (unsigned)(items <= sms || (int64_t)items * 7 > steps * sms ? std::min(items, sms) : items); }
 
 // Shared-memory descriptors of a tile of 128 tokens in boxes: features as the contraction (K-major: 32 bytes per step of 16, the
