@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
   const uint32_t ring = smem_u32(raw) + warp * Ring::WARP;
   const int piece = lane % CPR, first_row = lane / CPR;
   const bool kreal = piece * 8 < p.D, vreal = piece * 8 < p.E;
-  // 16 keys from i0 on; past the end the last key once more, which weighs nothing there
+  // 16 keys from i0 on; past the end the last key once more, which weighs nothing there, and zeros for its value, which may be infinite
   auto fetch = [&](int i0, int stage) {
     if (i0 < to) {
 #pragma unroll
@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
         const int64_t slot = keys.slot(i);
         const uint32_t at = ring + stage * Ring::STAGE + row * (DC * 2);
         copy_async16(at + ((piece ^ ((row & 1) << 2)) * 16), (fresh ? kn : kc + slot * ks) + (kreal ? piece * 8 : 0), kreal);
-        copy_async16(at + Ring::HALF + ((piece ^ (row & 6)) * 16), (fresh ? vn : vc + slot * vs) + (vreal ? piece * 8 : 0), vreal);
+        copy_async16(at + Ring::HALF + ((piece ^ (row & 6)) * 16), (fresh ? vn : vc + slot * vs) + (vreal ? piece * 8 : 0),
+                     vreal && i0 + row < to);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -380,8 +381,10 @@ __global__ void __launch_bounds__(kStepThreads) win_step_f32_kernel(const __grid
       vv[x] = *reinterpret_cast<const float4*>((fresh ? vn : vc + slot * vs) + (c < p.E ? c : 0));
     }
 #pragma unroll
-    for (int x = 0; x < U; ++x)
+    for (int x = 0; x < U; ++x) {
       if (c >= p.D) kv[x] = zero;
+      if (i0 + x * PARTS + part >= to) vv[x] = zero;      // it may be infinite
+    }
     int bk[U];
 #pragma unroll
     for (int x = 0; x < U; ++x) {

@@ -1,0 +1,141 @@
+"""Windowed attention where blocks take many items in turn, where buckets of a row cancel and where the sinks' tiles are shared by blocks,
+against the definition in 64 bits.
+
+Two tolerances. Per element, that of test_windowed_attention.py with the number of terms of that output. Per output, by norm, which a lost
+tile or diagonal does not pass: errors that are independent of each other add up by their squares. Root mean squares, u = 2^-24:
+  a rounding to bf16 is off by half a step of 2^-8 at most and evenly spread: 2^-8 / sqrt(3) of the value. The weights (x, dv, dtable) or the
+  weights and the logits' gradients (dq, dk) are rounded, and each result;
+  a sum of n Float32 terms of random sign: u sqrt(n) of its value; a logit of D products therefore u sqrt(D) times its size, its weight as
+  much of itself, with 16 u for the exponential, the row's sum and the products of a term; BFloat16's exponential: 2^-20;
+  dx . x, which a row's logits share: 4 u sqrt(E), and for BFloat16 2^-17, for its x comes in two parts of 8 bits each.
+Half as much again is allowed (the least outputs have eight entries)."""
+import math
+
+import pytest
+import torch
+
+import luxlib_b200 as L
+from luxlib_b200 import _cabi
+import window_reference as R
+from test_windowed_attention import B6, B32, B32C, DT, U16, U32
+
+NAMES = ("x", "dq", "dk", "dv", "dtable")
+
+
+def norm_limit(dt, name, ref, D, E, n):
+    r16 = U16 / math.sqrt(3) if dt == "bf16" else 0.0
+    r32 = U32 * (math.sqrt(D) + 16) * (ref["zrms"] + 1) + (2.0 ** -20 if dt == "bf16" else 0.0)
+    terms, value = float(ref[name + "_rms"].norm()), float(ref[name].norm())
+    roundings = 2 if name in ("dq", "dk") else 1
+    lim = r16 * math.sqrt(roundings * terms ** 2 + value ** 2) + r32 * terms + U32 * (math.sqrt(n) + 1) * value
+    if name == "dtable":
+        lim += (4 * U32 * math.sqrt(E) + (2.0 ** -17 if dt == "bf16" else 0.0)) * float(ref["dtable_row"].norm())
+    return 1.5 * lim
+
+
+def element_limit(dt, name, ref, D, E, n):
+    rel = U32 * (2 * (D + 4) * (ref["zmax"] + 1) + 2 * E + n + 32)
+    if dt == "bf16":
+        rel += 2.0 ** -20 + 2.0 ** -16 + U16 * 3
+    return rel * ref[name + "_mag"] + 1e-35
+
+
+def close(got, ref, dt, D, E, terms, names=NAMES, where=None):
+    """`where`: name -> mask of the entries that are compared."""
+    for name in names:
+        if name not in ref:
+            continue
+        g, r = got[name].double(), ref[name]
+        assert g.shape == r.shape, name
+        mask = torch.ones_like(r, dtype=torch.bool) if where is None or name not in where else where[name]
+        err = torch.where(mask, (g - r).abs(), 0.0)
+        assert torch.isfinite(err).all(), f"{name}: not finite at {(~torch.isfinite(err)).nonzero()[0].tolist()}"
+        over = err > element_limit(dt, name, ref, D, E, terms[name])
+        assert not over.any(), f"{name}: {int(over.sum())} entries off, first at {over.nonzero()[0].tolist()}"
+        lim = norm_limit(dt, name, ref, D, E, terms[name])
+        assert float(err.norm()) <= lim, f"{name}: off by {float(err.norm()):.3e}, {float(err.norm()) / lim:.2f} times the limit"
+
+
+# ---- single tokens -------------------------------------------------------------------------------
+def step_inputs(seed, dt, D, E, H, Hkv, B, cap, columns):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*reversed(s), generator=g).to(DT[dt]).cuda().permute(*reversed(range(len(s))))
+    t = {"q": r(D, H, B), "k": r(D, Hkv, B), "v": r(E, Hkv, B), "kc": r(D, Hkv, cap, B), "vc": r(E, Hkv, cap, B)}
+    if columns:
+        t["table"] = r(H, columns)
+    return t
+
+
+def slot(p, sinks, cap):
+    return p if p < sinks else sinks + (p - sinks) % (cap - sinks)
+
+
+def step_reference(t, lens, window, sinks, buckets):
+    """x, its measures, and the caches afterwards, in 64 bits."""
+    d = {n: x.double().clone() for n, x in t.items()}
+    D, H, B = d["q"].shape
+    E, Hkv, cap = d["vc"].shape[:3]
+    out = {n: torch.zeros(E, H, B, dtype=torch.float64, device="cuda") for n in ("x", "x_mag", "x_rms")}
+    out["zmax"], squares, pairs = 0.0, 0.0, 0
+    for b, n in enumerate(lens):
+        d["kc"][:, :, slot(n, sinks, cap), b], d["vc"][:, :, slot(n, sinks, cap), b] = d["k"][:, :, b], d["v"][:, :, b]
+        pos = list(range(max(0, n - window + 1), n + 1))
+        pos = list(range(min(sinks, pos[0]))) + pos
+        at = torch.tensor([slot(p, sinks, cap) for p in pos], device="cuda")
+        for h in range(H):
+            kk, vv, qq = d["kc"][:, h * Hkv // H, at, b], d["vc"][:, h * Hkv // H, at, b], d["q"][:, h, b]
+            z, zm = qq @ kk / D ** 0.5, qq.abs() @ kk.abs() / D ** 0.5
+            if buckets is not None:
+                bias = d["table"][h, torch.tensor([buckets.bucket(p - n) for p in pos], device="cuda")]
+                z, zm = z + bias, zm + bias.abs()
+            out["zmax"] = max(out["zmax"], float(zm.max()))
+            squares, pairs = squares + float((z ** 2).sum()), pairs + z.numel()
+            p = torch.softmax(z, 0)
+            out["x"][:, h, b], out["x_mag"][:, h, b], out["x_rms"][:, h, b] = vv @ p, vv.abs() @ p, vv ** 2 @ p ** 2
+    out["x_rms"], out["zrms"] = out["x_rms"].sqrt(), (squares / pairs) ** 0.5
+    return out, d["kc"], d["vc"]
+
+
+def step(t, lens, window, sinks, buckets):
+    x = L.windowed_attention_step(t["q"], t["k"], t["v"], t["kc"], t["vc"], torch.tensor(lens, dtype=torch.int32, device="cuda"), window=window,
+                                  sinks=sinks, table=t.get("table"), buckets=buckets)
+    torch.cuda.synchronize()
+    return x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128, 40, 24])
+@pytest.mark.parametrize("rep,Hkv,window,sinks,buckets", [(3, 2, 37, 0, None), (5, 2, 60, 3, B32C), (9, 1, 200, 4, None), (12, 2, 1300, 4, B32C), (16, 1, 64, 1, None),
+                                                         (20, 2, 150, 2, B32C), (33, 1, 1100, 0, None)])
+def test_steps_of_many_query_heads_per_key_head(dt, D, rep, Hkv, window, sinks, buckets):
+    cap = window + sinks + 5
+    t = step_inputs(46, dt, D, D, rep * Hkv, Hkv, 3, cap, len(buckets) if buckets else 0)
+    lens = [3 * cap + 1, window // 2, 0]
+    ref, kc, vc = step_reference(t, lens, window, sinks, buckets)
+    got = step(t, lens, window, sinks, buckets)
+    close({"x": got}, ref, dt, D, D, {"x": window + sinks}, names=("x",))
+    assert torch.equal(t["kc"].double(), kc) and torch.equal(t["vc"].double(), vc)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D,rep", [(64, 2), (128, 1), (128, 12), (32, 5), (33, 2)])
+@pytest.mark.parametrize("window", [21, 600])
+def test_an_infinite_value_that_a_step_sees(dt, D, rep, window):
+    """One infinite feature of one key: that feature of x is infinite, the others are as without it, whichever key it is."""
+    sinks, cap, n = 2, window + 9, 3 * window
+    clean = step_inputs(47, dt, D, D, 2 * rep, 2, 1, cap, 0)
+    ref, _, _ = step_reference(clean, [n], window, sinks, None)
+    seen = list(range(sinks)) + list(range(n - window + 1, n + 1))
+    for p in seen if window < 100 else seen[::37] + seen[-17:]:
+        t = {m: x.clone(memory_format=torch.preserve_format) for m, x in clean.items()}
+        if p == n:
+            t["v"][5, 1, 0] = -math.inf
+        else:
+            t["vc"][5, 1, slot(p, sinks, cap), 0] = -math.inf
+        got = step(t, [n], window, sinks, None)
+        assert (got[5, rep:] == -math.inf).all(), p
+        where = torch.ones_like(ref["x"], dtype=torch.bool)
+        where[5, rep:] = False
+        close({"x": got}, ref, dt, D, D, {"x": window + sinks}, names=("x",), where={"x": where})
