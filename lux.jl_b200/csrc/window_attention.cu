@@ -673,9 +673,16 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   int32_t rc = win_check(d, buckets, table, lengths, dtype);
   if (rc != LB2_OK) return rc;
   const size_t es = dtype_size(dtype);
-  if (win_empty(d)) {                   // no samples: the table's gradient is a sum over nothing
-    if (buckets != nullptr && dtable != nullptr && d->heads > 0)
-      cudaMemsetAsync(dtable, 0, (size_t)(d->heads * win_columns(buckets)) * es, static_cast<cudaStream_t>(stream));
+  if (win_empty(d)) {                   // no samples or no query heads: the gradients are sums over nothing
+    const int64_t keys = d->kv_heads * d->keys * d->batch;
+    void* at[3] = {dk, dv, dtable};
+    const int64_t count[3] = {keys * d->head_dim, keys * d->value_dim, dtable == nullptr ? 0 : d->heads * win_columns(buckets)};
+    for (int i = 0; i < 3; ++i) {
+      if (count[i] == 0) continue;
+      LB2_REQUIRE(at[i] != nullptr, LB2_BAD_ARG, "null tensor pointer");
+      const cudaError_t e = cudaMemsetAsync(at[i], 0, (size_t)count[i] * es, static_cast<cudaStream_t>(stream));
+      if (e != cudaSuccess) return fail(LB2_LAUNCH_FAIL, "windowed attention: gradients of nothing: %s", cudaGetErrorString(e));
+    }
     return LB2_OK;
   }
   const bool nq = d->queries > 0, nk = d->keys > 0, nd = d->head_dim > 0, ne = d->value_dim > 0;

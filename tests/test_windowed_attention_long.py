@@ -139,3 +139,22 @@ def test_an_infinite_value_that_a_step_sees(dt, D, rep, window):
         where = torch.ones_like(ref["x"], dtype=torch.bool)
         where[5, rep:] = False
         close({"x": got}, ref, dt, D, D, {"x": window + sinks}, names=("x",), where={"x": where})
+
+
+# ---- no query heads ------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_without_query_heads_the_keys_gradients_are_zero(dt):
+    """Sums over nothing, not what the memory held."""
+    lib = _cabi.load()
+    full = lambda *s: L.jl_empty(s, DT[dt], "cuda").fill_(7.0)
+    k, v, dk, dv = full(64, 2, 9, 3), full(32, 2, 9, 3), full(64, 2, 9, 3), full(32, 2, 9, 3)
+    dims = _cabi.WindowDims(64, 32, 0, 2, 9, 9, 3, 4, 1, 1)
+    call = lambda dk, dv: lib.lb2_window_attention_bwd(None, dk, dv, None, None, None, None, None, None, k.data_ptr(), v.data_ptr(), None, None, None, 0.125,
+                                                       dims, L.arrays.dtype_code(DT[dt]), None, 0, L.arrays.current_stream(k.device))
+    assert call(dk.data_ptr(), dv.data_ptr()) == _cabi.OK
+    assert not dk.any() and not dv.any()
+    assert call(None, dv.data_ptr()) == _cabi.BAD_ARG
+    x, pb = L.rrule_windowed_attention(full(64, 0, 9, 3), k, v, window=4)
+    dq, dk, dv, _ = pb(x)
+    assert tuple(x.shape) == (32, 0, 9, 3) and tuple(dq.shape) == (64, 0, 9, 3) and not dk.any() and not dv.any()
