@@ -393,7 +393,8 @@ LB2_API int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dta
  * vcache (value_dim, kv_heads, capacity, batch); position p lies in slot p while p < sinks, then in sinks + (p - sinks) mod
  * (capacity - sinks). capacity >= sinks + window. lengths[b] tokens are in the cache; the new one, at position lengths[b], is put there
  * and attends: q (head_dim, heads, batch), k, v of kv_heads -> x (value_dim, heads, batch). lengths[b] < 0: no sequence in that place,
- * x = 0 and the cache stays. lengths itself is not changed. dims->queries and dims->causal are not read. */
+ * x = 0 and the cache stays. lengths itself is not changed. dims->queries and dims->causal are not read. heads = 0 is refused where there
+ * are key heads. */
 LB2_API int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, const void* q, const void* k, const void* v,
                                           const void* table, const lb2_rel_buckets* buckets, const int32_t* lengths, double scale,
                                           const lb2_window_dims* dims, int32_t dtype, void* stream);

@@ -558,7 +558,8 @@ int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, const voi
   if (rc != LB2_OK) return rc;
   LB2_REQUIRE(d->window >= 1, LB2_BAD_ARG, "the window must hold at least one token");
   LB2_REQUIRE(d->heads == 0 || (d->kv_heads > 0 && d->heads % d->kv_heads == 0), LB2_BAD_SHAPE, "heads must be a multiple of kv_heads");
-  if (d->batch == 0 || d->heads == 0) return LB2_OK;
+  if (d->batch == 0 || d->kv_heads == 0) return LB2_OK;
+  LB2_REQUIRE(d->heads > 0, LB2_BAD_SHAPE, "a step without query heads");       // it would leave the token out of the cache
   LB2_REQUIRE(d->window <= d->keys - d->sinks, LB2_BAD_ARG, "a cache of %lld slots does not hold %lld sinks and a window of %lld", (long long)d->keys,
               (long long)d->sinks, (long long)d->window);
   const size_t es = dtype_size(dtype);

@@ -158,3 +158,11 @@ def test_without_query_heads_the_keys_gradients_are_zero(dt):
     x, pb = L.rrule_windowed_attention(full(64, 0, 9, 3), k, v, window=4)
     dq, dk, dv, _ = pb(x)
     assert tuple(x.shape) == (32, 0, 9, 3) and tuple(dq.shape) == (64, 0, 9, 3) and not dk.any() and not dv.any()
+
+
+def test_a_step_without_query_heads_is_refused():
+    """It has no place for the token's keys and values but the cache, which it would not reach."""
+    lib, one = _cabi.load(), 256
+    step = lambda **kw: lib.lb2_window_attention_step(one, one, one, one, one, one, None, None, one, 0.125, _cabi.WindowDims(*dict(dict(
+        head_dim=64, value_dim=64, heads=0, kv_heads=2, queries=1, keys=9, batch=3, window=4, sinks=1, causal=1), **kw).values()), 0, None)
+    assert step() == _cabi.BAD_SHAPE and step(batch=0) == _cabi.OK and step(kv_heads=0) == _cabi.OK
