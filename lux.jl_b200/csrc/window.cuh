@@ -146,8 +146,9 @@ template <typename T> __device__ __forceinline__ const T* win_kv_row(const WinPa
 
 // stats of a row: the reference m2 that its logits were compared with (their maximum, or a little less) and log2(sum of 2^(z2 - m2)),
 // apart: their sum would lose the second beside an m2 as large as the type's lowest value. A row that sees nothing has (0, inf).
-// rest: x less its rounding, or null
-template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, T* rest, float2* stats, int l, int h, int b, int keys) {
+// rest: x less its rounding, or null. ROUNDED: weights are summed as the
+// tensor-core forward with a bias table sums them, rounded, and m2 grows by whole numbers.
+template <typename T, bool ROUNDED = false> __device__ __noinline__ void win_row_fwd(const WinParams& p, T* x, T* rest, float2* stats, int l, int h, int b, int keys) {
   const int lane = threadIdx.x & 31, g = h / p.rep;
   float q[kWinLaneDims], t[kWinLaneDims], o[kWinLaneDims] = {};
   win_load_lane(win_q_row<T>(p, p.q, p.D, l, h, b), p.D, lane, q);
@@ -159,8 +160,10 @@ template <typename T> __device__ __noinline__ void win_row_fwd(const WinParams& 
     win_load_lane(win_kv_row<T>(p, p.k, p.D, s, g, b), p.D, lane, t);
     float z = win_dot_lane(q, t, p.D) * p.scale2;
     if (p.buckets.count > 0) z += win_bias<T>(p, h, s - l);
-    const float mn = fmaxf(m, z), ref = mn == -INFINITY ? 0.f : mn;
-    const float keep = exp2f(m - ref), w = exp2f(z - ref);
+    const float mn = z > m ? (ROUNDED && z - m < 1024.f ? m + ceilf(z - m) : z) : m, ref = mn == -INFINITY ? 0.f : mn;
+    const float keep = exp2f(m - ref);
+    float w = exp2f(z - ref);
+    if constexpr (ROUNDED) w = __bfloat162float(__float2bfloat16_rn(w));
     win_load_lane(win_kv_row<T>(p, p.v, p.E, s, g, b), p.E, lane, t);
 #pragma unroll
     for (int i = 0; i < kWinLaneDims; ++i) o[i] = fmaf(w, t[i], o[i] * keep);

@@ -5,7 +5,9 @@
 // Per tile of 128 keys: S = Q K' into TMEM, the group turns S into weights 2^(z2 - m2), which go back to TMEM as bf16 over S,
 // O += P V with P taken from TMEM. While one group is in its softmax the tensor cores work for the other. O is rescaled only when
 // a row's maximum has grown by more than 2^8 (the reference m2 may lag behind the maximum by that: weights up to 256 are as exact in
-// bf16 as weights up to 1).
+// bf16 as weights up to 1). With a bias table the sum is that of the rounded weights, and m2 grows by whole numbers, so
+// that rescaling changes no rounding: x is the average over weights that the pullback can form again bit by bit, so that the gradients of
+// a row's logits, summed by bucket, add up to zero as they must.
 //
 // Blocks stay on their SM and take pairs of tiles in turn: the next pair's Q and keys are loaded, and its first logits formed, while
 // the groups finish and store this one's.
@@ -64,7 +66,7 @@ struct WtPair {
   }
 };
 
-template <int NB>
+template <int NB, bool BIASED>
 __global__ void __launch_bounds__(kWtFwdThreads, 1)
 win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ WtFwdParams p) {
@@ -195,7 +197,6 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int grp = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, gt = threadIdx.x - 128 - grp * 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16, tS = tmem + lanes + grp * 128, tO = tmem + lanes + 256 + grp * 128;
     const float c2 = w.scale2;
-    const bool biased = w.buckets.count > 0;
     __nv_bfloat16* rest = static_cast<__nv_bfloat16*>(p.rest);
     bool ok = true, redo = false;                // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
     uint32_t made = 0;                           // steps so far
@@ -212,7 +213,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!view.some(s0)) continue;
         float flat = 0.f;
         const float* bias = nullptr;
-        if (biased) {
+        if constexpr (BIASED) {
           const int low = s0 - l0 - (kWtTile - 1);
           if (tail.is_left(low + 2 * (kWtTile - 1))) {
             flat = tail.left;
@@ -257,8 +258,8 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float mx = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), mul, add);
         const bool grow = mx > m2 + 8.f;
         if (__any_sync(0xffffffffu, grow)) {
-          const float keep = grow ? ex2(m2 - mx) : 1.f;
-          if (grow) { m2 = mx; sum *= keep; }
+          const float to = BIASED && mx - m2 < 1024.f ? m2 + ceilf(mx - m2) : mx, keep = grow ? ex2(m2 - to) : 1.f;     // beyond, nothing of the old weights is left
+          if (grow) { m2 = to; sum *= keep; }
           if (begun) {                           // the logits came after the last product: O is still
 #pragma unroll 1
             for (int q = 0; q < 4 * NB; ++q) {
@@ -274,6 +275,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float ref = m2 == -INFINITY ? 0.f : m2;
         const uint64_t mul_2 = pack2(mul, mul), off_2 = pack2(add - ref, add - ref);
         uint64_t part[2] = {0, 0};
+        float each[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           uint32_t v[32];
@@ -282,12 +284,15 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             float a, c;
             unpack2(fma2(pack2(z[q * 64 + 2 * x], z[q * 64 + 2 * x + 1]), mul_2, off_2), a, c);
             a = ex2(a); c = ex2(c);
-            part[x & 1] = add2(part[x & 1], pack2(a, c));
+            if constexpr (!BIASED) part[x & 1] = add2(part[x & 1], pack2(a, c));
             v[x] = pack_bf16(a, c);
+            if constexpr (BIASED) add_bf16(each[2 * x & 3], each[(2 * x + 1) & 3], v[x]);
           }
           tmem_st32(tS + q * 32, v);
         }
-        {
+        if constexpr (BIASED) {
+          sum += (each[0] + each[1]) + (each[2] + each[3]);
+        } else {
           float a, c;
           unpack2(add2(part[0], part[1]), a, c);
           sum += a + c;
@@ -348,7 +353,7 @@ win_tc_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           for (int e = 0; e < w.E; ++e) bad = bad || !isfinite(__bfloat162float(xr[e]));
         for (uint32_t again = __ballot_sync(0xffffffffu, bad); again != 0; again &= again - 1) {
           const int r = l - lane + __ffs(again) - 1;
-          win_row_fwd<__nv_bfloat16>(w, static_cast<__nv_bfloat16*>(p.x), rest, p.stats != nullptr ? p.stats + ((int64_t)t.b * w.H + h) * w.L + r : nullptr, r, h,
+          win_row_fwd<__nv_bfloat16, BIASED>(w, static_cast<__nv_bfloat16*>(p.x), rest, p.stats != nullptr ? p.stats + ((int64_t)t.b * w.H + h) * w.L + r : nullptr, r, h,
                                      t.b, t.keys);
         }
       }
@@ -396,7 +401,9 @@ int32_t win_tc_fwd(const WinParams& w, void* x, void* rest, float2* stats, cudaS
     LB2_CHECK_LAUNCH("windowed attention");
     return LB2_OK;
   };
-  return p.boxes_d == 1 && p.boxes_e == 1 ? launch(win_tc_fwd_kernel<1>, WtFwd<1>::SMEM) : launch(win_tc_fwd_kernel<2>, WtFwd<2>::SMEM);
+  if (w.buckets.count > 0)
+    return p.boxes_d == 1 && p.boxes_e == 1 ? launch(win_tc_fwd_kernel<1, true>, WtFwd<1>::SMEM) : launch(win_tc_fwd_kernel<2, true>, WtFwd<2>::SMEM);
+  return p.boxes_d == 1 && p.boxes_e == 1 ? launch(win_tc_fwd_kernel<1, false>, WtFwd<1>::SMEM) : launch(win_tc_fwd_kernel<2, false>, WtFwd<2>::SMEM);
 }
 
 }  // namespace lb2

@@ -191,6 +191,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
   return u;
 }
+// lo and hi plus the halves of a pair of bf16, in one mixed-precision instruction each
+__device__ __forceinline__ void add_bf16(float& lo, float& hi, uint32_t pair) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\nadd.rn.f32.bf16 %0, a, %0;\nadd.rn.f32.bf16 %1, b, %1;\n}\n" : "+f"(lo), "+f"(hi) : "r"(pair));
+}
 __device__ __forceinline__ void bar_group(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // The tiles of 128 keys that a tile of queries visits: [0, nsink) and [first, last).

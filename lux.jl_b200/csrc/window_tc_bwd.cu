@@ -8,8 +8,10 @@
 // already (tokens as the contraction). Two warpgroups share the exponentials of a tile.
 //
 // The weights of the logits' gradient are rounded to bf16 for dq and dk, as the weights are for dv: with the result's own rounding that leaves
-// 0.0024 of the result, where a result rounded once has 0.0017. The table's gradient sums them unrounded; where one bucket holds nearly all
-// of the rows' weight its sum cancels (a row's logit gradients sum to zero) and is as good as the magnitude of its terms, not its own.
+// 0.0024 of the result, where a result rounded once has 0.0017. The table's gradient sums them in fp32, from weights rounded as the forward pass rounded
+// them: over a row those add up to nothing, so that a bucket that holds nearly all of a row's weight gets minus the sum of the few others
+// and not what rounding leaves (2 samples of 1100 tokens, window 246, four buckets: error 0.0087 -> 0.0028 of the gradient; all in one
+// bucket: 40 times what dx . x rounds to -> a fifth of it). dq takes 8 % longer for it.
 //
 // Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 42 us (201 MB), dq 312 us, dk dv 356 us.
 // What bounds them: in dq a tile's chain through the softmax warps (weights 1140 cycles, their gradients 650, the signals and waits between
@@ -20,6 +22,7 @@
 // The bias table's gradient: sums of dS (fp32) by bucket. A tile of one bucket is summed in registers; in the others each warp adds
 // along its diagonals with shuffles, then joins neighbouring diagonals of a bucket; per-warp sums, fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "window_tc.cuh"
@@ -149,7 +152,7 @@ __device__ __forceinline__ void wt_diagonals(const float (&d)[64], float* my_dia
 }
 __device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-template <int NB>
+template <int NB, bool BIASED>
 __global__ void __launch_bounds__(kWtBwdThreads, 1)
 win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ WtBwdParams p) {
@@ -293,7 +296,6 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int sw = warp - 4, half = sw >> 2, quarter = warp & 3, row = quarter * 32 + lane, st = threadIdx.x - 128;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const float c2 = w.scale2;
-    const bool biased = w.buckets.count > 0;
     float* my_bsum = bsum + sw * 2 * kWinMaxBuckets;
     float* my_diag = diag + sw * 4 * 48;
     bool ok = true;                     // after a wait that ran out: no more waits, but the same way through, whose barriers all warps share
@@ -306,8 +308,10 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const WtFlat tail(w, static_cast<const __nv_bfloat16*>(w.table), h);
       const float* of_row = p.rows + (((int64_t)t.b * w.H + h) * p.query_tiles + l0 / kWtTile) * 3 * kWtTile + row;
       const float neg_m = of_row[0], neg_l = of_row[kWtTile], neg_d = of_row[2 * kWtTile];
-      const uint64_t nm = pack2(neg_m, neg_m), nl = pack2(neg_l, neg_l), nd = pack2(neg_d, neg_d);
+      // ds = p / sum (dp - delta); a row that sees one key alone: dp times nothing, which is nothing unless dp is not finite
       const bool single = win_single(w, l, t.keys);
+      const float inv = single ? 0.f : ex2(neg_l), off_d = single ? 0.f : neg_d * inv;
+      const uint64_t nm = pack2(neg_m, neg_m), inv2 = pack2(inv, inv), off_d2 = pack2(off_d, off_d);
       float left_sum = 0.f, right_sum = 0.f;
       for (int i = 0; i < n; ++i) {
         const int s0 = t.own.at(i) * kWtTile, low = s0 - l0 - (kWtTile - 1);
@@ -315,8 +319,8 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         float flat = 0.f;
         const float* bias = nullptr;
         const uint8_t* bucket = nullptr;
-        const bool whole = view.whole(s0), in_left = biased && tail.is_left(low + 2 * (kWtTile - 1));
-        if (biased) {
+        const bool whole = view.whole(s0), in_left = BIASED && tail.is_left(low + 2 * (kWtTile - 1));
+        if constexpr (BIASED) {
           if (in_left) {
             flat = tail.left;
           } else if (tail.is_right(w, low)) {
@@ -341,7 +345,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_row64<0>(tS, d);
         const uint64_t mul2_ = pack2(c2, c2);
         if (bias == nullptr && wt_apart(c2, flat)) {
-          const float off = (flat + neg_m) + neg_l;
+          const float off = flat + neg_m;
           const uint64_t off2_ = pack2(off, off);
 #pragma unroll
           for (int j = 0; j < 64; j += 2) {
@@ -355,45 +359,54 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int j = 0; j < 64; j += 2) {
             const uint64_t add = bias != nullptr ? pack2(bias[j], bias[j + 1]) : flat2_;
             float e0, e1;
-            unpack2(add2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add), nm), nl), e0, e1);
+            unpack2(add2(fma2(pack2(d[j], d[j + 1]), mul2_, add), nm), e0, e1);
             d[j] = ex2(e0); d[j + 1] = ex2(e1);
           }
         }
         ok = ok && wt_wait(dp_full, cur, p.status, 0x2000u);
         tc_fence_after();
-        {
-          float e[64];
-          tmem_row64<0>(tDP + lanes + half * 64, e);
-          if (!whole && __any_sync(0xffffffffu, single)) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) e[j] = single ? (e[j] - e[j]) - neg_d : e[j];     // plus neg_d: nothing, unless dp is not finite
-          }
-#pragma unroll
-          for (int j = 0; j < 64; j += 2) {
-            const uint64_t y = mul2(add2(pack2(e[j], e[j + 1]), nd), pack2(d[j], d[j + 1]));
-            unpack2(y, d[j], d[j + 1]);
-          }
-        }
+        float e[64];
+        tmem_row64<0>(tDP + lanes + half * 64, e);
+        uint32_t bits[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
         if (!whole) {
           const WtSeen seen(w, l, t.queries, s0, t.keys);
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t bits = seen.bits(half * 64 + q * 32);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) d[q * 32 + j] = bits >> j & 1u ? d[q * 32 + j] : 0.f;
-          }
+          bits[0] = seen.bits(half * 64);
+          bits[1] = seen.bits(half * 64 + 32);
         }
         {
           uint32_t v[32];
+          const auto gradients = [&](auto masked) {                       // e: what the weights are multiplied with
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = pack_bf16(d[2 * j], d[2 * j + 1]);
+            for (int j = 0; j < 64; j += 2) {
+              const uint64_t f = fma2(pack2(e[j], e[j + 1]), inv2, off_d2);
+              float y0, y1;
+              unpack2(mul2(f, pack2(d[j], d[j + 1])), y0, y1);
+              unpack2(f, e[j], e[j + 1]);
+              if constexpr (decltype(masked)::value) {
+                y0 = bits[j >> 5] >> (j & 31) & 1u ? y0 : 0.f;
+                y1 = bits[j >> 5] >> ((j + 1) & 31) & 1u ? y1 : 0.f;
+              }
+              v[j >> 1] = pack_bf16(y0, y1);
+            }
+          };
+          if (whole) gradients(std::false_type{});
+          else gradients(std::true_type{});
           tmem_st32(tS, v);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_ready);
-        if (biased) {
+        if constexpr (BIASED) {                    // the table's share, of the weights that the forward pass used
+#pragma unroll
+          for (int j = 0; j < 64; j += 2) {
+            const uint32_t both = pack_bf16(d[j], d[j + 1]);
+            unpack2(mul2(pack2(e[j], e[j + 1]), pack2(__uint_as_float(both << 16), __uint_as_float(both & 0xFFFF0000u))), d[j], d[j + 1]);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) d[j] = bits[j >> 5] >> (j & 31) & 1u ? d[j] : 0.f;
+          }
           if (bucket == nullptr) {
             float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -405,7 +418,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       done += (uint32_t)n;
-      if (biased) {
+      if constexpr (BIASED) {
         const float a = warp_sum(left_sum), c = warp_sum(right_sum);
         if (lane == 0) {
           my_bsum[tail.left_bucket] += a;
@@ -865,7 +878,8 @@ int32_t win_tc_bwd(const WinParams& w, void* dq, void* dk, void* dv, float* part
   p.items = (int)(qt * w.H * w.B);
   p.wide_d = aligned_to(dq, 32) && w.D % 16 == 0;
   const int64_t steps = std::min<int64_t>(w.S, (int64_t)w.window + kWtTile) / kWtTile + 1, resident = wt_blocks(p.items, sm_count(), steps);
-  int32_t rc = one ? launch(win_tc_dq_kernel<1>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2>, WtBwd<2>::SMEM, qt, resident);
+  int32_t rc = w.buckets.count > 0 ? (one ? launch(win_tc_dq_kernel<1, true>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2, true>, WtBwd<2>::SMEM, qt, resident))
+                                    : (one ? launch(win_tc_dq_kernel<1, false>, WtBwd<1>::SMEM, qt, resident) : launch(win_tc_dq_kernel<2, false>, WtBwd<2>::SMEM, qt, resident));
   if (rc != LB2_OK) return rc;
   const int64_t blocks = (kt - p.sinks.tiles + (int64_t)p.sinks.tiles * p.sinks.splits) * w.Hkv * w.B;
   LB2_REQUIRE(blocks <= 0x7FFF0000, LB2_BAD_SHAPE, "too many rows");

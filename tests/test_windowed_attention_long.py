@@ -56,6 +56,70 @@ def close(got, ref, dt, D, E, terms, names=NAMES, where=None):
         assert float(err.norm()) <= lim, f"{name}: off by {float(err.norm()):.3e}, {float(err.norm()) / lim:.2f} times the limit"
 
 
+def inputs(seed, dt, D, E, H, Hkv, Lq, S, B, columns=0, device="cuda"):
+    """Julia arrays of the type, and the same values in 64 bits."""
+    g = torch.Generator().manual_seed(seed)
+    t = {}
+    for n, (f, h, tokens) in (("q", (D, H, Lq)), ("k", (D, Hkv, S)), ("v", (E, Hkv, S)), ("dx", (E, H, Lq))):
+        t[n] = torch.randn(B, tokens, h, f, generator=g).to(DT[dt]).to(device).permute(3, 2, 1, 0)
+    if columns:
+        t["table"] = torch.randn(columns, H, generator=g).to(DT[dt]).to(device).permute(1, 0)
+    return t, {n: x.double() for n, x in t.items()}
+
+
+def terms_of(H, Hkv, Lq, S, window, sinks, causal):
+    keys = min(S, (1 if causal else 2) * window + sinks)
+    queries = (H // Hkv) * (Lq if sinks else min(Lq, 2 * window))
+    return {"x": keys, "dq": keys, "dk": queries, "dv": queries, "dtable": 64 + 127 * (keys // 32 + 2)}
+
+
+def run(t, window, sinks, causal, buckets, lengths):
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    kw = dict(window=window, sinks=sinks, is_causal=causal, table=t.get("table"), buckets=buckets, lengths=lens)
+    x, pb = L.rrule_windowed_attention(t["q"], t["k"], t["v"], **kw)
+    got = dict(zip(NAMES, (x,) + pb(t["dx"])))
+    torch.cuda.synchronize()
+    assert _cabi.load().lb2_poll_device_status(L.arrays.current_stream(x.device)) == _cabi.OK
+    return got
+
+
+def reference(d, window, sinks, causal, buckets, lengths, **kw):
+    return R.attention(d["q"], d["k"], d["v"], d["dx"], window, sinks, causal, d.get("table"), buckets.first if buckets else None,
+                       bool(buckets and buckets.bidirectional), lengths, **kw)
+
+
+# ---- the table's gradient ------------------------------------------------------------------------
+# D, H, Hkv, B, L, S, window, sinks, causal, buckets, lengths: nearly all pairs of a row lie in one bucket, whose gradients cancel
+F4 = lambda top: L.RelativeBuckets.make(4, top, True)
+CANCEL = [
+    (128, 2, 1, 5, 127, 127, 129, 0, True, F4(6), None),
+    (64, 3, 1, 2, 1100, 1100, 246, 28, True, F4(10), [1100, 1]),
+    (32, 6, 3, 1, 820, 445, 129, 64, True, F4(5), None),
+    (80, 8, 2, 1, 300, 300, 64, 130, False, L.RelativeBuckets.make(8, 20, False), None),
+    (128, 4, 4, 1, 700, 700, 500, 0, True, L.RelativeBuckets((0, 700), False), None),     # one bucket holds all: nothing
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", CANCEL, ids=lambda c: "-".join(str(len(v) if hasattr(v, "__len__") else v) for v in c))
+def test_gradients_of_buckets_that_cancel(dt, case):
+    D, H, Hkv, B, T, S, window, sinks, causal, buckets, lengths = case
+    t, d = inputs(44, dt, D, D, H, Hkv, T, S, B, len(buckets))
+    got = run(t, window, sinks, causal, buckets, lengths)
+    close(got, reference(d, window, sinks, causal, buckets, lengths), dt, D, D, terms_of(H, Hkv, T, S, window, sinks, causal))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_a_table_gradient_without_one_diagonal_is_off_limits(dt):
+    """The limit by norm is narrow enough to miss a diagonal that a kernel forgets."""
+    _, d = inputs(45, dt, 64, 64, 2, 1, 300, 300, 1, len(B32C), device="cpu")
+    ref = reference(d, 64, 4, True, B32C, None)
+    for rel in (0, -5, -40, -63):
+        less = reference(d, 64, 4, True, B32C, None, without_diagonal=rel)
+        assert float((less["dtable"] - ref["dtable"]).norm()) > norm_limit(dt, "dtable", ref, 64, 64, terms_of(2, 1, 300, 300, 64, 4, True)["dtable"]), rel
+
+
 # ---- single tokens -------------------------------------------------------------------------------
 def step_inputs(seed, dt, D, E, H, Hkv, B, cap, columns):
     g = torch.Generator().manual_seed(seed)
