@@ -88,6 +88,77 @@ def reference(d, window, sinks, causal, buckets, lengths, **kw):
                        bool(buckets and buckets.bidirectional), lengths, **kw)
 
 
+# D, E, H, Hkv, B, L, window, sinks, causal, buckets, lengths: more tiles than twice the SMs, and no even number of them
+MANY = [
+    (64, 64, 32, 8, 2, 1300, 200, 5, True, B32C, None),
+    (128, 128, 32, 16, 1, 1300, 200, 5, True, B32C, None),
+    (64, 64, 15, 5, 6, 1100, 130, 0, False, B32, [1100, 0, 700, 1, 0, 129]),        # three heads on one, empty sequences between full ones
+    (128, 128, 15, 15, 3, 1300, 300, 1, False, B32, [1300, 0, 1290]),
+    (128, 128, 16, 8, 41, 70, 20, 2, False, B6, [70 - 7 * (i % 11) for i in range(41)]),   # many short sequences
+    (64, 64, 16, 8, 41, 70, 20, 0, True, B6, [70 - 7 * (i % 11) for i in range(41)]),
+    (96, 40, 24, 12, 3, 900, 260, 140, True, None, None),                         # sinks over more than a tile, shared by blocks
+    (64, 64, 16, 4, 1, 2600, 2500, 3, True, B32C, None),                          # long items, which SMs take as they come free
+    (128, 128, 16, 16, 1, 2600, 2500, 0, False, None, None),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(str(len(v) if hasattr(v, "__len__") else v) for v in c))
+def test_blocks_that_take_many_tiles(dt, case):
+    D, E, H, Hkv, B, T, window, sinks, causal, buckets, lengths = case
+    t, d = inputs(41, dt, D, E, H, Hkv, T, T, B, len(buckets) if buckets else 0)
+    got = run(t, window, sinks, causal, buckets, lengths)
+    close(got, reference(d, window, sinks, causal, buckets, lengths), dt, D, E, terms_of(H, Hkv, T, T, window, sinks, causal))
+    again = run(t, window, sinks, causal, buckets, lengths)
+    assert all(torch.equal(got[n], again[n]) for n in NAMES if got[n] is not None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_padding_that_is_not_finite_with_shared_sinks_and_many_tiles(dt, D, value):
+    """NaN or infinities past the lengths, in sink tiles that several blocks share and in blocks that take many tiles: as without them."""
+    H, Hkv, B, T, window, sinks, lengths = 32, 8, 2, 1300, 200, 5, [1300, 1130]
+    t, d = inputs(42, dt, D, D, H, Hkv, T, T, B, len(B32C))
+    ref = reference(d, window, sinks, True, B32C, lengths)
+    for n in ("q", "k", "v", "dx"):
+        t[n][..., lengths[1]:, 1] = value
+    got = run(t, window, sinks, True, B32C, lengths)
+    close(got, ref, dt, D, D, terms_of(H, Hkv, T, T, window, sinks, True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_sink_that_is_not_finite(dt, D):
+    """An infinite value in a sink of one key head, NaN in a late key of another: they reach the queries that see them and nothing else."""
+    H, Hkv, B, T, window, sinks = 32, 8, 2, 1300, 200, 5
+    rep = H // Hkv
+    t, d = inputs(43, dt, D, D, H, Hkv, T, T, B)
+    ref = reference(d, window, sinks, True, None, None)
+    t["v"][2, 3, 1, 0] = math.inf
+    t["k"][1, 7, 1250, 1] = math.nan
+    got = run(t, window, sinks, True, None, None)
+    of3, of7 = slice(3 * rep, 4 * rep), slice(7 * rep, 8 * rep)
+    inf = got["x"][2, of3, 1:, 0]
+    assert (inf == math.inf).all()                                       # all weights are positive
+    seers = R.sees(T, T, window, sinks, True, T, "cuda")[:, 1250]
+    assert torch.isnan(got["x"][:, of7, seers, 1]).all() and torch.isnan(got["dq"][:, of7, seers, 1]).all()
+    assert torch.isnan(got["dv"][:, 7, 1250, 1]).all() and torch.isnan(got["dk"][:, 7, 1250, 1]).all()
+    where = {n: torch.ones_like(ref[n], dtype=torch.bool) for n in NAMES if n in ref}
+    where["x"][2, of3, 1:, 0] = False
+    where["dq"][:, of3, 1:, 0] = False                                   # dp and dx . x are infinite; weights, and with them dv, are not
+    where["dk"][:, 3, :, 0] = False
+    seen = R.sees(T, T, window, sinks, True, T, "cuda")[seers].any(0)
+    where["x"][:, of7, seers, 1] = False
+    where["dq"][:, of7, seers, 1] = False
+    for n in ("dk", "dv"):
+        where[n][:, 7, seen, 1] = False
+    close(got, ref, dt, D, D, terms_of(H, Hkv, T, T, window, sinks, True), where=where)
+
+
 # ---- the table's gradient ------------------------------------------------------------------------
 # D, H, Hkv, B, L, S, window, sinks, causal, buckets, lengths: nearly all pairs of a row lie in one bucket, whose gradients cancel
 F4 = lambda top: L.RelativeBuckets.make(4, top, True)
