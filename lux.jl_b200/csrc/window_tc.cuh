@@ -26,11 +26,17 @@ inline bool wt_encode(CUtensorMap* map, const void* ptr, int64_t features, int64
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Blocks for `items`, each of about `steps` tiles: one per SM that takes its items in turn, or one per item, which the device hands out as
-// SMs come free. Taking them in turn saves some 3 us an item (start, first loads, last stores); the other way saves about half an
-// item (2 us a step) where they do not come out even. Measured at 16 heads on 4, 8192 tokens, 128 features, in turn and as they come:
-// forward, 3.5 items an SM of 9 steps 108 and 117 us, of 33 steps 270 and 237; dq, 6.9 items of 2 steps 50 and 71, of 33 steps 305
-// and 296 (the rule's side is the slower one by 3 %); dk dv, 1.7 items of 36 steps 168 and 171, of 132 steps 477 and 449.
+// Blocks for `items`: one per SM that takes its items in turn, or one per item, which the device hands out as SMs come free. Taking them
+// in turn saves some 3 us an item (start, first loads, last stores); the other way saves about half an item where they do not come out
+// even. `steps`: tiles of one window, though queries that look both ways see two: what does not come out even is that the first
+// tokens see fewer, and with two sides they see half as many, not one. Measured at 16 heads on 4, 8192 tokens, 128 features, in turn and
+// as they come, us, an asterisk at the side that the rule takes:
+//   window            512         1024        2048        4096      both ways  512         1024        2048        4096
+//   forward           76* 87      107* 116    167* 162    265 229*             107* 118    168* 172    266* 270    433 420*
+//   dq                78* 93      116* 127    187* 191    297* 286             114* 129    186* 198    299* 322    492* 511
+//   dk dv             100 104*    158 164*    276 282*    467 434*             157 161*    274 275*    464 464*    709 711*
+// With 2048 sinks and window 512, whose tiles `steps` leaves out: forward 195* 181, dq 219* 219, dk dv 305 281*; with 512 sinks 105* 114,
+// 115* 127, 164 170*. 16 heads of 64 features, 4096 tokens, both ways, window 1024: 71* 74, 82* 86, 108* 115; 2048: 105 111*, 125* 128, 165* 172.
 inline unsigned wt_blocks(int items, int sms, int64_t steps) { return (unsigned)(items <= sms || (int64_t)items * 7 > steps * sms ? std::min(items, sms) : items); }
 
 // Shared-memory descriptors of a tile of 128 tokens in boxes: features as the contraction (K-major: 32 bytes per step of 16, the
