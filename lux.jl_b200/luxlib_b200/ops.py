@@ -978,6 +978,14 @@ def _lengths(lengths):
     return as_colmajor((lengths.clamp(-1, 2 ** 31 - 1) if lengths.dtype == torch.int64 else lengths).to(torch.int32))
 
 
+def _check_lengths(shape, batch_shape):
+    """One number per sample: in the batch's shape, or in a vector; not in another order of its dimensions."""
+    drop = lambda dims: tuple(d for d in dims if d != 1)
+    Bn = math.prod(batch_shape)
+    if math.prod(shape) != Bn or drop(shape) not in (drop(batch_shape), drop((Bn,))):
+        raise DimensionMismatch(f"lengths must hold one number per sample {tuple(batch_shape)}, not {tuple(shape)}")
+
+
 def _number(scale):
     """A plain number: plans are kept by their arguments' values, and an array's may change."""
     return None if scale is None else float(scale)
@@ -998,8 +1006,8 @@ def _windowed_plan(q, k, v, window, sinks, is_causal, scale, table, buckets, len
     if Hkv == 0 or H % Hkv != 0:
         raise AssertionError("num_heads must be divisible by num_kv_groups")
     Bn = math.prod(batch_shape)
-    if lengths is not None and math.prod(lengths[0]) != Bn:
-        raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {math.prod(lengths[0])}")
+    if lengths is not None:
+        _check_lengths(lengths[0], batch_shape)
     _check_table(table, buckets, H)
     sc = 1.0 / (scale if scale is not None else float(D) ** 0.5)
     dims = _cabi.WindowDims(D, E, H, Hkv, Lq, S, Bn, window, sinks, int(is_causal))
@@ -1088,6 +1096,7 @@ def _step_plan(q, k, v, kcache, vcache, lengths, window, sinks, scale, table, bu
     Bn = math.prod(batch_shape)
     if lengths[2] != torch.int32 or math.prod(lengths[0]) != Bn:
         raise ArgumentError(f"lengths must hold one Int32 per sample ({Bn})")
+    _check_lengths(lengths[0], batch_shape)
     _check_table(table, buckets, H)
     sc = 1.0 / (scale if scale is not None else float(D) ** 0.5)
     dims = _cabi.WindowDims(D, E, H, Hkv, 1, kcache[0][2], Bn, window, sinks, 1)
@@ -1124,8 +1133,7 @@ def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
         raise DimensionMismatch("k, v and the caches must have the same heads, tokens and batch")
     Bn = math.prod(Kx.shape[3:])
     if lengths is not None:
-        if lengths.numel() != Bn:
-            raise DimensionMismatch(f"lengths must hold one number per sample ({Bn}), not {lengths.numel()}")
+        _check_lengths(tuple(lengths.shape), tuple(Kx.shape[3:]))
         lengths = _lengths(lengths)
     dims = _cabi.WindowDims(Kx.shape[0], V.shape[0], 0, Kx.shape[1], 0, Kx.shape[2], Bn, 1, int(sinks), 1)
     _launch(device, "lb2_window_cache_fill", ptr(kcache), ptr(vcache), ptr(Kx), ptr(V), ptr(lengths), kcache.shape[2], C.byref(dims),

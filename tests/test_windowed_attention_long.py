@@ -301,3 +301,29 @@ def test_a_step_without_query_heads_is_refused():
     step = lambda **kw: lib.lb2_window_attention_step(one, one, one, one, one, one, None, None, one, 0.125, _cabi.WindowDims(*dict(dict(
         head_dim=64, value_dim=64, heads=0, kv_heads=2, queries=1, keys=9, batch=3, window=4, sinks=1, causal=1), **kw).values()), 0, None)
     assert step() == _cabi.BAD_SHAPE and step(batch=0) == _cabi.OK and step(kv_heads=0) == _cabi.OK
+
+
+@pytest.mark.gpu
+def test_lengths_in_another_order_than_the_batch_are_refused():
+    """Two batch dimensions: lengths of their shape or a vector in its order, not the transposed shape, which holds as many numbers."""
+    z = lambda *s: L.jl_zeros(s, torch.float32, "cuda")
+    n = lambda *s: L.jl_zeros(s, torch.int32, "cuda")
+    q, c, one = z(8, 2, 4, 2, 3), z(8, 2, 5, 2, 3), z(8, 2, 2, 3)
+    calls = (lambda lens: L.windowed_attention(q, q, q, window=2, lengths=lens), lambda lens: L.windowed_cache_fill(c, c.clone(), q, q, lens),
+             lambda lens: L.windowed_attention_step(one, one, one, c, c.clone(), lens, window=2))
+    for call in calls:
+        call(n(2, 3)), call(n(6)), call(n(1, 2, 3))
+        for wrong in (n(3, 2), n(6, 1)[:5], n(2, 1, 3)[:1]):
+            with pytest.raises((L.DimensionMismatch, L.ArgumentError)):
+                call(wrong)
+    L.windowed_attention(q[..., :1], q[..., :1], q[..., :1], window=2, lengths=n(2))
+    L.windowed_attention(q[..., :1, :1], q[..., :1, :1], q[..., :1, :1], window=2, lengths=torch.tensor(3, dtype=torch.int32, device="cuda"))
+
+
+def test_shapes_of_lengths():
+    ok = lambda shape, batch: L.ops._check_lengths(shape, batch)
+    for shape, batch in (((2, 3), (2, 3)), ((6,), (2, 3)), ((), (1,)), ((1,), (1, 1)), ((4, 1), (4,)), ((0,), (0,)), ((0,), (0, 3)), ((0, 3), (0, 3))):
+        ok(shape, batch)
+    for shape, batch in (((3, 2), (2, 3)), ((5,), (2, 3)), ((), (2,)), ((2, 3), (6,)), ((0,), (2,)), ((3, 0), (0, 3))):
+        with pytest.raises(L.DimensionMismatch):
+            ok(shape, batch)
