@@ -763,7 +763,7 @@ def rrule_scaled_dot_product_attention(q, k, v, *, scale=None, mask=None, is_cau
     shared = None                # a bias per head that all samples share (relative_position_bias): its shape
     if bias is not None:
         bias_c = bias.to(Q.dtype)
-        if Bn > 1 and tuple(bias_c.shape) == (S, Lq, H) + (1,) * len(batch_shape):
+        if Bn != 1 and tuple(bias_c.shape) == (S, Lq, H) + (1,) * len(batch_shape):
             shared, bias_c = tuple(bias_c.shape), bias_c.expand((S, Lq, H) + batch_shape)
         bias_c = as_colmajor(bias_c)
         if tuple(bias_c.shape) == (S, Lq):

@@ -327,3 +327,17 @@ def test_shapes_of_lengths():
     for shape, batch in (((3, 2), (2, 3)), ((5,), (2, 3)), ((), (2,)), ((2, 3), (6,)), ((0,), (2,)), ((3, 0), (0, 3))):
         with pytest.raises(L.DimensionMismatch):
             ok(shape, batch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_a_bias_that_all_samples_share_where_there_are_none(dt):
+    """scaled_dot_product_attention takes relative_position_bias for a batch of nothing too; its gradient is a sum over nothing."""
+    table = L.jl_empty((2, len(B6)), DT[dt], "cuda").fill_(1.0)
+    e = lambda n: L.jl_empty((64, 2, n, 0), DT[dt], "cuda")
+    bias, pb_bias = L.rrule_relative_position_bias(table, B6, 5, 4)
+    (x, _), pb = L.rrule_scaled_dot_product_attention(e(4), e(5), e(5), bias=bias)
+    junk = torch.full((4096,), 7.0, device="cuda")                       # what the memory may hold
+    del junk
+    dbias = pb(x)[3]
+    assert tuple(x.shape) == (64, 2, 4, 0) and tuple(dbias.shape) == tuple(bias.shape) and not dbias.any() and not pb_bias(dbias).any()
