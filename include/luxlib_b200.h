@@ -399,7 +399,7 @@ LB2_API int32_t lb2_window_attention_step(void* x, void* kcache, void* vcache, c
                                           const void* table, const lb2_rel_buckets* buckets, const int32_t* lengths, double scale,
                                           const lb2_window_dims* dims, int32_t dtype, void* stream);
 /* Puts the tokens of k (head_dim, kv_heads, keys, batch) and v that a cache of `capacity` slots holds after lengths[b] of them (NULL: all
- * keys) into their slots; the other slots stay. No counterpart in the reference. */
+ * keys) into their slots; the other slots stay. k and v must not overlap the caches. No counterpart in the reference. */
 LB2_API int32_t lb2_window_cache_fill(void* kcache, void* vcache, const void* k, const void* v, const int32_t* lengths, int64_t capacity,
                                       const lb2_window_dims* dims, int32_t dtype, void* stream);
 

@@ -1077,6 +1077,18 @@ def _check_apart(kcache, vcache):
         raise ArgumentError("kcache and vcache must not share memory")
 
 
+def _check_prompt_apart(kcache, vcache, k, v):
+    """A prompt that lies in the caches' memory would be overwritten while it is read; where it begins with its cache and has the same
+    samples' stride, each token that is read is its own slot's or past the slots."""
+    def over(a, b):
+        return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+    for c, own, other in ((kcache, k, v), (vcache, v, k)):
+        aligned = own.data_ptr() == c.data_ptr() and (own.shape[2] == c.shape[2] or math.prod(own.shape[3:]) == 1)
+        if over(c, other) or (over(c, own) and not aligned):
+            raise ArgumentError("the tokens must not share memory with the caches")
+
+
 @functools.lru_cache(maxsize=4096)
 def _step_plan(q, k, v, kcache, vcache, lengths, window, sinks, scale, table, buckets):
     """The checks of a step, as _windowed_plan: (dims, scale, dtype code, device, output shape, whether all arrays are dense)."""
@@ -1122,7 +1134,8 @@ def windowed_attention_step(q, k, v, kcache, vcache, lengths, *, window: int, si
 
 def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     """Puts a prompt k (D, Hkv, S, B...), v (E, Hkv, S, B...) into the caches of windowed_attention_step, as if its tokens had come one by
-    one; `lengths` (B...) as in windowed_attention. The slots that hold none of them stay as they are."""
+    one; `lengths` (B...) as in windowed_attention. The slots that hold none of them stay as they are. The prompt does not lie in the caches'
+    memory, unless it begins with them."""
     _check_apart(kcache, vcache)
     device = _same_device(kcache=_meta(kcache), vcache=_meta(vcache), k=_meta(k), v=_meta(v), lengths=_meta(lengths))
     if k.dim() < 4 or v.dim() != k.dim():
@@ -1131,6 +1144,7 @@ def windowed_cache_fill(kcache, vcache, k, v, lengths=None, *, sinks: int = 0):
     Kx, V = as_colmajor(k), as_colmajor(v)
     if tuple(Kx.shape[1:]) != tuple(V.shape[1:]) or tuple(Kx.shape[3:]) != tuple(kcache.shape[3:]):
         raise DimensionMismatch("k, v and the caches must have the same heads, tokens and batch")
+    _check_prompt_apart(kcache, vcache, Kx, V)
     Bn = math.prod(Kx.shape[3:])
     if lengths is not None:
         _check_lengths(tuple(lengths.shape), tuple(Kx.shape[3:]))

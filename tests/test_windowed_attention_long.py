@@ -341,3 +341,30 @@ def test_a_bias_that_all_samples_share_where_there_are_none(dt):
     del junk
     dbias = pb(x)[3]
     assert tuple(x.shape) == (64, 2, 4, 0) and tuple(dbias.shape) == tuple(bias.shape) and not dbias.any() and not pb_bias(dbias).any()
+
+
+def test_a_prompt_in_the_memory_of_the_caches():
+    """Refused unless it begins with its own cache and their samples lie alike."""
+    flat = torch.arange(4000.0)
+    at = lambda first, tokens, batch=1: L.arrays.jl_reshape(flat[first:first + 4 * 2 * tokens * batch], (4, 2, tokens, batch))
+    check = L.ops._check_prompt_apart
+    check(at(0, 9), at(1000, 9), at(0, 20), at(1000, 20))                # the prompt's first tokens are the cache
+    check(at(0, 9, 2), at(1000, 9, 2), at(0, 9, 2), at(1000, 9, 2))
+    check(at(0, 9), at(1000, 9), at(72, 20), at(1072, 20))               # side by side
+    for kc, vc, k, v in ((at(0, 9), at(1000, 9), at(8, 20), at(2000, 20)), (at(0, 9), at(1000, 9), at(2000, 20), at(992, 20)),
+                         (at(0, 9), at(1000, 9), at(1000, 9), at(2000, 9)), (at(0, 9), at(1000, 9), at(2000, 9), at(0, 9)),
+                         (at(0, 9, 2), at(1000, 9, 2), at(0, 20, 2), at(2000, 20, 2))):
+        with pytest.raises(L.ArgumentError, match="share memory"):
+            check(kc, vc, k, v)
+
+
+@pytest.mark.gpu
+def test_a_cache_that_is_the_beginning_of_its_prompt():
+    g = torch.Generator().manual_seed(48)
+    k, v = (torch.randn(1, 23, 2, 4, generator=g).cuda().permute(3, 2, 1, 0) for _ in range(2))
+    kc, vc = L.jl_zeros((4, 2, 9, 1), torch.float32, "cuda"), L.jl_zeros((4, 2, 9, 1), torch.float32, "cuda")
+    L.windowed_cache_fill(kc, vc, k.clone(), v.clone(), sinks=2)
+    with pytest.raises(L.ArgumentError, match="share memory"):
+        L.windowed_cache_fill(k[:, :, 1:10], vc, k, v, sinks=2)
+    L.windowed_cache_fill(k[:, :, :9], v[:, :, :9], k, v, sinks=2)
+    assert torch.equal(k[:, :, :9], kc) and torch.equal(v[:, :, :9], vc)
