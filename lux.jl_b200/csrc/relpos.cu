@@ -57,9 +57,6 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
 // all in a fixed order. Measured: 16 heads of 1024 x 1024, 4 samples, bf16: 134 MB in 33 us (4.1 TB/s, 0.62 of the copy rate); the conversions
 // and sums of a value are five instructions.
 constexpr int kRelWarps = 4, kRelBwdRows = 32;    // 32 rows: blocks enough to even out over the SMs
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __restrict__ partial, const T* __restrict__ dbias,
                                                                     const __grid_constant__ lb2_rel_buckets t, int S, int L, int H, int B, int offset,
@@ -176,19 +173,6 @@ __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __res
     if (lane == 0) partial[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * H + h) * columns + j] = v;
   }
 }
-// dtable[h, bucket]: the blocks' sums, 64 bits, a warp per entry
-template <typename T>
-__global__ void __launch_bounds__(256) relpos_join_kernel(T* __restrict__ dtable, const float* __restrict__ partial, int H, int columns, int64_t n) {
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);     // h + H * bucket
-  if (i >= H * columns) return;
-  const int h = i % H, c = i / H;
-  double s = 0.0;
-  for (int64_t j = lane; j < n; j += 32) s += partial[(j * H + h) * columns + c];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) dtable[i] = from_f32<T>((float)s);
-}
-
 int rel_columns(const lb2_rel_buckets* t) { return t->count * (t->bidirectional ? 2 : 1); }
 int64_t rel_blocks(int64_t n, int64_t per) { return (n + per - 1) / per; }
 
@@ -260,7 +244,7 @@ int32_t lb2_relpos_bias_bwd(void* dtable, const void* dbias, const lb2_rel_bucke
       else launch(relpos_bwd_kernel<T, 1>, 32);
       LB2_CHECK_LAUNCH("relative position bias gradient");
     }
-    relpos_join_kernel<T><<<(unsigned)rel_blocks(H * columns, 8), 256, 0, st>>>((T*)dtable, partial, (int)H, columns, blocks);
+    win_dtable_kernel<T><<<(unsigned)rel_blocks(H * columns, 8), 256, 0, st>>>((T*)dtable, partial, (int)H, columns, blocks);
   });
   LB2_CHECK_LAUNCH("relative position bias gradient's sums");
   return LB2_OK;

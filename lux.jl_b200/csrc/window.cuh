@@ -84,6 +84,23 @@ template <typename T> __device__ __forceinline__ float win_bias(const WinParams&
   return win_bias2(to_f32(static_cast<const T*>(p.table)[h + (int64_t)p.H * win_bucket(p.buckets, first, rel)]));
 }
 
+// 16 bytes into shared memory, zeros in their place if not `real`
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool real = true) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+// dtable[h, bucket]: the blocks' sums [n][head][bucket], 64 bits, a warp per entry
+template <typename T>
+__global__ void __launch_bounds__(256) win_dtable_kernel(T* __restrict__ dtable, const float* __restrict__ partial, int H, int columns, int64_t n) {
+  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);     // h + H * bucket
+  if (i >= H * columns) return;
+  const int h = i % H, c = i / H;
+  double s = 0.0;
+  for (int64_t j = lane; j < n; j += 32) s += partial[(j * H + h) * columns + c];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane == 0) dtable[i] = from_f32<T>((float)s);
+}
+
 // The tiles of keys that hold sinks, and by how many blocks each is shared in dk, dv: a block walks no more tiles of queries than an
 // ordinary one or, if that is more, half an SM's share of the whole. 8192 tokens, 32 heads on 8, window 1024, 4 sinks: 4 blocks, 450 us
 // where one block for the sinks took 995.

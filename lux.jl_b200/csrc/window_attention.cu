@@ -32,26 +32,19 @@ __device__ __forceinline__ void win_load_tile(float* dst, const T* src, int64_t 
       for (int i = threadIdx.x; i < ROWS * quads; i += kWinThreads) {
         const int r = i / quads, c = (i - r * quads) * 4;
         const bool in = row0 + r < rows;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * LD + c)),
-                     "l"(src + (int64_t)(in ? row0 + r : 0) * stride + c), "r"(in ? 16 : 0)
-                     : "memory");
+        copy_async16(smem_u32(dst + r * LD + c), src + (int64_t)(in ? row0 + r : 0) * stride + c, in);
       }
-      return;
-    }
-    for (int i = threadIdx.x; i < ROWS * quads; i += kWinThreads) {
-      const int r = i / quads, c = (i - r * quads) * 4;
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row0 + r < rows) {
-        const T* at = src + (int64_t)(row0 + r) * stride + c;
-        if constexpr (sizeof(T) == 4) {
-          f = *reinterpret_cast<const float4*>(at);
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(at);
+    } else {
+      for (int i = threadIdx.x; i < ROWS * quads; i += kWinThreads) {
+        const int r = i / quads, c = (i - r * quads) * 4;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row0 + r < rows) {
+          const uint2 u = *reinterpret_cast<const uint2*>(src + (int64_t)(row0 + r) * stride + c);
           f = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
                           __uint_as_float(u.y & 0xFFFF0000u));
         }
+        *reinterpret_cast<float4*>(dst + r * LD + c) = f;
       }
-      *reinterpret_cast<float4*>(dst + r * LD + c) = f;
     }
   } else {
     for (int i = threadIdx.x; i < ROWS * n4; i += kWinThreads) {
@@ -395,19 +388,6 @@ __global__ void __launch_bounds__(kWinThreads, DP == 64 ? 2 : 1) win_dq_kernel(T
   __syncthreads();
   for (int r = threadIdx.x >> 5; r < BM; r += kWinThreads / 32)
     if (bad[r]) win_row_dq<T>(p, dq, dx, lb[l0 + r], db[l0 + r], l0 + r, h, b, keys);
-}
-
-// dtable[h, bucket] = sum over tiles and batch of the partial sums, 64 bits, a warp per entry
-template <typename T>
-__global__ void __launch_bounds__(256) win_dtable_kernel(T* __restrict__ dtable, const float* __restrict__ partial, int H, int columns, int64_t n) {
-  const int lane = threadIdx.x & 31, i = blockIdx.x * 8 + (threadIdx.x >> 5);     // h + H * bucket
-  if (i >= H * columns) return;
-  const int h = i % H, c = i / H;
-  double s = 0.0;
-  for (int64_t j = lane; j < n; j += 32) s += partial[(j * H + h) * columns + c];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (lane == 0) dtable[i] = from_f32<T>((float)s);
 }
 
 template <typename T, int DP>

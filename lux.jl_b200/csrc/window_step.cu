@@ -160,9 +160,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // Measured: 32 sequences of 1000 to 9000 tokens, 8 key heads of 128 features, 4 query heads each, window 4096: 455 MB in 93 us (4.9 TB/s, 0.75
 // of the copy rate); 133 us with the loads in registers. One sequence, window 1024: 10 us, start, two groups of keys and the join.
 constexpr int kStepStages = 3;
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
 template <int DC, int R> struct StepRing {
   static constexpr int HALF = 16 * DC * 2, STAGE = 2 * HALF, WARP = kStepStages * STAGE;      // 16 keys, then their 16 values
   static constexpr int BYTES = kStepWarps * WARP > (int)sizeof(StepJoin<R, DC, kStepWarps>) ? kStepWarps * WARP : (int)sizeof(StepJoin<R, DC, kStepWarps>);
