@@ -1080,13 +1080,15 @@ def _check_apart(kcache, vcache):
 def _check_prompt_apart(kcache, vcache, k, v):
     """A prompt that lies in the caches' memory would be overwritten while it is read; where it begins with its cache and has the same
     samples' stride, each token that is read is its own slot's or past the slots."""
-    def over(a, b):
-        return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+    kc, vc, ks, vs = kcache.data_ptr(), vcache.data_ptr(), k.data_ptr(), v.data_ptr()
+    kce, vce, ke, ve = kc + kcache.nbytes, vc + vcache.nbytes, ks + k.nbytes, vs + v.nbytes
+    if (kc < ke and ks < kce and not (kc == ks and _lie_alike(kcache, k))) or (vc < ve and vs < vce and not (vc == vs and _lie_alike(vcache, v))) or \
+            (kc < ve and vs < kce) or (vc < ke and ks < vce):
+        raise ArgumentError("the tokens must not share memory with the caches")
 
-    for c, own, other in ((kcache, k, v), (vcache, v, k)):
-        aligned = own.data_ptr() == c.data_ptr() and (own.shape[2] == c.shape[2] or math.prod(own.shape[3:]) == 1)
-        if over(c, other) or (over(c, own) and not aligned):
-            raise ArgumentError("the tokens must not share memory with the caches")
+
+def _lie_alike(cache, tokens):
+    return tokens.shape[2] == cache.shape[2] or math.prod(tokens.shape[3:]) == 1
 
 
 @functools.lru_cache(maxsize=4096)
