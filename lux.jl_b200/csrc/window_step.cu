@@ -157,7 +157,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // neighbouring ones of a key's row with one 16-byte load as its share of two steps; for V it joins two keys' rows by halves.
 // Each warp has its own ring of kStepStages groups of keys in shared memory, filled by asynchronous copies: what is in flight does not
 // depend on registers. 16-byte pieces are swizzled by row so that the fragments' loads meet no bank twice.
-// Measured: 32 sequences of 1000 to 9000 tokens, 8 key heads of 128 features, 4 query heads each, window 4096: 455 MB in 93 us (4.9 TB/s, 0.75
+// Measured: 32 sequences of 1000 to 9000 tokens, 8 key heads of 128 features, 4 query heads each, window 4096: 455 MB in 91 us (5.0 TB/s, 0.77
 // of the copy rate); 133 us with the loads in registers. One sequence, window 1024: 10 us, start, two groups of keys and the join.
 constexpr int kStepStages = 3;
 template <int DC, int R> struct StepRing {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
   const uint32_t ring = smem_u32(raw) + warp * Ring::WARP;
   const int piece = lane % CPR, first_row = lane / CPR;
   const bool kreal = piece * 8 < p.D, vreal = piece * 8 < p.E;
-  // 16 keys from i0 on; past the end the last key once more, which weighs nothing there, and zeros for its value, which may be infinite
+  // 16 keys from i0 on; past the end the last key once more, which does not count there
   auto fetch = [&](int i0, int stage) {
     if (i0 < to) {
 #pragma unroll
@@ -201,8 +201,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
         const int64_t slot = keys.slot(i);
         const uint32_t at = ring + stage * Ring::STAGE + row * (DC * 2);
         copy_async16(at + ((piece ^ ((row & 1) << 2)) * 16), (fresh ? kn : kc + slot * ks) + (kreal ? piece * 8 : 0), kreal);
-        copy_async16(at + Ring::HALF + ((piece ^ (row & 6)) * 16), (fresh ? vn : vc + slot * vs) + (vreal ? piece * 8 : 0),
-                     vreal && i0 + row < to);
+        copy_async16(at + Ring::HALF + ((piece ^ (row & 6)) * 16), (fresh ? vn : vc + slot * vs) + (vreal ? piece * 8 : 0), vreal);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -231,7 +230,9 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
 #pragma unroll
   for (int x = 0; x < kStepStages - 1; ++x) fetch(begin + x * kStepWarps * 16, x);
   int stage = 0;
-  for (int i0 = begin; i0 < to; i0 += kStepWarps * 16) {
+  int i0 = begin;
+  const auto group = [&](auto ends) {              // ends: some of the 16 keys are past the end
+    constexpr bool ENDS = decltype(ends)::value;
     asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 2) : "memory");
     __syncwarp();
     fetch(i0 + (kStepStages - 1) * kStepWarps * 16, stage == 0 ? kStepStages - 1 : stage - 1);      // over what was read last
@@ -256,12 +257,12 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int i = i0 + (k >> 1) * 8 + 2 * t + (k & 1);
-      const int bk = p.buckets.count > 0 && i < to ? win_bucket(p.buckets, first_of, -keys.distance(i, w.n)) : 0;
+      const int bk = p.buckets.count > 0 && (!ENDS || i < to) ? win_bucket(p.buckets, first_of, -keys.distance(i, w.n)) : 0;
 #pragma unroll
       for (int a = 0; a < R / 8; ++a) {
         float v = s[k >> 1][2 * a + (k & 1)] * p.scale2;
         if (p.buckets.count > 0 && u + 8 * a < w.heads) v += head_bias[u + 8 * a][bk];
-        z[a][k] = i < to ? v : -INFINITY;
+        z[a][k] = !ENDS || i < to ? v : -INFINITY;
         top[a] = fmaxf(top[a], z[a][k]);
       }
     }
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
       for (int r = 0; r < 4; ++r) {
         const int row = (r >> 1) * 8 + 2 * t + (r & 1);
         vv[r] = *reinterpret_cast<const uint4*>(at + Ring::HALF + row * (DC * 2) + (((c * 8 + u) ^ (row & 6)) * 16));
+        if (ENDS && i0 + row >= to) vv[r] = zero;  // nothing times an infinite value is NaN
       }
       const uint32_t w0[4] = {vv[0].x, vv[0].y, vv[0].z, vv[0].w}, w1[4] = {vv[1].x, vv[1].y, vv[1].z, vv[1].w};
       const uint32_t w2[4] = {vv[2].x, vv[2].y, vv[2].z, vv[2].w}, w3[4] = {vv[3].x, vv[3].y, vv[3].z, vv[3].w};
@@ -315,7 +317,9 @@ __global__ void __launch_bounds__(kStepThreads) win_step_bf16_kernel(const __gri
       }
     }
     __syncwarp();                                  // all have read the stage before it is filled again
-  }
+  };
+  for (; i0 + 16 <= to; i0 += kStepWarps * 16) group(std::false_type{});
+  if (i0 < to) group(std::true_type{});
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();                                 // the ring's memory becomes the join's
   auto& j = *reinterpret_cast<StepJoin<R, DC, kStepWarps>*>(raw);
