@@ -292,11 +292,12 @@ __global__ void __launch_bounds__(256) win_delta_kernel(float* __restrict__ delt
   }
 }
 
-// dq, and partial[tile][batch][head][bucket] of dtable
+// dq, and partial[tile][batch][head][bucket] of dtable. `rounded`: the forward pass with a table ran on the tensor cores, over the sum of
+// weights rounded to bf16; the gradients of a row add up to nothing with those alone.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kWinThreads, DP == 64 ? 2 : 1) win_dq_kernel(T* __restrict__ dq, float* __restrict__ partial, const T* __restrict__ dx,
                                                              const float2* __restrict__ stats, const float* __restrict__ delta,
-                                                             const __grid_constant__ WinParams p, int tiles, int vecq, int vecv) {
+                                                             const __grid_constant__ WinParams p, int tiles, int vecq, int vecv, int rounded) {
   using C = WinTile<DP>;
   constexpr int BM = C::BM, TM = C::TM, LD = C::LD, LDP = C::LDP, NC = C::NC;
   extern __shared__ __align__(16) float sm[];
@@ -349,7 +350,12 @@ __global__ void __launch_bounds__(kWinThreads, DP == 64 ? 2 : 1) win_dq_kernel(T
         const int r = ty + 16 * i, c = tx + 16 * j, l = l0 + r, s = s0 + c;
         float u = z[i][j] * p.scale2;
         if (p.buckets.count > 0) u += sD[r - c + BM - 1];
-        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? exp2f((u - ls[i].x) - ls[i].y) * (dp[i][j] - (single[i] ? dp[i][j] : de[i])) : 0.f;
+        const auto weight = [&] {
+          if constexpr (sizeof(T) == 2)
+            if (rounded) return __bfloat162float(__float2bfloat16_rn(exp2f(u - ls[i].x))) * exp2f(-ls[i].y);
+          return exp2f((u - ls[i].x) - ls[i].y);
+        };
+        sP[r * LDP + c] = l < queries && s < keys && win_sees(p, l, s) ? weight() * (dp[i][j] - (single[i] ? dp[i][j] : de[i])) : 0.f;
       }
     if (p.buckets.count > 0) {          // sums along the diagonals, then those of a bucket, each in order
       __syncthreads();
@@ -686,9 +692,9 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
   const int64_t qt = win_tiles(d->queries, tile), kt = win_tiles(d->keys, tile);
   LB2_REQUIRE(qt * d->heads * d->batch <= 0x7FFFFFFF && kt * d->kv_heads * d->batch <= 0x7FFFFFFF && (rows + 7) / 8 <= 0x7FFFFFFF, LB2_BAD_SHAPE,
               "too many rows");
-  if (win_tc_serves(d, dtype) && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16) && aligned_to(x, 16) && aligned_to(x_rest, 16) &&
-      aligned_to(q, 16) &&
-      aligned_to(k, 16) && aligned_to(v, 16)) {
+  const bool tc = win_tc_serves(d, dtype) && aligned_to(x, 16) && aligned_to(x_rest, 16) && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(v, 16);
+  const int rounded = tc && columns > 0;                                         // as the forward pass decided
+  if (tc && aligned_to(dq, 16) && aligned_to(dk, 16) && aligned_to(dv, 16) && aligned_to(dx, 16)) {
     float* constants = sink_sums + win_sink_bytes(d, dtype) / sizeof(float);
     rc = win_tc_bwd(p, dq, dk, dv, partial, sink_sums, constants, dx, x, x_rest, reinterpret_cast<const float2*>(stats), delta, st);
     if (rc != LB2_OK || columns == 0) return rc;
@@ -702,7 +708,7 @@ int32_t lb2_window_attention_bwd(void* dq, void* dk, void* dv, void* dtable, con
       if ((rc = win_delta(delta, (const T*)dx, (const T*)x, (const T*)x_rest, p, rows, st)) != LB2_OK) return rc;
       if ((rc = win_smem(win_dq_kernel<T, DP>, C::DQ_BYTES)) != LB2_OK) return rc;
       win_dq_kernel<T, DP><<<(unsigned)(qt * d->heads * d->batch), kWinThreads, C::DQ_BYTES, st>>>((T*)dq, partial, (const T*)dx, (const float2*)stats, delta, p, (int)qt,
-                                                                                                   vecq, vecv);
+                                                                                                   vecq, vecv, rounded);
       LB2_CHECK_LAUNCH("windowed attention dq");
     }
     if (columns > 0) {

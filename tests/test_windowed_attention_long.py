@@ -181,6 +181,21 @@ def test_gradients_of_buckets_that_cancel(dt, case):
     close(got, reference(d, window, sinks, causal, buckets, lengths), dt, D, D, terms_of(H, Hkv, T, S, window, sinks, causal))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", CANCEL, ids=lambda c: "-".join(str(len(v) if hasattr(v, "__len__") else v) for v in c))
+def test_gradients_of_buckets_that_cancel_from_a_cotangent_off_its_alignment(dt, case):
+    """Whichever kernels the pullback takes: with the weights of the forward pass, which the cotangent's address does not change."""
+    D, H, Hkv, B, T, S, window, sinks, causal, buckets, lengths = case
+    t, d = inputs(49, dt, D, D, H, Hkv, T, S, B, len(buckets))
+    flat = torch.zeros(t["dx"].numel() + 1, dtype=DT[dt], device="cuda")
+    dx = torch.as_strided(flat, t["dx"].shape, t["dx"].stride(), 1)
+    dx.copy_(t["dx"])
+    assert L.is_colmajor(dx) and dx.data_ptr() % 16
+    got = run(dict(t, dx=dx), window, sinks, causal, buckets, lengths)
+    close(got, reference(d, window, sinks, causal, buckets, lengths), dt, D, D, terms_of(H, Hkv, T, S, window, sinks, causal))
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_a_table_gradient_without_one_diagonal_is_off_limits(dt):
     """The limit by norm is narrow enough to miss a diagonal that a kernel forgets."""
