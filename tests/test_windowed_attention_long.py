@@ -117,6 +117,24 @@ def test_blocks_that_take_many_tiles(dt, case):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("buckets", [None, B32C], ids=["plain", "bias"])
+@pytest.mark.parametrize("rising", [True, False])
+def test_rows_whose_maximum_moves_from_tile_to_tile(dt, D, buckets, rising):
+    """Logits that rise (or fall) by some 2^10 a tile: sums and accumulators are scaled again at every tile, or never."""
+    H, Hkv, T, window, sinks = 6, 3, 700, 500, 2
+    t, _ = inputs(50, dt, D, D, H, Hkv, T, T, 1, len(buckets) if buckets else 0)
+    ramp = torch.linspace(0.0, 5.0, T, device="cuda")
+    ramp = ramp if rising else ramp.flip(0)
+    t["k"] = L.as_colmajor((t["k"].float() * 0.5 + ramp[None, None, :, None]).to(DT[dt]))
+    t["q"] = L.as_colmajor((t["q"].float() * 0.5 + 60.0 / (7.0 * math.sqrt(D))).to(DT[dt]))      # times D / sqrt(D) and 5 / 700 a key
+    got = run(t, window, sinks, True, buckets, None)
+    ref = reference({n: x.double() for n, x in t.items()}, window, sinks, True, buckets, None)
+    close(got, ref, dt, D, D, terms_of(H, Hkv, T, T, window, sinks, True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_padding_that_is_not_finite_with_shared_sinks_and_many_tiles(dt, D, value):
     """NaN or infinities past the lengths, in sink tiles that several blocks share and in blocks that take many tiles: as without them."""
