@@ -134,6 +134,46 @@ def test_rows_whose_maximum_moves_from_tile_to_tile(dt, D, buckets, rising):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_calls_at_once_from_threads_on_their_own_streams(dt):
+    """Forward, pullback, fill and step of three threads at the same time give what they give alone."""
+    import threading
+
+    def work(t, steps):
+        x, pb = L.rrule_windowed_attention(t["q"], t["k"], t["v"], window=150, sinks=3, table=t["table"], buckets=B32C)
+        out = [x, *pb(t["dx"])]
+        kc, vc = (L.jl_zeros((64, 4, 200, 2), DT[dt], "cuda") for _ in range(2))
+        L.windowed_cache_fill(kc, vc, t["k"], t["v"], sinks=3)
+        lens = torch.full((2,), 600, dtype=torch.int32, device="cuda")
+        for i in range(steps):
+            out.append(L.windowed_attention_step(t["q"][:, :, i], t["k"][:, :, i], t["v"][:, :, i], kc, vc, lens, window=150, sinks=3))
+            lens += 1
+        return out + [kc, vc]
+
+    sets = [inputs(51 + i, dt, 64, 64, 8, 4, 600, 600, 2, len(B32C))[0] for i in range(3)]
+    alone = [work(t, 5) for t in sets]
+    torch.cuda.synchronize()
+    results, errors = [[] for _ in sets], []
+
+    def run_one(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(4):
+                    results[i].append(work(sets[i], 5))
+            stream.synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=run_one, args=(i,)) for i in range(3)]
+    [th.start() for th in threads], [th.join() for th in threads]
+    assert not errors
+    for want, got in zip(alone, results):
+        assert all(torch.equal(a, b) for once in got for a, b in zip(want, once))
+    assert _cabi.load().lb2_poll_device_status(None) == _cabi.OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_padding_that_is_not_finite_with_shared_sinks_and_many_tiles(dt, D, value):
