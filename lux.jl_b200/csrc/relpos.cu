@@ -20,7 +20,7 @@ constexpr int kRelRows = 64;      // queries per block
 
 // Forward: a block writes kRelRows x kRelKeys values of a head, all from the kRelRows + kRelKeys - 1 diagonals that it works out once.
 // Shared memory holds the diagonals once per alignment (copy r starts at diagonal r), so that a 16-byte store of neighbouring keys is
-// one aligned 16-byte load whatever the row. Bounded by the stores: 16 heads of 1024 x 1024 bf16, 33.5 MB in 9.4 us (3.6 TB/s).
+// one aligned 16-byte load whatever the row. Bounded by the stores: 16 heads of 1024 x 1024 bf16, 33.5 MB in 9.6 us (3.5 TB/s).
 constexpr int kRelKeys = 1024;
 template <typename T>
 __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, const T* __restrict__ table, const __grid_constant__ lb2_rel_buckets t,
@@ -54,8 +54,9 @@ __global__ void __launch_bounds__(256) relpos_fwd_kernel(T* __restrict__ bias, c
 // Backward: a warp takes 32 V neighbouring keys (V per lane, one load) of V queries at a time. A lane's V x V values lie on 2 V - 1
 // diagonals; V of them, complete for this lane, are the next lane's upper ones in the next V queries: they move there with
 // a shuffle, and out of lane 31 to the warp's sums in shared memory. The block joins its warps, then diagonals by bucket;
-// all in a fixed order. Measured: 16 heads of 1024 x 1024, 4 samples, bf16: 134 MB in 33 us (4.1 TB/s, 0.62 of the copy rate); the conversions
-// and sums of a value are five instructions.
+// all in a fixed order. Measured: 16 heads of 1024 x 1024, 4 samples, bf16: 134 MB in 33.6 us (4.0 TB/s, 0.61 of the copy rate); the conversions
+// and sums of a value are five instructions. A diagonal's 32 rows (and all samples of a warp) are summed in fp32, the blocks' sums in
+// 64 bits: 197 x 197 Float32 values are off by 9e-8 where 64 bits throughout leave 2.4e-8, the result's own rounding.
 constexpr int kRelWarps = 4, kRelBwdRows = 32;    // 32 rows: blocks enough to even out over the SMs
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kRelWarps) relpos_bwd_kernel(float* __restrict__ partial, const T* __restrict__ dbias,

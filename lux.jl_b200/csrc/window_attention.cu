@@ -10,8 +10,9 @@
 //
 // This file: the CUDA-core kernels, which serve Float32 and every feature count up to 256, and the entry points (window_tc.cu,
 // window_tc_bwd.cu: the tensor-core kernels of BFloat16 with up to 128 features in whole 16-byte vectors). Measured, Float32, 4 x 8 heads of
-// 64 features, 1024 tokens, window 256, 4 sinks, bias: forward 127 us, dq 206, dk dv 207 + 6; 17 TFLOP/s of the tiles' products, a quarter of
-// the CUDA cores' rate. What bounds them: two blocks per SM (registers, shared memory) and 512 equal blocks, 1.7 rounds.
+// 64 features, 1024 tokens, window 256, 4 sinks, bias: forward 126 us, dq 206, dk dv 202 + 6; 17 TFLOP/s of the tiles' products, a quarter of
+// the CUDA cores' rate. What bounds them: two blocks per SM (registers, shared memory) and 512 equal blocks, 1.7 rounds. BFloat16, the same tokens
+// and heads: 36 features forward 104 us, pullback 304; 192 features 400 and 1473 (32 x 32 tiles).
 #include "common.cuh"
 #include "window_tc.cuh"
 

@@ -12,12 +12,12 @@
 // Blocks stay on their SM and take pairs of tiles in turn: the next pair's Q and keys are loaded, and its first logits formed, while
 // the groups finish and store this one's.
 //
-// Measured: 32 heads on 8, 128 features, 16384 tokens, window 4096: 1.06 ms, 909 TFLOP/s of the visible pairs (0.55 of the GEMM rate);
-// 8192 tokens, window 1024, bias: 226 us. What bounds it: a group's chain per tile, 3780 cycles by the SM's clock: from its signal to
+// Measured: 32 heads on 8, 128 features, 16384 tokens, window 4096: 0.93 ms by itself, 1031 TFLOP/s of the visible pairs (0.63 of the GEMM
+// rate), 1.05 ms where calls follow one another under the power limit; 8192 tokens, window 1024, bias: 217 us. What bounds it: a group's chain per tile, 3780 cycles by the SM's clock: from its signal to
 // the next logits 1600 (1024 of MMA time at full rate; S from shared memory takes all of its 128 bytes per cycle), reading S 140,
 // maximum 560, exponentials 1370 (the 16 per cycle and SM), storing 130; the other group's fills the same time.
 // A third of the chain would go if the next S were formed during the softmax, but 512 TMEM columns hold two S and two O and no more;
-// 64 keys at a time with two S each were slower (303 against 262 us at 8192 tokens, 16 heads, window 4096; the kernel as it is takes 237): S at N = 64 is bound by its shared-memory reads.
+// 64 keys at a time with two S each were slower (303 against 262 us at 8192 tokens, 16 heads, window 4096; the kernel as it is takes 229): S at N = 64 is bound by its shared-memory reads.
 //
 // TMEM columns: S0 | S1 | O0 | O1, 128 each. Shared memory: both tiles of Q, a ring of key and value tiles in turn.
 #include "common.cuh"

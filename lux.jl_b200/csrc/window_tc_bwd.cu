@@ -13,7 +13,7 @@
 // and not what rounding leaves (2 samples of 1100 tokens, window 246, four buckets: error 0.0087 -> 0.0028 of the gradient; all in one
 // bucket: 40 times what dx . x rounds to -> a fifth of it). dq takes 8 % longer for it.
 //
-// Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 42 us (201 MB), dq 312 us, dk dv 356 us.
+// Measured: 32 heads on 8, 128 features, 8192 tokens, window 1024, 4 sinks, bias: rows' constants 43 us (201 MB), dq 313 us, dk dv 331 us.
 // What bounds them: in dq a tile's chain through the softmax warps (weights 1140 cycles, their gradients 650, the signals and waits between
 // 700) and at 128 features the values, whose one place in shared memory is free only after the product before; in dk dv, whose four
 // accumulators leave TMEM no second S, weights and products take turns, and the products and loads take 2300 cycles a tile of
@@ -255,7 +255,7 @@ win_tc_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (i == 0 && !mbar_wait_uniform(o_empty, (turn & 1u) ^ 1u, p.status, 0x40u)) { ok = false; break; }
             tc_fence_after();
           }
-          // 128 features wait for their one tile of values here: the product with the finished tile first (361 -> 303 us at window 4096)
+          // 128 features wait for their one tile of values here: the product with the finished tile first (361 -> 303 us at window 4096; 297 as the kernel is now)
           const auto product_dq = [&] {
             if (i < 0) return;
             if (elect_one()) {
