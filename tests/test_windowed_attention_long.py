@@ -17,7 +17,7 @@ import torch
 import luxlib_b200 as L
 from luxlib_b200 import _cabi
 import window_reference as R
-from test_windowed_attention import B6, B32, B32C, DT, U16, U32
+from test_windowed_attention import B6, B32, B32C, CASES, DT, U16, U32
 
 NAMES = ("x", "dq", "dk", "dv", "dtable")
 
@@ -86,6 +86,17 @@ def run(t, window, sinks, causal, buckets, lengths):
 def reference(d, window, sinks, causal, buckets, lengths, **kw):
     return R.attention(d["q"], d["k"], d["v"], d["dx"], window, sinks, causal, d.get("table"), buckets.first if buckets else None,
                        bool(buckets and buckets.bidirectional), lengths, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(len(v) if hasattr(v, "first") else v) for v in c))
+def test_small_cases_by_norm(dt, case):
+    """The shapes of test_windowed_attention.py within the limit by norm, and element by element with each output's own number of terms."""
+    D, E, H, Hkv, T, S, B, window, sinks, causal, buckets, lengths = case
+    t, d = inputs(40, dt, D, E, H, Hkv, T, S, B, len(buckets) if buckets else 0)
+    got = run(t, window, sinks, causal, buckets, lengths)
+    close(got, reference(d, window, sinks, causal, buckets, lengths), dt, D, E, terms_of(H, Hkv, T, S, window, sinks, causal))
 
 
 # D, E, H, Hkv, B, L, window, sinks, causal, buckets, lengths: more tiles than twice the SMs, and no even number of them

@@ -55,7 +55,7 @@ def attention(q, k, v, dx, window, sinks=0, causal=True, table=None, first=None,
             p = torch.where(any_, torch.softmax(torch.where(m, z, -torch.inf), 1), 0.0).nan_to_num(0.0)
             x = p @ vv
             dp, delta = gg @ vv.T, (gg * x).sum(1, keepdim=True)
-            ds = p * (dp - delta)
+            ds = torch.where(m.sum(1, keepdim=True) == 1, 0.0, p * (dp - delta))      # one key alone: exactly nothing
             dm = p * (gg.abs() @ vv.abs().T + (gg.abs() * (p @ vv.abs())).sum(1, keepdim=True))
             put = lambda n, i, val, mag, sq: (out[n][:, i, :, b].add_(val.T), out[n + "_mag"][:, i, :, b].add_(mag.T),
                                               out[n + "_rms"][:, i, :, b].add_(sq.T))
